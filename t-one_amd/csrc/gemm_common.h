@@ -106,8 +106,8 @@ __device__ __forceinline__ void tile_epilogue_inv(const GemmArgs& p, f32x16 (&ac
         const int nl = wn * WTN + 64 * ip;                   // g rows nl..nl+31, u rows nl+32..nl+63
         float o[16];
         if (p.c_bf16) {
-          // bf16 output: v_exp_f32 / v_rcp_f32, value pairs (consecutive columns) as two-float vectors so the fused
-          // multiply-adds and products issue as v_pk_* with the scalar form's per-element roundings
+          // bf16 output: v_exp_f32 / v_rcp_f32, value pairs (consecutive columns) as two-float vectors; packed fp32
+          // instructions are off for the whole build, so each half is a scalar operation with the scalar form's rounding
           typedef float f32x2e __attribute__((ext_vector_type(2)));
           const f32x2e inv2 = {inv, inv};
 #pragma unroll
