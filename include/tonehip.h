@@ -162,6 +162,86 @@ double tone_session_kernel_us(const tone_session *s, const char *family, int64_t
 int tone_session_debug_stop(tone_session *s, int stage);
 int tone_session_debug_read(tone_session *s, const char *buffer, void *host_dst, int64_t bytes);
 
+/* ---- phrase operators -------------------------------------------------------------------------------
+ * What a server does with the logprob rows of a phrase once the model has answered: hold them in pages until the phrase
+ * ends (frames_*), ask what they say about given tokens (token_scores) and where and how likely a given text is
+ * (ctc_align).  Stateless: no session, every buffer the caller's, all tensors on `device`, asynchronous on `stream`; two
+ * calls may run at once as long as their outputs, workspaces and queues are different ones.  Nothing is allocated and
+ * nothing synchronizes, so every call can be captured into a graph (its arguments' contents are read at replay).
+ * Element types: */
+#define TONE_TYPE_FP32 0
+#define TONE_TYPE_FP16 1
+#define TONE_TYPE_BF16 2
+
+/* status bits of tone_frames_plan (device memory): 0, or the whole call changed nothing */
+#define TONE_FRAMES_NO_PAGES 1     /* more pages to take than were free before the call           */
+#define TONE_FRAMES_ROW_FULL 2     /* a stream would hold more than `width` pages                 */
+#define TONE_FRAMES_BAD_REQUEST 4  /* negative or decreasing counts, add > max_add, row ids       */
+#define TONE_FRAMES_BAD_QUEUE 8    /* the cursors describe no queue of n_pages pages              */
+
+/* Move `batch` streams from the frames [first, length) they hold to [max(first, keep), length + add), 0 <= keep <=
+ * length + add: pages of page_size frames that fall out go back to the free queue, missing ones come from it, in batch
+ * order.  Pages released by a call can be taken from the next call on.
+ *   table        int32 [n_rows][table_stride]  request b reads row rows_in[b] (entry j = page of frames
+ *                                              (first / page_size + j) page_size ...) and writes row rows_out[b] whole
+ *                                              (`width` entries, -1 behind the last page): ping-pong rows as
+ *                                              tone_session_run_rows, all named rows distinct
+ *   queue        int32 [n_pages]               free pages at [head, tail) modulo n_pages
+ *   cursors_in / _out  int64 [2]               head, tail before / after (distinct buffers)
+ *   first, length, keep, add  int32 [batch]
+ *   slots        int64 [batch][max_add]        page * page_size + offset of new frame length + j; -1 for j >= add and for
+ *                                              frames before keep
+ *   status       int32 [1]
+ * Indices are checked on the device: nothing outside the buffers is read or written whatever they hold. */
+int tone_frames_plan(int device, int32_t *table, int64_t table_stride, int n_rows, int width, int32_t *queue, int n_pages,
+                     int page_size, const int64_t *cursors_in, int64_t *cursors_out, const int32_t *rows_in,
+                     const int32_t *rows_out, const int32_t *first, const int32_t *length, const int32_t *keep,
+                     const int32_t *add, int batch, int64_t *slots, int max_add, int32_t *status, void *stream);
+
+/* Slots of the frames begin + j, j < count, of streams that hold frames from `first` on in table row `rows`:
+ * slots int64 [batch][max_count], -1 for j >= count, frames before `first` and pages outside the row or the pool. */
+int tone_frames_slots(int device, const int32_t *table, int64_t table_stride, int n_rows, int width, int n_pages, int page_size,
+                      const int32_t *rows, const int32_t *first, const int32_t *begin, const int32_t *count, int batch,
+                      int64_t *slots, int max_count, void *stream);
+
+/* pool row slots[i] = src row i (strides in elements; one rounding to the pool's type) for i < n; slots outside
+ * [0, pool_rows) are left out, pool rows that no slot names are left as they were.  Slots must be distinct. */
+int tone_frames_put(int device, const void *src, int src_type, int64_t src_stride, const int64_t *slots, int64_t n, int vocab,
+                    void *pool, int pool_type, int64_t pool_stride, int64_t pool_rows, void *stream);
+
+/* For row n of x (row rows[n] where `rows` is given), over `vocab` entries that need not be normalized:
+ *   logprob[n]   log probability of tokens[n]; rank[n] = entries above it (equal ones with a lower index count)
+ *   entropy[n]   in nats
+ *   top_logprob / top_ids [n][k]   the k best, equal values by the lowest index; k <= min(vocab, 64)
+ * A token outside [0, vocab) is none: logprob 0, rank -1.  A row outside [0, x_rows) is none: logprob 0, rank -1,
+ * entropy 0, top -inf / -1.  -inf entries have probability 0; a row of nothing else has log probabilities -inf and
+ * entropy 0.  A NaN or +inf in a row makes its floating outputs NaN and its rank and ids any values in range.
+ * tokens may be NULL (then logprob and rank are not written). */
+#define TONE_SCORES_MAX_K 64
+int64_t tone_token_scores_workspace(int64_t n, int vocab, int k);
+int tone_token_scores(int device, const void *x, int type, int64_t stride, int64_t x_rows, const int64_t *rows, int64_t n,
+                      int vocab, const int32_t *tokens, int k, float *logprob, float *entropy, int32_t *rank,
+                      float *top_logprob, int32_t *top_ids, void *workspace, int64_t workspace_bytes, void *stream);
+
+/* CTC alignment of tokens [batch][max_tokens] (token_lens of them) to frame_lens frames of log probabilities: frame (b, t)
+ * at b * batch_stride + t * stride of x, or row rows[b][t] of x [x_rows] where `rows` is given.
+ *   score  fp32 [batch]                 log probability of the best path; of equal ones the path that, looked at from
+ *                                       its end, stays before it moves by one and moves by one before it skips a blank,
+ *                                       and that ends in a blank
+ *   total  fp32 [batch] or NULL         log of the summed probability of all paths
+ *   labels int32 [batch][frames]        the best path's label per frame, `blank` or a token; -1 behind the last frame
+ *   spans  int32 [batch][max_tokens][2] each token's frames [begin, end); -1 behind the last token
+ * A sequence no path fits (more tokens and repeats than frames, a token outside the vocabulary or equal to `blank`, -inf
+ * on every path) has score and total -inf, labels and spans -1; no frames and no tokens score 0.  Entries that are NaN or
+ * infinite count as -inf, frames whose row is outside [0, x_rows) as -inf throughout.  Lengths are clamped to
+ * [0, frames] and [0, max_tokens]. */
+#define TONE_ALIGN_MAX_TOKENS 2047
+int64_t tone_ctc_align_workspace(int batch, int frames, int tokens);
+int tone_ctc_align(int device, const void *x, int type, int64_t stride, int64_t batch_stride, int64_t x_rows,
+                   const int64_t *rows, int batch, int frames, int vocab, int blank, const int32_t *tokens, int max_tokens,
+                   const int32_t *token_lens, const int32_t *frame_lens, float *score, float *total, int32_t *labels,
+                   int32_t *spans, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -41,6 +41,18 @@ SIGNATURES = {
     "tone_session_kernel_us": (_c_double, [_c_void_p, _c_char_p, ctypes.POINTER(_c_int64)]),
     "tone_session_debug_stop": (_c_int, [_c_void_p, _c_int]),
     "tone_session_debug_read": (_c_int, [_c_void_p, _c_char_p, _c_void_p, _c_int64]),
+    "tone_frames_plan": (_c_int, [_c_int, _c_void_p, _c_int64, _c_int, _c_int, _c_void_p, _c_int, _c_int] + [_c_void_p] * 8
+                         + [_c_int, _c_void_p, _c_int, _c_void_p, _c_void_p]),
+    "tone_frames_slots": (_c_int, [_c_int, _c_void_p, _c_int64, _c_int, _c_int, _c_int, _c_int] + [_c_void_p] * 4
+                          + [_c_int, _c_void_p, _c_int, _c_void_p]),
+    "tone_frames_put": (_c_int, [_c_int, _c_void_p, _c_int, _c_int64, _c_void_p, _c_int64, _c_int, _c_void_p, _c_int, _c_int64,
+                                 _c_int64, _c_void_p]),
+    "tone_token_scores_workspace": (_c_int64, [_c_int64, _c_int, _c_int]),
+    "tone_token_scores": (_c_int, [_c_int, _c_void_p, _c_int, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int, _c_void_p, _c_int]
+                          + [_c_void_p] * 6 + [_c_int64, _c_void_p]),
+    "tone_ctc_align_workspace": (_c_int64, [_c_int, _c_int, _c_int]),
+    "tone_ctc_align": (_c_int, [_c_int, _c_void_p, _c_int, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int, _c_int, _c_int, _c_int,
+                                _c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int64, _c_void_p]),
 }
 ABI_VERSION = 1
 

@@ -1086,6 +1086,11 @@ int run_common(tone_session* s, const int32_t* signal, StateRef sr, float* logp,
 }  // namespace
 
 // =============================================================================================
+// the entry points outside this file report through the same message (scoring.h)
+namespace tone {
+int set_error(int code, const std::string& msg) { return fail(code, msg); }
+}  // namespace tone
+
 extern "C" {
 
 int tone_abi_version(void) { return TONE_ABI_VERSION; }

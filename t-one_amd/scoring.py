@@ -1,0 +1,318 @@
+"""The phrase operators: frames held in pages, scores of given tokens, CTC alignment.
+
+The acoustic path answers with a row of log probabilities per 30 ms frame (``ToneSession.run*``).  The operators here work on
+those rows where they are, on the device, until the phrase they belong to has ended:
+
+* ``frames_plan`` / ``frames_slots`` -- page tables and slot maps from the streams' frame counts, ``frames_put`` -- a step's
+  rows written through such a map; :class:`FrameStore` keeps the buffers and the counts for them;
+* ``token_scores`` -- per row the log probability of a given token, its rank, the entropy, the k best tokens;
+* ``ctc_align`` -- the best path of given token sequences, each token's frames, the log probability of all paths.
+
+The functions are stateless (``include/tonehip.h`` has the exact definitions): they check types, shapes, strides and devices
+here, write new tensors (or the caller's buffers, where they are arguments), do not synchronize, and run on ``stream`` or the
+current stream of the tensors' device.  Contents are checked on the device: an index outside its range is left out or counts as
+"none", as documented per argument.  Every call can be captured into a graph.
+"""
+
+from __future__ import annotations
+
+from typing import NamedTuple, Optional, Sequence
+
+import numpy as np
+
+from . import _lib
+from . import config as C
+
+MAX_K = 64              # TONE_SCORES_MAX_K
+MAX_TOKENS = 2047       # TONE_ALIGN_MAX_TOKENS
+STATUS = {1: "out of pages", 2: "a stream's table row is full", 4: "bad request", 8: "bad queue cursors"}   # TONE_FRAMES_*
+
+
+def _torch():
+    import torch
+    return torch
+
+
+_types: dict = {}
+
+
+def _type(t, name: str) -> int:
+    if not _types:
+        torch = _torch()
+        _types.update({torch.float32: 0, torch.float16: 1, torch.bfloat16: 2})   # TONE_TYPE_*
+    try:
+        return _types[t.dtype]
+    except KeyError:
+        raise ValueError(f"{name} must be float32, float16 or bfloat16, got {t.dtype}") from None
+
+
+def _vector(t, name: str, dtype, n: int) -> None:
+    if t.dtype != dtype or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous ({n},) {dtype} tensor, got {tuple(t.shape)} {t.dtype}")
+
+
+def _device(first, *others):
+    """The common CUDA device of the tensors."""
+    dev = first.device
+    for t in others:
+        if t is not None and t.device != dev:
+            raise ValueError(f"tensors on different devices: {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise ValueError(f"tensors must be on a GPU, got {dev}")
+    return dev
+
+
+class _On:
+    """The stream of one call.  Outputs come from the allocator under that stream; where it is not the current one, the
+    inputs are marked as in use on it, so that they may be freed at once after the call."""
+
+    def __init__(self, dev, stream, *inputs):
+        torch = _torch()
+        cur = torch.cuda.current_stream(dev)
+        self._ctx = None
+        if stream is None or stream == cur:
+            self.raw = cur.cuda_stream
+            return
+        if stream.device != dev:
+            raise ValueError(f"stream on {stream.device}, tensors on {dev}")
+        self.raw = stream.cuda_stream
+        self._ctx = torch.cuda.stream(stream)
+        for t in inputs:
+            if t is not None:
+                t.record_stream(stream)
+
+    def __enter__(self):
+        if self._ctx is not None:
+            self._ctx.__enter__()
+        return self.raw
+
+    def __exit__(self, *exc):
+        if self._ctx is not None:
+            self._ctx.__exit__(*exc)
+        return False
+
+
+def _ptr(t) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+# --- pages ------------------------------------------------------------------------------------------------------------
+
+def _check_table(table, page_size: int, n_pages: int) -> None:
+    torch = _torch()
+    if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 \
+            or (table.shape[1] > 1 and table.stride(1) != 1) or table.stride(0) < table.shape[1]:
+        raise ValueError("table must be a (rows, width) int32 tensor with unit column stride")
+    if page_size < 1 or n_pages < 1 or table.shape[1] * page_size > 2 ** 31 - 1:
+        raise ValueError("page_size and n_pages must be positive and width * page_size below 2^31")
+
+
+def frames_plan(table, queue, cursors_in, cursors_out, rows_in, rows_out, first, length, keep, add, *, page_size: int,
+                max_add: int, slots=None, status=None, stream=None):
+    """Move streams from the frames [first, length) to [max(first, keep), length + add); returns (slots, status).
+
+    table int32 (rows, width): request b's pages are read from row rows_in[b] and written to row rows_out[b] (all rows
+    distinct); queue int32 (n_pages,) of free page ids with int64 (2,) cursors head, tail; the requests int32 (B,).
+    slots int64 (B, max_add): where each new frame goes, -1 for none.  status int32 (1,): 0, or a sum of the
+    ``STATUS`` bits and then nothing was taken, released or given a slot.  See ``tone_frames_plan`` (include/tonehip.h)."""
+    torch = _torch()
+    b = int(rows_in.shape[0]) if rows_in.dim() == 1 else -1
+    for t, name in ((rows_in, "rows_in"), (rows_out, "rows_out"), (first, "first"), (length, "length"), (keep, "keep"), (add, "add")):
+        _vector(t, name, torch.int32, b)
+    _vector(queue, "queue", torch.int32, queue.numel())
+    _vector(cursors_in, "cursors_in", torch.int64, 2)
+    _vector(cursors_out, "cursors_out", torch.int64, 2)
+    _check_table(table, page_size, queue.numel())
+    if max_add < 0:
+        raise ValueError(f"max_add must not be negative, got {max_add}")
+    if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (b, max_add) or not slots.is_contiguous()):
+        raise ValueError(f"slots must be a contiguous ({b}, {max_add}) int64 tensor")
+    if status is not None:
+        _vector(status, "status", torch.int32, 1)
+    if cursors_in.data_ptr() == cursors_out.data_ptr():
+        raise ValueError("cursors_out must not alias cursors_in")
+    ins = (table, queue, cursors_in, cursors_out, rows_in, rows_out, first, length, keep, add, slots, status)
+    dev = _device(*ins)
+    lib = _lib.load()
+    with _On(dev, stream, *ins) as st:
+        if slots is None:
+            slots = torch.empty((b, max_add), dtype=torch.int64, device=dev)
+        if status is None:
+            status = torch.empty(1, dtype=torch.int32, device=dev)
+        _lib.check(lib.tone_frames_plan(dev.index, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1],
+                                        queue.data_ptr(), queue.numel(), page_size, cursors_in.data_ptr(), cursors_out.data_ptr(),
+                                        rows_in.data_ptr(), rows_out.data_ptr(), first.data_ptr(), length.data_ptr(),
+                                        keep.data_ptr(), add.data_ptr(), b, slots.data_ptr(), max_add, status.data_ptr(), st),
+                   "tone_frames_plan")
+    return slots, status
+
+
+def frames_slots(table, rows, first, begin, count, *, page_size: int, n_pages: int, max_count: int, slots=None, stream=None):
+    """Slots int64 (B, max_count) of the frames begin[b] .. begin[b] + count[b] - 1 of the stream that holds frames from
+    first[b] on in table row rows[b]; -1 past the count, before ``first`` and where the row has no page."""
+    torch = _torch()
+    b = int(rows.shape[0]) if rows.dim() == 1 else -1
+    for t, name in ((rows, "rows"), (first, "first"), (begin, "begin"), (count, "count")):
+        _vector(t, name, torch.int32, b)
+    _check_table(table, page_size, n_pages)
+    if max_count < 0:
+        raise ValueError(f"max_count must not be negative, got {max_count}")
+    if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (b, max_count) or not slots.is_contiguous()):
+        raise ValueError(f"slots must be a contiguous ({b}, {max_count}) int64 tensor")
+    ins = (table, rows, first, begin, count, slots)
+    dev = _device(*ins)
+    lib = _lib.load()
+    with _On(dev, stream, *ins) as st:
+        if slots is None:
+            slots = torch.empty((b, max_count), dtype=torch.int64, device=dev)
+        _lib.check(lib.tone_frames_slots(dev.index, table.data_ptr(), table.stride(0), table.shape[0], table.shape[1], n_pages,
+                                         page_size, rows.data_ptr(), first.data_ptr(), begin.data_ptr(), count.data_ptr(), b,
+                                         slots.data_ptr(), max_count, st), "tone_frames_slots")
+    return slots
+
+
+def _rows_of(t, name: str):
+    """(tensor, row stride) of a (..., V) tensor whose leading dimensions are one run of equally spaced rows."""
+    if t.dim() < 2 or t.shape[-1] < 1:
+        raise ValueError(f"{name} must be (..., vocab), got {tuple(t.shape)}")
+    if t.shape[-1] > 1 and t.stride(-1) != 1:
+        raise ValueError(f"{name} must have unit stride along the vocabulary")
+    if t.dim() > 2:
+        step = t.stride(-2)
+        for d in range(t.dim() - 3, -1, -1):
+            if t.shape[d] > 1 and t.stride(d) != step * int(np.prod(t.shape[d + 1 : -1])):
+                raise ValueError(f"{name}'s leading dimensions must be one run of equally spaced rows")
+    return t.stride(-2) if t.shape[-2] > 1 or t.dim() > 2 else max(t.stride(-2), t.shape[-1])
+
+
+def frames_put(src, slots, pool, stream=None) -> None:
+    """pool[slots[i]] = row i of ``src`` (..., vocab), rounded once to the pool's type; slots int64 with one entry per row,
+    distinct, those outside the pool left out.  pool (n_rows, vocab) float32 / float16 / bfloat16."""
+    torch = _torch()
+    stype, ptype = _type(src, "src"), _type(pool, "pool")
+    sstride = _rows_of(src, "src")
+    if pool.dim() != 2 or pool.shape[1] != src.shape[-1] or (pool.shape[1] > 1 and pool.stride(1) != 1) \
+            or (pool.shape[0] > 1 and pool.stride(0) < pool.shape[1]):
+        raise ValueError(f"pool must be (rows, {src.shape[-1]}) with unit column stride, got {tuple(pool.shape)}")
+    n = src.numel() // src.shape[-1]
+    if slots.dtype != torch.int64 or slots.numel() != n or not slots.is_contiguous():
+        raise ValueError(f"slots must be {n} contiguous int64 entries, got {tuple(slots.shape)} {slots.dtype}")
+    if n > 1 and sstride < src.shape[-1]:
+        raise ValueError("src rows must not overlap")
+    dev = _device(src, slots, pool)
+    lib = _lib.load()
+    with _On(dev, stream, src, slots, pool) as st:
+        _lib.check(lib.tone_frames_put(dev.index, src.data_ptr(), stype, sstride, slots.data_ptr(), n, src.shape[-1],
+                                       pool.data_ptr(), ptype, max(pool.stride(0), pool.shape[1]), pool.shape[0], st),
+                   "tone_frames_put")
+
+
+# --- scores -----------------------------------------------------------------------------------------------------------
+
+class TokenScores(NamedTuple):
+    """Per row, shaped like ``tokens`` / ``rows`` / the leading dimensions of x (top_*: one dimension of k more)."""
+    logprob: Optional[object]       # float32; None without tokens
+    rank: Optional[object]          # int32; None without tokens
+    entropy: object                 # float32, nats
+    top_logprob: Optional[object]   # float32; None for k = 0
+    top_ids: Optional[object]       # int32; None for k = 0
+
+
+def token_scores(x, tokens=None, k: int = 0, rows=None, stream=None) -> TokenScores:
+    """What rows of logits or log probabilities (..., vocab) say: the log probability and rank of a given token, the entropy,
+    the ``k`` best tokens (equal values: lowest id first).
+
+    ``rows`` int64, any shape: row indices into x (n_rows, vocab), e.g. a slot map into a pool; an index outside is no row
+    (logprob 0, rank -1, entropy 0, top -inf / -1).  ``tokens`` int32, one per row; an id outside the vocabulary is no token
+    (logprob 0, rank -1).  -inf entries have probability 0.  k <= min(vocab, 64)."""
+    torch = _torch()
+    typ = _type(x, "x")
+    vocab = int(x.shape[-1]) if x.dim() >= 2 else 0
+    if rows is not None:
+        if x.dim() != 2:
+            raise ValueError(f"x must be (n_rows, vocab) with rows, got {tuple(x.shape)}")
+        if rows.dtype != torch.int64 or not rows.is_contiguous():
+            raise ValueError(f"rows must be a contiguous int64 tensor, got {rows.dtype}")
+    stride = _rows_of(x, "x")
+    shape = tuple(rows.shape) if rows is not None else tuple(x.shape[:-1])
+    x_rows = x.numel() // vocab
+    n = int(np.prod(shape, dtype=np.int64))
+    if tokens is not None and (tokens.dtype != torch.int32 or tuple(tokens.shape) != shape or not tokens.is_contiguous()):
+        raise ValueError(f"tokens must be a contiguous {shape} int32 tensor, got {tuple(tokens.shape)} {tokens.dtype}")
+    k = int(k)
+    if not 0 <= k <= min(vocab, MAX_K):
+        raise ValueError(f"k must be in 0 .. min(vocab, {MAX_K}), got {k}")
+    if x_rows > 1 and stride < vocab:
+        raise ValueError("x rows must not overlap")
+    dev = _device(x, tokens, rows)
+    lib = _lib.load()
+    with _On(dev, stream, x, tokens, rows) as st:
+        lp = rank = top = ids = None
+        entropy = torch.empty(shape, dtype=torch.float32, device=dev)
+        if tokens is not None:
+            lp = torch.empty(shape, dtype=torch.float32, device=dev)
+            rank = torch.empty(shape, dtype=torch.int32, device=dev)
+        if k:
+            top = torch.empty(shape + (k,), dtype=torch.float32, device=dev)
+            ids = torch.empty(shape + (k,), dtype=torch.int32, device=dev)
+        need = lib.tone_token_scores_workspace(n, vocab, k)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(lib.tone_token_scores(dev.index, x.data_ptr(), typ, stride, x_rows, _ptr(rows), n, vocab, _ptr(tokens), k,
+                                         _ptr(lp), entropy.data_ptr(), _ptr(rank), _ptr(top), _ptr(ids), _ptr(ws), need, st),
+                   "tone_token_scores")
+    return TokenScores(lp, rank, entropy, top, ids)
+
+
+# --- alignment --------------------------------------------------------------------------------------------------------
+
+class CtcAlignment(NamedTuple):
+    score: object               # float32 (B,): log probability of the best path
+    total: Optional[object]     # float32 (B,): of all paths; None unless asked for
+    labels: object              # int32 (B, T): the best path's label per frame, -1 behind the last frame
+    spans: object               # int32 (B, L, 2): each token's frames [begin, end), -1 behind the last token
+
+
+def ctc_align(x, tokens, token_lens, frame_lens, rows=None, blank: int = C.BLANK_ID, total: bool = False,
+              stream=None) -> CtcAlignment:
+    """Align token sequences with frames of log probabilities.
+
+    x (B, T, vocab), batch and frame strides free (an expanded batch shares its frames), or with ``rows`` int64 (B, T) a pool
+    (n_rows, vocab) read through that slot map.  tokens int32 (B, L), token_lens / frame_lens int32 (B,), clamped to L and T.
+    A sequence that no path fits has score -inf and labels / spans -1.  See ``tone_ctc_align`` (include/tonehip.h)."""
+    torch = _torch()
+    typ = _type(x, "x")
+    if tokens.dtype != torch.int32 or tokens.dim() != 2 or not tokens.is_contiguous():
+        raise ValueError(f"tokens must be a contiguous (B, L) int32 tensor, got {tuple(tokens.shape)} {tokens.dtype}")
+    b, most = int(tokens.shape[0]), int(tokens.shape[1])
+    if most > MAX_TOKENS:
+        raise ValueError(f"at most {MAX_TOKENS} tokens per sequence, got {most}")
+    _vector(token_lens, "token_lens", torch.int32, b)
+    _vector(frame_lens, "frame_lens", torch.int32, b)
+    if rows is not None:
+        if rows.dtype != torch.int64 or rows.dim() != 2 or rows.shape[0] != b or not rows.is_contiguous():
+            raise ValueError(f"rows must be a contiguous ({b}, T) int64 tensor, got {tuple(rows.shape)} {rows.dtype}")
+        if x.dim() != 2:
+            raise ValueError(f"x must be (n_rows, vocab) with rows, got {tuple(x.shape)}")
+        frames, x_rows, stride, bstride = int(rows.shape[1]), int(x.shape[0]), x.stride(0), 0
+    else:
+        if x.dim() != 3 or x.shape[0] != b:
+            raise ValueError(f"x must be ({b}, T, vocab), got {tuple(x.shape)}")
+        frames, x_rows, stride, bstride = int(x.shape[1]), 0, x.stride(1), x.stride(0)
+    vocab = int(x.shape[-1])
+    if vocab < 1 or (vocab > 1 and x.stride(-1) != 1):
+        raise ValueError("x must have unit stride along a vocabulary of at least one entry")
+    if not 0 <= blank < vocab:
+        raise ValueError(f"blank {blank} outside the vocabulary of {vocab}")
+    dev = _device(x, tokens, token_lens, frame_lens, rows)
+    lib = _lib.load()
+    with _On(dev, stream, x, tokens, token_lens, frame_lens, rows) as st:
+        score = torch.empty(b, dtype=torch.float32, device=dev)
+        tot = torch.empty(b, dtype=torch.float32, device=dev) if total else None
+        labels = torch.empty((b, frames), dtype=torch.int32, device=dev)
+        spans = torch.empty((b, most, 2), dtype=torch.int32, device=dev)
+        need = lib.tone_ctc_align_workspace(b, frames, most)
+        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
+        _lib.check(lib.tone_ctc_align(dev.index, x.data_ptr(), typ, stride, bstride, x_rows, _ptr(rows), b, frames, vocab, blank,
+                                      tokens.data_ptr(), most, token_lens.data_ptr(), frame_lens.data_ptr(), score.data_ptr(),
+                                      _ptr(tot), labels.data_ptr(), spans.data_ptr(), _ptr(ws), need, st), "tone_ctc_align")
+    return CtcAlignment(score, tot, labels, spans)

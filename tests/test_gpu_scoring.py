@@ -1,0 +1,667 @@
+"""The phrase operators on a real MI355X against their 64-bit restatements (oracle/phrase_oracle.py): page plans and slot maps,
+row puts, token scores, CTC alignment; odd sizes, masks, strides, streams, graphs, and the phrase path as a server runs it.
+
+Tolerances.  EPS = 2^-24 is half a step of fp32.  A sum of n positive terms added one after another is off by at most n EPS of its
+value; a term e^z (z <= 0) by 2 |z| EPS for the rounding of z and its product with log2 e, and 4 EPS for the exponential.
+With s = sum e^z and mean = sum p |z|, ln s and the logprob are off by (n + 2 mean + 4) EPS plus their own last roundings, the
+entropy's sum u / s by the same factor twice of its value (mean) and 2 mean for the rounded products.  n counts the longest chain
+of additions that any split of the row over 64 lanes can have, V / 64 + 16.  One frame of the log-sum-exp over paths
+adds at most 3 terms in 32 bits: an exponential of at most 4 EPS each, a sum of at most 3 and a logarithm of at most 1.1, so
+4 + 2 + 2 + 4 EPS and in all below 16 EPS per frame; all else of it is 64 bits wide.  Best paths are 64 bits throughout and must agree exactly."""
+
+import numpy as np
+import pytest
+
+import phrase_oracle as O
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+EPS = 2.0 ** -24
+TYPES = {"fp32": torch.float32, "fp16": torch.float16, "bf16": torch.bfloat16}
+
+
+@pytest.fixture(autouse=True)
+def _gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm GPU")
+
+
+def S():
+    from tone_amd import scoring
+    return scoring
+
+
+def _dev(a, dtype=None):
+    return torch.from_numpy(np.ascontiguousarray(a if dtype is None else np.asarray(a, dtype))).cuda()
+
+
+# --- pages ------------------------------------------------------------------------------------------------------------
+
+class Pool:
+    """Streams that hold frames, as a server's buffers have them: rows of the table in ping-pong, the free queue."""
+
+    def __init__(self, rng, n, page, width, pages, head=0):
+        self.page, self.width, self.n = page, width, n
+        self.table = np.full((2 * n, width), -1, np.int32)
+        self.queue = np.full(pages, -1, np.int32)
+        self.queue[(head + np.arange(pages)) % pages] = rng.permutation(pages)
+        self.cursors = np.array([head, head + pages], np.int64)
+        self.first, self.length, self.par = np.zeros(n, np.int64), np.zeros(n, np.int64), np.zeros(n, np.int64)
+        self.dev = [_dev(self.table), _dev(self.queue), _dev(self.cursors), torch.zeros(2, dtype=torch.int64, device="cuda")]
+
+    def step(self, ids, keep, add, max_add, **kw):
+        ids = np.asarray(ids)
+        rows = 2 * ids + self.par[ids], 2 * ids + 1 - self.par[ids]
+        first, length = self.first[ids], self.length[ids]
+        t, q, cin, cout = self.dev
+        slots, status = S().frames_plan(t, q, cin, cout, *(_dev(v, np.int32) for v in (*rows, first, length, keep, add)),
+                                        page_size=self.page, max_add=max_add, **kw)
+        assert int(status) == 0
+        self.table, self.queue, self.cursors, want = O.plan(self.table, self.queue, self.cursors, *rows, first, length, keep, add, self.page, max_add)
+        self.first[ids], self.length[ids], self.par[ids] = np.maximum(first, keep), length + add, 1 - self.par[ids]
+        self.dev[2], self.dev[3] = cout, cin
+        np.testing.assert_array_equal(slots.cpu().numpy(), want)
+        np.testing.assert_array_equal(t.cpu().numpy(), self.table)
+        np.testing.assert_array_equal(q.cpu().numpy(), self.queue)
+        np.testing.assert_array_equal(cout.cpu().numpy(), self.cursors)
+        return slots
+
+
+@pytest.mark.parametrize("n,page,max_add,steps", [(1, 4, 3, 25), (1, 1, 10, 8), (7, 5, 10, 20), (70, 16, 13, 12), (300, 64, 10, 10),
+                                                  (700, 7, 3, 6), (3, 48, 2000, 4), (9000, 64, 10, 2)])
+def test_plan_over_steps(n, page, max_add, steps):
+    """Random subsets of streams over many steps: ragged adds (zero among them), frames let go, streams closed, the queue wrapping."""
+    rng = np.random.default_rng(n + page)
+    window = 4 * max(page, max_add)
+    width = -(-window // page) + 2
+    p = Pool(rng, n, page, width, n * (width + -(-max_add // page) + 1) + 3, head=int(rng.integers(0, 1000)))
+    for _ in range(steps):
+        ids = rng.permutation(n)[: rng.integers(1, n + 1)]
+        first, length = p.first[ids], p.length[ids]
+        add = rng.integers(0, max_add + 1, len(ids))
+        low = np.maximum(first, length + add - window)
+        keep = np.where(rng.random(len(ids)) < 0.3, rng.integers(low, length + add + 1), low)
+        p.step(ids, keep, add, max_add)
+
+
+def test_plan_of_no_requests_and_no_frames():
+    p = Pool(np.random.default_rng(0), 3, 4, 5, 20)
+    slots = p.step(np.array([], int), np.array([], int), np.array([], int), 6)
+    assert tuple(slots.shape) == (0, 6)
+    p.step([0, 1], [0, 0], [6, 3], 6)
+    p.step([0, 1, 2], [6, 2, 0], [0, 0, 0], 0)          # nothing new: one stream closed, one shortened
+
+
+@pytest.mark.parametrize("what,bit", [("pages", 1), ("row", 2), ("first", 4), ("keep", 4), ("add", 4), ("row_id", 4), ("same_row", 4),
+                                      ("cursors", 8), ("queue_short", 8)])
+def test_plan_refused_on_the_device_changes_nothing(what, bit):
+    """Every status bit: no page is taken or released, the rows keep their pages, every slot is -1."""
+    p = Pool(np.random.default_rng(1), 4, 4, 5, 40, head=33)
+    p.step([0, 1, 2, 3], [0, 0, 0, 0], [6, 9, 1, 4], 12)
+    rows_in, rows_out = 2 * np.arange(4) + p.par, 2 * np.arange(4) + 1 - p.par
+    first, length, keep, add = p.first.copy(), p.length.copy(), p.first.copy(), np.array([4, 4, 4, 4])
+    t, q, cin, cout = p.dev
+    if what == "pages":
+        cin = _dev(np.array([p.cursors[1] - 2, p.cursors[1]]))
+        add = np.array([6, 6, 6, 6])
+    elif what == "row":
+        add = np.array([4, 12, 4, 4])
+    elif what == "first":
+        first = first + np.array([0, 0, 30, 0])
+    elif what == "keep":
+        keep = keep + np.array([0, 0, 0, 30])
+    elif what == "add":
+        add = np.array([4, 4, 4, 13])
+    elif what == "row_id":
+        rows_out = rows_out + np.array([0, 0, 0, 100])
+    elif what == "same_row":
+        rows_out = np.where(np.arange(4) == 2, rows_in, rows_out)
+    elif what == "cursors":
+        cin = _dev(np.array([9, 3]))
+    else:
+        cin = _dev(np.array([5, 46]))
+    before = t.clone(), q.clone()
+    slots, status = S().frames_plan(t, q, cin, cout, *(_dev(v, np.int32) for v in (rows_in, rows_out, first, length, keep, add)),
+                                    page_size=4, max_add=12)
+    assert int(status) & bit and bool((slots == -1).all())
+    assert torch.equal(cout, cin) and torch.equal(q, before[1])
+    for b in range(4):
+        assert torch.equal(t[int(rows_in[b])], before[0][int(rows_in[b])])
+        if rows_out[b] < 8:
+            assert torch.equal(t[int(rows_out[b])], before[0][int(rows_in[b])])
+
+
+def test_plan_near_the_largest_frame_numbers():
+    """Frame numbers up to 2^31 - 1 (a stream that never closes) do not wrap."""
+    p = Pool(np.random.default_rng(2), 2, 64, 6, 30)
+    p.first[:] = p.length[:] = 2 ** 31 - 120
+    p.step([0, 1], [0, 0], [100, 119], 119)
+    p.step([1, 0], [0, 2 ** 31 - 100], [0, 10], 119)
+
+
+@pytest.mark.parametrize("page", [1, 7, 64])
+def test_slots_read_what_was_planned(page):
+    rng = np.random.default_rng(page)
+    n = 40
+    width = 300 // page + 3
+    p = Pool(rng, n, page, width, n * (width + 60 // page + 2))
+    for _ in range(5):
+        p.step(np.arange(n), np.maximum(p.first, p.length - 200), rng.integers(0, 60, n), 60)
+    ids = rng.integers(0, n, 50)                        # the same stream may be read twice
+    first = p.first[ids]
+    begin = first + rng.integers(-3, 40, 50)
+    count = rng.integers(0, 260, 50)
+    rows = 2 * ids + p.par[ids]
+    rows[:2] = (-1, 2 * n)                              # no such row
+    got = S().frames_slots(p.dev[0], *(_dev(v, np.int32) for v in (rows, first, begin, count)), page_size=page,
+                           n_pages=len(p.queue), max_count=250)
+    want = O.slots(p.table, rows, first, begin, count, page, len(p.queue), 250)
+    np.testing.assert_array_equal(got.cpu().numpy(), want)
+    bad = p.dev[0].clone()
+    bad[:, 1] = len(p.queue)                            # a page outside the pool, another below it
+    bad[:, 0] = -5
+    got = S().frames_slots(bad, *(_dev(v, np.int32) for v in (rows, first, begin, count)), page_size=page, n_pages=len(p.queue), max_count=250)
+    np.testing.assert_array_equal(got.cpu().numpy(), O.slots(bad.cpu().numpy(), rows, first, begin, count, page, len(p.queue), 250))
+
+
+@pytest.mark.parametrize("src", sorted(TYPES))
+@pytest.mark.parametrize("pool", sorted(TYPES))
+@pytest.mark.parametrize("n,vocab,pad", [(1, 35, 0), (10, 35, 0), (1000, 35, 3), (333, 1, 0), (257, 64, 0), (77, 1000, 5), (20, 8, 8), (3, 20000, 0)])
+def test_put(src, pool, n, vocab, pad):
+    g = torch.Generator(device="cuda").manual_seed(n + vocab)
+    x = torch.randn((n, vocab + pad), device="cuda", generator=g).mul_(30).to(TYPES[src])[:, :vocab]
+    x[0, 0] = float("nan")
+    x[-1, vocab - 1] = float("-inf")
+    wide = torch.full((2 * n + 3, vocab + pad), 7.0, dtype=TYPES[pool], device="cuda")
+    slots = torch.randperm(2 * n + 3, device="cuda", generator=g)[:n].contiguous()
+    slots[n // 2] = -1 if n > 2 else slots[n // 2]
+    if n > 3:
+        slots[1], slots[3] = 2 * n + 3, -(2 ** 40)      # outside: left out
+    want = wide.clone()
+    ok = (slots >= 0) & (slots < 2 * n + 3)
+    want[slots[ok], :vocab] = x[ok].to(TYPES[pool])
+    S().frames_put(x, slots, wide[:, :vocab])
+    assert torch.equal(wide.nan_to_num(1e4), want.nan_to_num(1e4)) and torch.equal(wide.isnan(), want.isnan())
+
+
+# --- scores -----------------------------------------------------------------------------------------------------------
+
+def _check_scores(x, tokens, k, rows=None, **kw):
+    """x: a device tensor (n, V); every output of every row."""
+    r = S().token_scores(x, None if tokens is None else _dev(tokens, np.int32), k=k, rows=None if rows is None else _dev(rows, np.int64), **kw)
+    v = x.shape[-1]
+    data = x.float().cpu().numpy().astype(np.float64)
+    n = len(rows) if rows is not None else data.shape[0]
+    got = [None if t is None else t.cpu().numpy() for t in r]
+    for i in range(n):
+        at = i if rows is None else int(rows[i])
+        tok = -1 if tokens is None else int(tokens[i])
+        if not 0 <= at < data.shape[0]:
+            want = (0.0, -1, 0.0, [(-1, -np.inf)] * k, 0.0)
+        else:
+            want = O.scores(data[at], tok, k)
+        lp, rank, entropy, top, mean = want
+        tol = (v / 64 + 16 + 2 * mean + 4) * EPS
+        where = f"row {i}"
+        if tokens is not None:
+            _close(got[0][i], lp, tol + 4 * EPS * (abs(lp) if np.isfinite(lp) else 0), where)
+            assert got[1][i] == rank, where
+        _close(got[2][i], entropy, tol + mean * (2 * tol + 2 * EPS) + 4 * EPS * (1 + entropy), where)
+        if k:
+            assert got[4][i].tolist() == [t for t, _ in top], where
+            for a, (_, b) in zip(got[3][i], top):
+                _close(a, b, tol + 4 * EPS * (abs(b) if np.isfinite(b) else 0), where)
+    return r
+
+
+def _close(a, b, tol, where):
+    # a difference of two fp32 values can lie outside fp32 (lowest - highest = -2 x the largest): rounded to the nearest
+    # fp32 value that is an infinity, from (2 - 2^-24) 2^127 on
+    if abs(b) >= (2 - 2.0 ** -24) * 2.0 ** 127:
+        b = np.sign(b) * np.inf
+    if not np.isfinite(b):
+        assert a == b, (where, a, b)
+    else:
+        assert abs(float(a) - b) <= tol, (where, float(a), b, tol)
+
+
+def _rows(n, v, dtype, seed, scale=3.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn((n, v), device="cuda", generator=g).mul_(scale).to(TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("n,v,k", [(1, 1, 1), (1, 2, 0), (3, 35, 35), (10, 35, 8), (130, 35, 1), (65, 34, 5), (5, 63, 63), (5, 64, 64),
+                                   (5, 65, 64), (7, 127, 16), (9, 512, 20), (6, 513, 9), (4, 1023, 64), (3, 2049, 10), (2, 5000, 33),
+                                   (1, 20011, 50)])
+def test_scores(dtype, n, v, k):
+    rng = np.random.default_rng(n * v)
+    x = _rows(n, v, dtype, n * v)
+    _check_scores(x, rng.integers(-1, v + 1, n), k)
+
+
+@pytest.mark.parametrize("n", [4097, 20000])
+def test_scores_of_many_short_rows(n):
+    """The forms for many rows: every whole output against float64 on the device's host copy, and a sample in full."""
+    x = _rows(n, 35, "fp32", n)
+    tokens = np.random.default_rng(n).integers(-1, 36, n)
+    r = S().token_scores(x, _dev(tokens, np.int32), k=8)
+    d = x.cpu().double()
+    lp = torch.log_softmax(d, -1).numpy()
+    given = (tokens >= 0) & (tokens < 35)
+    want = np.where(given, lp[np.arange(n), tokens.clip(0, 34)], 0.0)
+    assert np.abs(r.logprob.cpu().numpy() - want).max() <= 64 * EPS * (1 + np.abs(want).max())
+    order = np.argsort(-d.numpy(), axis=1, kind="stable")
+    np.testing.assert_array_equal(r.top_ids.cpu().numpy(), order[:, :8])
+    rank = np.where(given, (order == tokens[:, None].clip(0, 34)).argmax(1), -1)
+    np.testing.assert_array_equal(r.rank.cpu().numpy(), rank)
+    np.testing.assert_allclose(r.top_logprob.cpu().numpy(), np.take_along_axis(lp, order[:, :8], 1), rtol=1e-6, atol=64 * EPS)
+    entropy = -(np.exp(lp) * lp).sum(1)
+    assert np.abs(r.entropy.cpu().numpy() - entropy).max() <= 200 * EPS
+    sample = slice(0, 50)
+    _check_scores(x[sample], tokens[sample], 8)
+
+
+@pytest.mark.parametrize("v", [35, 64, 300, 4096, 9001])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_scores_of_equal_values(v, dtype):
+    """Ties everywhere: the lowest index first, the rank counts lower indices; -0 and +0 are one value."""
+    x = torch.randint(0, 3, (6, v), device="cuda", generator=torch.Generator(device="cuda").manual_seed(v)).to(TYPES[dtype])
+    x[0] = 1.5
+    x[1] = torch.where(torch.arange(v, device="cuda") % 2 == 0, -0.0, 0.0).to(TYPES[dtype])
+    x[2] = torch.arange(v, device="cuda").div(v, rounding_mode="floor").to(TYPES[dtype])
+    x[3] = (torch.arange(v, device="cuda") // 5).to(TYPES[dtype])          # ascending
+    x[4] = -(torch.arange(v, device="cuda") // 5).to(TYPES[dtype])         # descending
+    _check_scores(x, [v - 1, v // 2, 0, v // 3, 1, v - 1], min(v, 40))
+
+
+@pytest.mark.parametrize("v", [5, 35, 64, 200, 3000, 9001])
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+def test_scores_of_masked_rows(v, dtype):
+    """-inf entries, rows of nothing else, rows of the type's lowest value, one entry left, huge values."""
+    low, high = torch.finfo(TYPES[dtype]).min, torch.finfo(TYPES[dtype]).max
+    x = _rows(9, v, dtype, v)
+    x[0] = float("-inf")
+    x[1] = low
+    x[2, : v - 1] = float("-inf")
+    x[3, 1:] = low
+    x[4, ::2] = float("-inf")
+    x[5, : v // 2] = low
+    x[6] = float("-inf")
+    x[6, v // 2] = low                       # all of the probability on the lowest value
+    x[7, 0] = high
+    x[8, -1] = high
+    x[8, 0] = low
+    _check_scores(x, [0, v - 1, v - 1, 1, 0, 2, v // 2, 1, 0], min(v, 12))
+    _check_scores(x, [v - 1, 0, 0, 0, 1, v - 1, 0, 0, v - 1], min(v, 64))
+
+
+@pytest.mark.parametrize("v", [35, 64, 300, 9001])
+def test_scores_of_rows_with_nan_or_infinity(v):
+    """They make their own row NaN and no other, and the ids stay in range."""
+    x = _rows(5, v, "fp32", v)
+    clean = x.clone()
+    x[1, v // 2] = float("nan")
+    x[3, 0] = float("inf")
+    r = S().token_scores(x, torch.tensor([0, 1, 2, 3, 4], dtype=torch.int32, device="cuda"), k=4)
+    for i in (1, 3):
+        assert bool(r.entropy[i].isnan()) and bool(r.logprob[i].isnan())
+    assert int(r.top_ids.min()) >= 0 and int(r.top_ids.max()) < v and int(r.rank.min()) >= 0 and int(r.rank.max()) < v
+    want = S().token_scores(clean, torch.tensor([0, 1, 2, 3, 4], dtype=torch.int32, device="cuda"), k=4)
+    for a, b in zip(r, want):
+        assert torch.equal(a[[0, 2, 4]], b[[0, 2, 4]])
+
+
+@pytest.mark.parametrize("v", [35, 130, 2500])
+def test_scores_through_a_slot_map(v):
+    """Rows in any order, twice, none at all; x with spare columns; shapes kept."""
+    rng = np.random.default_rng(v)
+    x = _rows(50, v + 3, "fp32", v)[:, :v]
+    rows = rng.integers(0, 50, 60)
+    rows[[0, 7, 59]] = (-1, 50, 2 ** 40)
+    _check_scores(x, rng.integers(0, v, 60), 6, rows)
+    r = S().token_scores(x, _dev(rng.integers(0, v, (4, 15)), np.int32), k=6, rows=_dev(rows.reshape(4, 15), np.int64))
+    assert tuple(r.logprob.shape) == (4, 15) and tuple(r.top_ids.shape) == (4, 15, 6)
+    flat = S().token_scores(x, None, k=6, rows=_dev(rows, np.int64))
+    assert torch.equal(flat.top_ids, r.top_ids.view(60, 6)) and flat.logprob is None and flat.rank is None
+    assert torch.equal(flat.entropy, r.entropy.view(-1))
+
+
+def test_scores_of_no_rows():
+    r = S().token_scores(torch.empty((0, 35), device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), k=3)
+    assert tuple(r.top_ids.shape) == (0, 3) and r.entropy.numel() == 0
+    r = S().token_scores(torch.empty((0, 35), device="cuda"), None, k=3, rows=torch.tensor([0, -1], device="cuda"))
+    assert r.top_ids.tolist() == [[-1] * 3] * 2
+    S().frames_put(torch.zeros((2, 35), device="cuda"), torch.tensor([0, 1], device="cuda"), torch.empty((0, 35), device="cuda"))
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    r = S().ctc_align(torch.empty((0, 35), device="cuda"), one.view(1, 1), one, one, rows=torch.zeros((1, 1), dtype=torch.int64, device="cuda"))
+    assert r.score.item() == -np.inf and r.labels.tolist() == [[-1]]
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("n,v,k", [(40, 35, 8), (4, 700, 10), (1, 65537, 20), (3, 131072, 5)])
+@pytest.mark.parametrize("offset", [1, 2, 3])
+def test_scores_of_unaligned_rows(dtype, n, v, k, offset):
+    """Rows that begin at any element: the same values as an aligned copy gives."""
+    flat = _rows(1, n * (v + 1) + 8, dtype, v).view(-1)
+    x = flat[offset : offset + n * (v + 1)].view(n, v + 1)[:, :v]
+    tokens = torch.arange(n, dtype=torch.int32, device="cuda") * 7 % v
+    a, b = S().token_scores(x, tokens, k=k), S().token_scores(x.contiguous(), tokens, k=k)
+    assert torch.equal(a.top_ids, b.top_ids) and torch.equal(a.rank, b.rank)
+    for u, w in ((a.logprob, b.logprob), (a.entropy, b.entropy), (a.top_logprob, b.top_logprob)):
+        # both are within the tolerance of the exact value, whatever chains of additions they take
+        assert float((u - w).abs().max()) <= 2 * (v / 64 + 40) * EPS * (1 + float(w.abs().max()))
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("v", [40000, 65537, 131072])
+def test_scores_of_one_wide_row(dtype, v):
+    """A single row over a wide vocabulary, random and in ascending order."""
+    x = _rows(2, v, dtype, v)
+    x[1] = x[1].float().sort().values.to(TYPES[dtype])
+    for i in range(2):
+        _check_scores(x[i : i + 1], [v // 3], 32)
+
+
+def test_scores_are_the_same_every_time():
+    x = _rows(3, 131072, "bf16", 1)
+    tokens = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
+    a = S().token_scores(x, tokens, k=20)
+    for _ in range(5):
+        assert all(torch.equal(u, w) for u, w in zip(a, S().token_scores(x, tokens, k=20)))
+
+
+# --- alignment --------------------------------------------------------------------------------------------------------
+
+def _ctc(rng, b, f, most, vocab, blank, peaked=True):
+    """Log probabilities (b, f, vocab), tokens (b, most) with repeats, lengths (one at full size)."""
+    tlen = rng.integers(0, most + 1, b)
+    flen = rng.integers(0, f + 1, b)
+    tlen[0], flen[0] = most, f
+    tokens = rng.integers(0, vocab, (b, most))
+    tokens = np.where(tokens == blank, (tokens + 1) % vocab, tokens)
+    rep = rng.random((b, most)) < 0.2
+    for i in range(1, most):
+        tokens[:, i] = np.where(rep[:, i], tokens[:, i - 1], tokens[:, i])
+    x = rng.normal(0, 1.5, (b, f, vocab))
+    if peaked:
+        for i in range(b):
+            for j in range(tlen[i]):
+                if flen[i]:
+                    x[i, int((j + 0.5) * flen[i] / tlen[i]), tokens[i, j]] += 5
+    x = x - np.log(np.exp(x).sum(-1, keepdims=True))
+    return x, tokens.astype(np.int32), tlen.astype(np.int32), flen.astype(np.int32)
+
+
+def _check_align(x, tokens, tlen, flen, blank, total, data=None, **kw):
+    r = S().ctc_align(x, _dev(tokens), _dev(tlen), _dev(flen), blank=blank, total=total, **kw)
+    data = x.float().cpu().numpy().astype(np.float64) if data is None else data
+    score, labels, spans = r.score.cpu().numpy(), r.labels.cpu().numpy(), r.spans.cpu().numpy()
+    b, most = tokens.shape
+    for i in range(b):
+        n, f = int(np.clip(tlen[i], 0, most)), int(np.clip(flen[i], 0, labels.shape[1]))
+        w_score, w_total, w_labels, w_spans = O.align(data[i, :f], tokens[i, :n].tolist(), blank)
+        assert score[i] == np.float32(w_score), (i, score[i], w_score)
+        alive = w_labels is not None
+        assert labels[i].tolist() == (w_labels if alive else [-1] * f) + [-1] * (labels.shape[1] - f), i
+        assert spans[i].tolist() == (w_spans if alive else [[-1, -1]] * n) + [[-1, -1]] * (most - n), i
+        if total:
+            _close(r.total[i].item(), w_total, (f + 1) * 16 * EPS + EPS * abs(w_total) if np.isfinite(w_total) else 0, f"sequence {i}")
+    return r
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("total", [False, True])
+@pytest.mark.parametrize("b,f,most,vocab", [(1, 1, 1, 2), (3, 1, 2, 5), (4, 2, 1, 35), (5, 7, 3, 35), (6, 33, 9, 35), (3, 64, 31, 35), (3, 65, 32, 35),
+                                            (2, 130, 33, 100), (2, 70, 63, 35), (2, 129, 64, 36), (2, 200, 100, 40), (1, 300, 127, 35)])
+def test_align(dtype, total, b, f, most, vocab):
+    rng = np.random.default_rng(b * f + most)
+    blank = vocab - 1 if most % 2 else 0
+    x, tokens, tlen, flen = _ctc(rng, b, f, most, vocab, blank)
+    _check_align(_dev(x).to(TYPES[dtype]), tokens, tlen, flen, blank, total)
+
+
+@pytest.mark.parametrize("f,most", [(700, 300), (520, 255), (300, 256), (2100, 700), (64, 700), (1400, 640), (2100, 1000)])
+def test_align_long(f, most):
+    """Long sequences; too few frames for the tokens among them."""
+    rng = np.random.default_rng(f)
+    x, tokens, _, _ = _ctc(rng, 2, f, most, 35, 34)
+    lens = np.array([[most, f], [most // 2, f - f // 3]], np.int32)
+    _align_by_rows(rng, x, tokens, lens)
+
+
+def _align_by_rows(rng, x, tokens, lens):
+    """Against the definition evaluated a frame at a time over all states (the oracle's loops are too slow here)."""
+    b, f, vocab = x.shape
+    x32 = x.astype(np.float32).astype(np.float64)
+    r = S().ctc_align(_dev(x, np.float32), _dev(tokens), _dev(lens[:, 0].copy()), _dev(lens[:, 1].copy()), blank=34, total=True)
+    for i in range(b):
+        n, fr = int(lens[i, 0]), int(lens[i, 1])
+        lab = np.full(2 * n + 1, 34)
+        lab[1::2] = tokens[i, :n]
+        jump = np.zeros(2 * n + 1, bool)
+        jump[3::2] = lab[3::2] != lab[1:-2:2]
+        v = np.where(np.arange(2 * n + 1) < 2, x32[i, 0, lab], -np.inf)
+        w = v.copy()
+        back = np.zeros((fr, 2 * n + 1), int)
+        for t in range(1, fr):
+            for a in (0, 1):
+                src = w if a else v
+                c = np.full((3, 2 * n + 1), -np.inf)
+                c[0], c[1, 1:], c[2, 2:] = src, src[:-1], np.where(jump[2:], src[:-2], -np.inf)
+                if a:
+                    h = np.maximum(c.max(0), -1e300)
+                    with np.errstate(divide="ignore"):
+                        w = h + np.log(np.exp(c - h).sum(0)) + x32[i, t, lab]
+                else:
+                    back[t] = c.argmax(0)
+                    v = c.max(0) + x32[i, t, lab]
+        s = 2 * n - 1 if v[2 * n - 1] > v[2 * n] else 2 * n
+        assert r.score[i].item() == np.float32(v[s])
+        if v[s] == -np.inf:
+            assert bool((r.labels[i] == -1).all()) and bool((r.spans[i] == -1).all()) and r.total[i].item() == -np.inf
+            continue
+        want = np.full(f, -1)
+        for t in range(fr - 1, -1, -1):
+            want[t] = lab[s]
+            s -= back[t, s]
+        np.testing.assert_array_equal(r.labels[i].cpu().numpy(), want)
+        tot = np.logaddexp(w[2 * n], w[2 * n - 1])
+        _close(r.total[i].item(), tot, (fr + 1) * 16 * EPS + EPS * abs(tot), f"sequence {i}")
+
+
+def test_align_edges():
+    """No frames, no tokens, more tokens than frames, repeats that need a blank, a token outside, the blank as a token."""
+    rng = np.random.default_rng(0)
+    x, _, _, _ = _ctc(rng, 9, 6, 4, 5, 4, peaked=False)
+    tokens = np.array([[0, 1, 2, 3], [0, 0, 0, 0], [1, 1, 1, 1], [0, 1, 2, 3], [0, 9, 1, 1], [0, 4, 1, 1], [0, -1, 1, 1], [2, 2, 2, 0], [3, 3, 1, 1]], np.int32)
+    tlen = np.array([4, 0, 4, 0, 2, 2, 2, 9, 2], np.int32)      # 9: clamped to 4
+    flen = np.array([0, 0, 6, 3, 6, 6, 6, 99, 3], np.int32)     # 99: clamped to 6
+    _check_align(_dev(x, np.float32), tokens, tlen, flen, 4, True)
+    tlen[0], flen[0] = -3, -1
+    _check_align(_dev(x, np.float32), tokens, tlen, flen, 4, False)
+
+
+def test_align_of_equal_scores_prefers_to_stay():
+    """Constant rows: every path has the same score, and the tie rule alone decides."""
+    for f, tokens in ((5, [0, 1]), (7, [0, 0]), (9, [0, 1, 1, 2]), (4, [0]), (40, [0, 1, 0, 2, 2, 1])):
+        x = np.full((1, f, 4), -2.0)
+        _check_align(_dev(x, np.float32), np.array([tokens], np.int32), np.array([len(tokens)], np.int32), np.array([f], np.int32), 3, True)
+
+
+def test_align_with_nan_and_infinity():
+    """NaN, +inf and -inf entries all close their label in that frame."""
+    rng = np.random.default_rng(4)
+    x, tokens, tlen, flen = _ctc(rng, 6, 30, 6, 8, 7)
+    x[1, 3, :] = np.nan
+    x[2, rng.random((30, 8)) < 0.2] = -np.inf
+    x[3, rng.random((30, 8)) < 0.2] = np.inf
+    x[4, rng.random((30, 8)) < 0.2] = np.nan
+    x[5] = -np.inf
+    tlen[:], flen[:] = 4, 30
+    _check_align(_dev(x, np.float32), tokens, tlen, flen, 7, True)
+
+
+def test_align_reads_any_strides_and_slot_maps():
+    rng = np.random.default_rng(5)
+    x, tokens, tlen, flen = _ctc(rng, 5, 50, 12, 35, 34)
+    base = _check_align(_dev(x, np.float32), tokens, tlen, flen, 34, True)
+    x32 = x.astype(np.float32)
+    wide = torch.full((50, 5, 40), float("nan"), device="cuda")
+    wide[:, :, :35] = _dev(x32.transpose(1, 0, 2))
+    again = S().ctc_align(wide.transpose(0, 1)[:, :, :35], _dev(tokens), _dev(tlen), _dev(flen), total=True)
+    assert all(torch.equal(a, b) for a, b in zip(base, again))
+    pool = torch.full((700, 37), float("nan"), device="cuda")
+    rows = rng.permutation(700)[:250].reshape(5, 50)
+    pool[_dev(rows), :35] = _dev(x32)
+    rows_d = torch.where(torch.arange(50, device="cuda") < _dev(flen)[:, None], _dev(rows), -1)
+    again = S().ctc_align(pool[:, :35], _dev(tokens), _dev(tlen), _dev(flen), rows=rows_d, total=True)
+    assert all(torch.equal(a, b) for a, b in zip(base, again))
+    # one phrase's frames under five texts: an expanded batch
+    same = S().ctc_align(_dev(x32[:1]).expand(5, 50, 35), _dev(tokens), _dev(tlen), _dev(np.full(5, 50, np.int32)), total=True)
+    _check_align(_dev(np.repeat(x32[:1], 5, 0)), tokens, tlen, np.full(5, 50, np.int32), 34, True)
+    full = S().ctc_align(_dev(np.repeat(x32[:1], 5, 0)), _dev(tokens), _dev(tlen), _dev(np.full(5, 50, np.int32)), total=True)
+    assert all(torch.equal(a, b) for a, b in zip(same, full))
+    # frames without a row are closed: no path crosses them
+    rows_d[0, 10] = 700
+    lost = S().ctc_align(pool[:, :35], _dev(tokens), _dev(tlen), _dev(flen), rows=rows_d, total=True)
+    assert lost.score[0].item() == -np.inf and lost.total[0].item() == -np.inf and torch.equal(lost.score[1:], base.score[1:])
+
+
+def test_align_of_an_empty_batch_and_no_frames():
+    z = lambda *s: torch.zeros(s, dtype=torch.int32, device="cuda")  # noqa: E731
+    r = S().ctc_align(torch.empty((0, 5, 35), device="cuda"), z(0, 3), z(0), z(0), total=True)
+    assert r.score.numel() == 0 and tuple(r.spans.shape) == (0, 3, 2)
+    r = S().ctc_align(torch.empty((2, 0, 35), device="cuda"), z(2, 3), _dev(np.array([0, 2], np.int32)), z(2), total=True)
+    assert r.score.tolist() == [0.0, -np.inf] and r.total.tolist() == [0.0, -np.inf] and bool((r.spans == -1).all())
+    r = S().ctc_align(_rows(8, 35, "fp32", 1).view(2, 4, 35).log_softmax(-1), z(2, 0), z(2), _dev(np.array([4, 0], np.int32)))
+    assert r.labels.tolist() == [[34] * 4, [-1] * 4] and r.score[1].item() == 0.0
+
+
+# --- streams, graphs, far offsets -------------------------------------------------------------------------------------
+
+def _small_calls():
+    """One call of each operator on fixed inputs: name -> (function of a stream, inputs that a replay may change)."""
+    rng = np.random.default_rng(9)
+    x, tokens, tlen, flen = _ctc(rng, 4, 60, 14, 35, 34)
+    xd, td, ld, fd = _dev(x, np.float32), _dev(tokens), _dev(tlen), _dev(flen)
+    wide = _rows(2, 70001, "bf16", 3)
+    wt = torch.tensor([1, 2], dtype=torch.int32, device="cuda")
+    flat = torch.randint(0, 35, (4, 60), dtype=torch.int32, device="cuda")
+    pool = torch.zeros((300, 35), device="cuda")
+    slots = torch.randperm(300, device="cuda")[:240].view(4, 60).contiguous()
+    table = torch.arange(40, dtype=torch.int32, device="cuda").view(8, 5).contiguous()
+    i = lambda *v: torch.tensor(v, dtype=torch.int32, device="cuda")  # noqa: E731
+    queue, cin, cout = torch.arange(100, 160, dtype=torch.int32, device="cuda") % 60, torch.tensor([7, 30], device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    req = [i(0, 2, 4, 6), i(1, 3, 5, 7), i(0, 3, 9, 0), i(0, 8, 20, 40), i(0, 5, 9, 40), i(9, 3, 0, 0)]
+    return {
+        "plan": (lambda st: S().frames_plan(table, queue, cin, cout, *req, page_size=16, max_add=10, stream=st) + (table, queue, cout), []),
+        "slots": (lambda st: (S().frames_slots(table, req[0], req[2], req[2], req[3], page_size=16, n_pages=60, max_count=50, stream=st),), []),
+        "put": (lambda st: (S().frames_put(xd, slots, pool, stream=st), pool)[1:], [xd]),
+        "scores": (lambda st: S().token_scores(xd, flat, k=5, stream=st), [xd]),
+        "scores-wide": (lambda st: S().token_scores(wide, wt, k=20, stream=st), [wide]),
+        "align": (lambda st: S().ctc_align(xd, td, ld, fd, total=True, stream=st), [xd]),
+    }
+
+
+@pytest.mark.parametrize("name", ["plan", "slots", "put", "scores", "scores-wide", "align"])
+def test_on_another_stream(name):
+    fn, _ = _small_calls()[name]
+    want = [t.clone() for t in fn(None)]
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    got = fn(s)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("name", ["plan", "slots", "put", "scores", "scores-wide", "align"])
+def test_captured_and_replayed(name):
+    """Two graphs of one call, replayed in turn with changed inputs and eager calls between: each agrees with the eager result."""
+    fn, inputs = _small_calls()[name]
+    fn(None)
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = fn(None)
+        graphs.append((g, out))
+    torch.cuda.synchronize()
+    for step in range(4):
+        for t in inputs:
+            t.add_(torch.randn_like(t, dtype=torch.float32).mul_(0.1).to(t.dtype))
+        want = [t.clone() for t in fn(None)]
+        torch.cuda.synchronize()
+        for g, out in (graphs if step % 2 else graphs[::-1]):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(want, out)), f"replay {step}"
+
+
+def test_two_calls_at_once():
+    """Calls on two streams with their own outputs do not touch each other."""
+    calls = _small_calls()
+    s1, s2 = torch.cuda.Stream(), torch.cuda.Stream()
+    for name in ("scores-wide", "align"):
+        fn = calls[name][0]
+        want = [t.clone() for t in fn(None)]
+        torch.cuda.synchronize()
+        got = [fn(s) for _ in range(8) for s in (s1, s2)]
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for out in got for a, b in zip(want, out))
+
+
+def test_rows_past_32_bit_offsets():
+    """A pool of more than 2^31 entries: rows written and read at its end (and none at the offsets' low 32 bits)."""
+    n = 2 ** 31 // 35 + 1000
+    pool = torch.zeros((n, 35), dtype=torch.bfloat16, device="cuda")
+    x = _rows(40, 35, "bf16", 8).float().log_softmax(-1).to(torch.bfloat16)
+    rows = torch.arange(n - 40, n, device="cuda")
+    S().frames_put(x, rows, pool)
+    assert torch.equal(pool[n - 40 :], x) and not bool(pool[:2000].any())
+    tokens = torch.arange(40, dtype=torch.int32, device="cuda") % 34
+    a, b = S().token_scores(pool, tokens, k=5, rows=rows), S().token_scores(x, tokens, k=5)
+    assert all(torch.equal(u, w) for u, w in zip(a, b))
+    one = torch.tensor([6], dtype=torch.int32, device="cuda")
+    lens = torch.tensor([40], dtype=torch.int32, device="cuda")
+    text = tokens[None, :6].contiguous()
+    a = S().ctc_align(pool, text, one, lens, rows=rows[None].contiguous(), total=True)
+    b = S().ctc_align(x[None], text, one, lens, total=True)
+    assert all(torch.equal(u, w) for u, w in zip(a, b))
+    far = torch.zeros((2, n * 35), dtype=torch.bfloat16, device="cuda")[:, -35:]      # two rows 2^31 entries apart
+    far[1] = x[3]
+    r = S().token_scores(far, torch.tensor([1, 2], dtype=torch.int32, device="cuda"), k=5)
+    assert torch.equal(r.top_ids[1], S().token_scores(x[3:4], None, k=5).top_ids[0])
+
+
+def test_the_phrase_path():
+    """The operators as a server runs them: frames put page by page over many steps, a phrase read back, aligned and scored."""
+    rng = np.random.default_rng(6)
+    n, page, steps = 5, 16, 12
+    p = Pool(rng, n, page, 12, 60, head=11)
+    x, tokens, tlen, _ = _ctc(rng, n, 10 * steps, 20, 35, 34)
+    x32 = _dev(x, np.float32)
+    pool = torch.full((60 * page, 35), float("nan"), device="cuda")
+    for t in range(steps):
+        slots = p.step(np.arange(n), p.first, np.full(n, 10), 10)
+        S().frames_put(x32[:, 10 * t : 10 * t + 10].contiguous(), slots, pool)
+    begin, count = np.array([0, 5, 17, 100, 60]), np.array([120, 90, 64, 20, 1])
+    rows = S().frames_slots(p.dev[0], *(_dev(v, np.int32) for v in (2 * np.arange(n) + p.par, p.first, begin, count)), page_size=page, n_pages=60,
+                            max_count=120)
+    data = np.zeros((n, 120, 35))
+    for i in range(n):
+        data[i, : count[i]] = x[i, begin[i] : begin[i] + count[i]].astype(np.float32)
+    a = _check_align(pool, tokens, tlen, count.astype(np.int32), 34, True, data=data, rows=rows)
+    r = S().token_scores(pool, a.labels, k=3, rows=rows)
+    labels = a.labels.cpu().numpy()
+    for i in range(n):
+        for t in range(120):
+            if labels[i, t] < 0:
+                assert r.logprob[i, t].item() == 0.0
+            else:
+                assert abs(r.logprob[i, t].item() - data[i, t, labels[i, t]]) <= 1e-5

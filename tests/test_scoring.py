@@ -1,0 +1,235 @@
+"""The phrase operators on the CPU: the oracle against brute force, and every refusal that needs no GPU -- of the Python
+functions and of the C entry points, which check their arguments before they touch the device."""
+
+import ctypes
+
+import numpy as np
+import pytest
+
+import phrase_oracle as O
+from tone_amd import _lib
+from tone_amd import scoring as S
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.parametrize("seed", range(12))
+def test_oracle_alignment_is_the_best_and_the_sum_of_all_paths(seed):
+    rng = np.random.default_rng(seed)
+    f, vocab = int(rng.integers(1, 7)), int(rng.integers(2, 5))
+    blank = int(rng.integers(0, vocab))
+    tokens = [int(t) for t in rng.integers(0, vocab, int(rng.integers(0, 4))) if t != blank]
+    x = np.log(rng.dirichlet(np.ones(vocab), f))
+    score, total, labels, spans = O.align(x, tokens, blank)
+    want = O.align_by_paths(x, tokens, blank)
+    np.testing.assert_allclose([score, total], want, rtol=1e-12)
+    if labels is not None:
+        assert [c for i, c in enumerate(labels) if c != blank and (i == 0 or labels[i - 1] != c)] == tokens
+        np.testing.assert_allclose(sum(x[t, c] for t, c in enumerate(labels)), score, rtol=1e-12)
+        for t, (a, b) in zip(tokens, spans):
+            assert all(labels[i] == t for i in range(a, b))
+
+
+def test_oracle_scores_sum_to_one():
+    rng = np.random.default_rng(0)
+    row = rng.normal(size=35)
+    lp, rank, entropy, top, _ = O.scores(row, 7, 35)
+    p = np.exp([v for _, v in top])
+    np.testing.assert_allclose(p.sum(), 1.0, rtol=1e-12)
+    np.testing.assert_allclose(entropy, -(p * np.log(p)).sum(), rtol=1e-12)
+    assert top[rank][0] == 7 and top[rank][1] == lp
+
+
+def test_oracle_plan_keeps_every_page_once():
+    rng = np.random.default_rng(3)
+    page, n, width, pages = 4, 3, 6, 20
+    table, queue, cur = np.full((2 * n, width), -1, np.int32), np.arange(pages, dtype=np.int32), np.array([0, pages])
+    first, length, par = np.zeros(n, int), np.zeros(n, int), np.zeros(n, int)
+    for _ in range(40):
+        add = rng.integers(0, 6, n)
+        keep = np.minimum(length + add, np.maximum(first, length - rng.integers(0, 12, n)))
+        table, queue, cur, slots = O.plan(table, queue, cur, 2 * np.arange(n) + par, 2 * np.arange(n) + 1 - par, first, length, keep, add, page, 6)
+        first, length, par = np.maximum(first, keep), length + add, 1 - par
+        held = np.concatenate([table[2 * i + par[i]] for i in range(n)])
+        free = [int(queue[i % pages]) for i in range(cur[0], cur[1])]
+        assert sorted(list(held[held >= 0]) + free) == list(range(pages))
+        got = slots[slots >= 0]
+        assert len(set(got)) == len(got)
+
+
+# --- refusals of the Python functions ---------------------------------------------------------------------------------
+
+def _i32(*v):
+    return torch.tensor(v, dtype=torch.int32)
+
+
+def _plan_args(**change):
+    a = dict(table=torch.zeros((4, 3), dtype=torch.int32), queue=torch.arange(8, dtype=torch.int32),
+             cursors_in=torch.tensor([0, 8]), cursors_out=torch.zeros(2, dtype=torch.int64), rows_in=_i32(0, 2), rows_out=_i32(1, 3),
+             first=_i32(0, 0), length=_i32(0, 0), keep=_i32(0, 0), add=_i32(1, 2), page_size=4, max_add=2)
+    a.update(change)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    {"table": torch.zeros((4, 3), dtype=torch.int64)}, {"table": torch.zeros((3, 4), dtype=torch.int32).t()},
+    {"table": torch.zeros(4, dtype=torch.int32)}, {"queue": torch.arange(8)}, {"queue": torch.empty(0, dtype=torch.int32)},
+    {"cursors_in": _i32(0, 8)}, {"cursors_out": torch.zeros(3, dtype=torch.int64)}, {"rows_in": _i32(0)},
+    {"rows_out": torch.tensor([1, 3])}, {"first": _i32(0, 0, 0)}, {"add": _i32(0, 1, 2, 3)[::2]}, {"page_size": 0},
+    {"max_add": -1}, {"page_size": 2 ** 30}, {"slots": torch.zeros((2, 3), dtype=torch.int64)},
+    {"slots": torch.zeros((2, 2), dtype=torch.int32)}, {"status": torch.zeros(2, dtype=torch.int32)}, {},
+])
+def test_frames_plan_refuses(change):
+    """Wrong types, shapes and strides; with nothing changed, tensors that are not on a GPU."""
+    with pytest.raises(ValueError):
+        S.frames_plan(**_plan_args(**change))
+
+
+def test_frames_plan_refuses_aliased_cursors():
+    a = _plan_args()
+    a["cursors_out"] = a["cursors_in"]
+    with pytest.raises(ValueError, match="alias"):
+        S.frames_plan(**a)
+
+
+@pytest.mark.parametrize("change", [{"rows": torch.tensor([0])}, {"first": _i32(0, 1)}, {"max_count": -1}, {"n_pages": 0},
+                                    {"slots": torch.zeros((1, 3), dtype=torch.int64)}, {}])
+def test_frames_slots_refuses(change):
+    a = dict(table=torch.zeros((4, 3), dtype=torch.int32), rows=_i32(0), first=_i32(0), begin=_i32(0), count=_i32(1), page_size=4,
+             n_pages=3, max_count=2)
+    a.update(change)
+    with pytest.raises(ValueError):
+        S.frames_slots(**a)
+
+
+@pytest.mark.parametrize("change", [
+    {"src": torch.zeros((2, 5), dtype=torch.float64)}, {"src": torch.zeros((2, 4))}, {"src": torch.zeros((5, 2)).t()},
+    {"slots": torch.zeros(3, dtype=torch.int64)}, {"slots": torch.zeros(2, dtype=torch.int32)}, {"pool": torch.zeros((9, 5), dtype=torch.int8)},
+    {"pool": torch.zeros((3, 3, 5))}, {"pool": torch.zeros((1, 5)).expand(9, 5)}, {"src": torch.zeros((1, 5)).expand(2, 5)}, {},
+])
+def test_frames_put_refuses(change):
+    a = dict(src=torch.zeros((2, 5)), slots=torch.zeros(2, dtype=torch.int64), pool=torch.zeros((9, 5)))
+    a.update(change)
+    with pytest.raises(ValueError):
+        S.frames_put(**a)
+
+
+@pytest.mark.parametrize("change", [
+    {"x": torch.zeros((2, 5), dtype=torch.int32)}, {"x": torch.zeros(5)}, {"x": torch.zeros((2, 0))}, {"x": torch.zeros((5, 2)).t()},
+    {"tokens": torch.zeros(2, dtype=torch.int64)}, {"tokens": torch.zeros(3, dtype=torch.int32)}, {"k": 6}, {"k": -1},
+    {"x": torch.zeros((2, 100)), "k": 65}, {"rows": torch.zeros(2, dtype=torch.int32)},
+    {"x": torch.zeros((1, 2, 5)), "rows": torch.zeros(2, dtype=torch.int64)}, {"rows": torch.zeros(3, dtype=torch.int64)},
+    {"x": torch.zeros((1, 5)).expand(2, 5)}, {},
+])
+def test_token_scores_refuses(change):
+    a = dict(x=torch.zeros((2, 5)), tokens=torch.zeros(2, dtype=torch.int32), k=2)
+    a.update(change)
+    with pytest.raises(ValueError):
+        S.token_scores(**a)
+
+
+@pytest.mark.parametrize("change", [
+    {"x": torch.zeros((2, 6, 5), dtype=torch.float64)}, {"x": torch.zeros((3, 6, 5))}, {"x": torch.zeros((6, 5))},
+    {"x": torch.zeros((2, 5, 6)).transpose(1, 2)}, {"tokens": torch.zeros((2, 3), dtype=torch.int64)},
+    {"tokens": torch.zeros(2, dtype=torch.int32)}, {"tokens": torch.zeros((2, S.MAX_TOKENS + 1), dtype=torch.int32)},
+    {"token_lens": _i32(1)}, {"frame_lens": torch.tensor([1, 1])}, {"blank": 5}, {"blank": -1},
+    {"rows": torch.zeros((2, 6), dtype=torch.int64)}, {"x": torch.zeros((9, 5)), "rows": torch.zeros((3, 6), dtype=torch.int64)},
+    {"x": torch.zeros((9, 5)), "rows": torch.zeros((2, 6), dtype=torch.int32)}, {},
+])
+def test_ctc_align_refuses(change):
+    a = dict(x=torch.zeros((2, 6, 5)), tokens=torch.zeros((2, 3), dtype=torch.int32), token_lens=_i32(3, 2), frame_lens=_i32(6, 6), blank=4)
+    a.update(change)
+    with pytest.raises(ValueError):
+        S.ctc_align(**a)
+
+
+# --- refusals of the C entry points: before any device call, so the pointers here are never followed --------------------
+
+P = ctypes.c_void_p(4096)      # not null
+Q = ctypes.c_void_p(8192)
+
+
+def _refused(rc, *words):
+    msg = _lib.load().tone_last_error().decode()
+    assert rc == -1 and all(w in msg for w in words), (rc, msg)
+
+
+def test_c_frames_plan_refuses():
+    def call(table=P, stride=3, n_rows=4, width=3, queue=P, n_pages=8, page=4, cin=P, cout=Q, req=P, batch=2, slots=P, max_add=2, status=P):
+        return _lib.load().tone_frames_plan(0, table, stride, n_rows, width, queue, n_pages, page, cin, cout, req, P, P, P, P, P, batch,
+                                            slots, max_add, status, None)
+    _refused(call(table=None), "tone_frames_plan", "null")
+    _refused(call(queue=None), "null")
+    _refused(call(status=None), "null")
+    _refused(call(req=None), "null")
+    _refused(call(slots=None), "null")
+    _refused(call(cout=P), "cursors_out")
+    _refused(call(stride=2), "table_stride")
+    _refused(call(page=0), "positive")
+    _refused(call(n_pages=0), "positive")
+    _refused(call(batch=-1), "negative")
+    _refused(call(page=1 << 30), "2^31")
+
+
+def test_c_frames_slots_and_put_refuse():
+    lib = _lib.load()
+    _refused(lib.tone_frames_slots(0, P, 3, 4, 3, 8, 4, None, P, P, P, 1, P, 2, None), "null")
+    _refused(lib.tone_frames_slots(0, P, 2, 4, 3, 8, 4, P, P, P, P, 1, P, 2, None), "table_stride")
+    _refused(lib.tone_frames_slots(0, P, 3, 4, 3, 8, 4, P, P, P, P, -1, P, 2, None), "negative")
+    _refused(lib.tone_frames_slots(0, P, 3, 4, 3, 8, 4, P, P, P, P, 1 << 30, P, 1 << 20, None), "one launch")
+    _refused(lib.tone_frames_put(0, P, 7, 5, P, 2, 5, P, 0, 5, 9, None), "type")
+    _refused(lib.tone_frames_put(0, P, 0, 4, P, 2, 5, P, 0, 5, 9, None), "stride")
+    _refused(lib.tone_frames_put(0, P, 0, 5, None, 2, 5, P, 0, 5, 9, None), "null")
+    _refused(lib.tone_frames_put(0, P, 0, 5, P, -2, 5, P, 0, 5, 9, None), "range")
+
+
+def test_c_token_scores_refuses():
+    lib = _lib.load()
+
+    def call(x=P, typ=0, stride=5, x_rows=2, rows=None, n=2, vocab=5, tokens=P, k=2, lp=P, ent=P, top=P, ws=None, wb=0):
+        return lib.tone_token_scores(0, x, typ, stride, x_rows, rows, n, vocab, tokens, k, lp, ent, P, top, P, ws, wb, None)
+    _refused(call(x=None), "null")
+    _refused(call(ent=None), "null")
+    _refused(call(top=None), "null")
+    _refused(call(lp=None), "logprob")
+    _refused(call(k=6), "k must")
+    _refused(call(vocab=100, stride=100, k=65), "k must")
+    _refused(call(typ=3), "type")
+    _refused(call(x_rows=1), "fewer rows")
+    _refused(call(stride=4), "stride")
+    _refused(call(n=-1), "range")
+    assert lib.tone_token_scores_workspace(-1, 5, 2) == -1
+    need = lib.tone_token_scores_workspace(1, 131072, 20)
+    if need:
+        _refused(call(n=1, vocab=131072, stride=131072, k=20), "workspace")
+        _refused(call(n=1, vocab=131072, stride=131072, k=20, ws=P, wb=need - 1), "workspace")
+
+
+def test_c_ctc_align_refuses():
+    lib = _lib.load()
+    need = lib.tone_ctc_align_workspace(2, 6, 3)
+
+    def call(x=P, typ=0, batch=2, frames=6, vocab=5, blank=4, tokens=P, most=3, lens=P, score=P, labels=P, spans=P, ws=P, wb=need):
+        return lib.tone_ctc_align(0, x, typ, 5, 30, 0, None, batch, frames, vocab, blank, tokens, most, lens, P, score, None, labels, spans,
+                                  ws, wb, None)
+    _refused(call(x=None), "null")
+    _refused(call(tokens=None), "null")
+    _refused(call(lens=None), "null")
+    _refused(call(score=None), "null")
+    _refused(call(labels=None), "null")
+    _refused(call(spans=None), "null")
+    _refused(call(typ=-1), "type")
+    _refused(call(blank=5), "blank")
+    _refused(call(most=S.MAX_TOKENS + 1), "max_tokens")
+    _refused(call(frames=-1), "range")
+    _refused(call(ws=None), "workspace")
+    _refused(call(wb=need - 1), "workspace")
+    assert lib.tone_ctc_align_workspace(2, 6, S.MAX_TOKENS + 1) == -1
+
+
+def test_c_empty_calls_do_nothing():
+    lib = _lib.load()
+    assert lib.tone_frames_slots(0, None, 3, 4, 3, 8, 4, None, None, None, None, 0, None, 2, None) == 0
+    assert lib.tone_frames_put(0, None, 0, 5, None, 0, 5, None, 0, 5, 9, None) == 0
+    assert lib.tone_token_scores(0, None, 0, 5, 0, None, 0, 5, None, 0, None, None, None, None, None, None, 0, None) == 0
+    assert lib.tone_ctc_align(0, None, 0, 5, 0, 0, None, 0, 6, 5, 4, None, 3, None, None, None, None, None, None, None, 0, None) == 0
