@@ -218,10 +218,9 @@ int tone_frames_put(int device, const void *src, int src_type, int64_t src_strid
  * entropy 0.  A NaN or +inf in a row makes its floating outputs NaN and its rank and ids any values in range.
  * tokens may be NULL (then logprob and rank are not written). */
 #define TONE_SCORES_MAX_K 64
-int64_t tone_token_scores_workspace(int64_t n, int vocab, int k);
 int tone_token_scores(int device, const void *x, int type, int64_t stride, int64_t x_rows, const int64_t *rows, int64_t n,
                       int vocab, const int32_t *tokens, int k, float *logprob, float *entropy, int32_t *rank,
-                      float *top_logprob, int32_t *top_ids, void *workspace, int64_t workspace_bytes, void *stream);
+                      float *top_logprob, int32_t *top_ids, void *stream);
 
 /* CTC alignment of tokens [batch][max_tokens] (token_lens of them) to frame_lens frames of log probabilities: frame (b, t)
  * at b * batch_stride + t * stride of x, or row rows[b][t] of x [x_rows] where `rows` is given.

@@ -47,9 +47,8 @@ SIGNATURES = {
                           + [_c_int, _c_void_p, _c_int, _c_void_p]),
     "tone_frames_put": (_c_int, [_c_int, _c_void_p, _c_int, _c_int64, _c_void_p, _c_int64, _c_int, _c_void_p, _c_int, _c_int64,
                                  _c_int64, _c_void_p]),
-    "tone_token_scores_workspace": (_c_int64, [_c_int64, _c_int, _c_int]),
     "tone_token_scores": (_c_int, [_c_int, _c_void_p, _c_int, _c_int64, _c_int64, _c_void_p, _c_int64, _c_int, _c_void_p, _c_int]
-                          + [_c_void_p] * 6 + [_c_int64, _c_void_p]),
+                          + [_c_void_p] * 6),
     "tone_ctc_align_workspace": (_c_int64, [_c_int, _c_int, _c_int]),
     "tone_ctc_align": (_c_int, [_c_int, _c_void_p, _c_int, _c_int64, _c_int64, _c_int64, _c_void_p, _c_int, _c_int, _c_int, _c_int,
                                 _c_void_p, _c_int] + [_c_void_p] * 7 + [_c_int64, _c_void_p]),

@@ -156,6 +156,7 @@ int tone_ctc_align(int device, const void* x, int type, int64_t stride, int64_t 
   if (batch == 0) return TONE_OK;
   if ((!x && frames && (!rows || x_rows)) || !token_lens || !frame_lens || !score || (frames && !labels) || (max_tokens && (!tokens || !spans)))
     return refuse(what, "null pointer");
+  if (!aligned(x, type)) return refuse(what, "x not aligned to its element type");
   const int64_t need = tone_ctc_align_workspace(batch, frames, max_tokens);
   if (workspace_bytes < need || (need && !workspace)) return refuse(what, "workspace smaller than tone_ctc_align_workspace");
   AlignArgs p{x, stride, batch_stride, x_rows, rows, batch, frames, vocab, blank, tokens, max_tokens, token_lens, frame_lens,

@@ -306,6 +306,7 @@ int tone_frames_put(int device, const void* src, int src_type, int64_t src_strid
   if (n == 0) return TONE_OK;
   if (!src || !slots || (!pool && pool_rows)) return refuse(what, "null pointer");
   if (src_stride < vocab || pool_stride < vocab) return refuse(what, "row stride < vocab");
+  if (!aligned(src, src_type) || !aligned(pool, pool_type)) return refuse(what, "src or pool not aligned to its element type");
   if ((n + 15) / 16 > INT32_MAX) return refuse(what, "too many rows for one launch");
   PutArgs p{src, src_type, src_stride, slots, n, vocab, pool, pool_type, pool_stride, pool_rows};
   return launch_on(device, what, [&] { return launch_put(p, static_cast<hipStream_t>(stream)); });

@@ -7,6 +7,7 @@
 #include "scoring.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tone {
 namespace {
@@ -24,94 +25,444 @@ struct ScoreArgs {
   int32_t* top_ids;
 };
 
-// larger value = larger key; equal values: the lower index has the larger key.  -0 and +0 are one value.
-__device__ __forceinline__ uint64_t order_key(float v, int i) {
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  const uint32_t o = b & 0x80000000u ? ~b : b | 0x80000000u;
-  return ((uint64_t)o << 32) | (uint32_t)~i;
+constexpr float kLog2e = 1.4426950408889634f;
+// e^z for z <= 0 (v_exp_f32; z log2 e is rounded once, so e^z is off by about |z| 2^-24 of its value)
+__device__ __forceinline__ float exp_neg(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
+
+// total order of the values as integers: larger value = larger integer, -0 and +0 are one value, never INT_MIN
+__device__ __forceinline__ int order_of(float v) {
+  const int b = __float_as_int(v + 0.0f);
+  return max(b < 0 ? b ^ 0x7fffffff : b, -0x7fffffff);
+}
+// larger value = larger key; equal values: the lower index has the larger key.  Never 0.
+__device__ __forceinline__ uint64_t key_of(float v, int i) {
+  return ((uint64_t)((uint32_t)order_of(v) ^ 0x80000000u) << 32) | (uint32_t)~i;
 }
 __device__ __forceinline__ float key_value(uint64_t key) {
-  const uint32_t o = (uint32_t)(key >> 32);
-  return __uint_as_float(o & 0x80000000u ? o & 0x7fffffffu : ~o);
+  const int o = (int)((uint32_t)(key >> 32) ^ 0x80000000u);
+  return __int_as_float(o < 0 ? o ^ 0x7fffffff : o);
+}
+__device__ __forceinline__ int key_index(uint64_t key) { return (int)~(uint32_t)key; }
+
+// lane ^ X of a 16-lane row without LDS (DPP); X = 16 or 32: ds_bpermute
+template <int X>
+__device__ __forceinline__ int xor_lane(int v) {
+  if constexpr (X == 1) return __builtin_amdgcn_mov_dpp(v, 0xb1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+  else if constexpr (X == 2) return __builtin_amdgcn_mov_dpp(v, 0x4e, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  else if constexpr (X == 3) return __builtin_amdgcn_mov_dpp(v, 0x1b, 0xf, 0xf, true);   // quad_perm 3 2 1 0
+  else if constexpr (X == 7) return __builtin_amdgcn_mov_dpp(v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  else if constexpr (X == 15) return __builtin_amdgcn_mov_dpp(v, 0x140, 0xf, 0xf, true); // row_mirror
+  else if constexpr (X == 8) return __builtin_amdgcn_mov_dpp(v, 0x128, 0xf, 0xf, true);  // row_ror 8
+  else if constexpr (X < 7) return xor_lane<7 - X>(xor_lane<7>(v));
+  else return __shfl_xor(v, X);
+}
+template <int X>
+__device__ __forceinline__ float xor_lane(float v) { return __int_as_float(xor_lane<X>(__float_as_int(v))); }
+template <int X>
+__device__ __forceinline__ uint64_t xor_lane(uint64_t v) {
+  return ((uint64_t)(uint32_t)xor_lane<X>((int)(v >> 32)) << 32) | (uint32_t)xor_lane<X>((int)(uint32_t)v);
+}
+__device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
+  return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+         (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+}
+__device__ __forceinline__ float read_lane(float v, int lane) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
 }
 
-// one wave per row
-template <typename T>
-__global__ void __launch_bounds__(256) scores_kernel(ScoreArgs p) {
-  const int lane = threadIdx.x & 63;
-  const int64_t n = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (n >= p.n) return;
-  const int64_t row = p.rows ? p.rows[n] : n;
-  const bool here = row >= 0 && row < p.x_rows;
-  if (!here) {
-    if (lane == 0) {
-      if (p.logprob) p.logprob[n] = 0.f;
-      if (p.rank) p.rank[n] = -1;
-      p.entropy[n] = 0.f;
+// what a row that is none gives
+__device__ __forceinline__ void write_none(const ScoreArgs& p, int64_t n, int first, int step) {
+  if (first == 0) {
+    if (p.tokens) {
+      p.logprob[n] = 0.f;
+      p.rank[n] = -1;
     }
-    if (lane < p.k) {
-      p.top_lp[n * p.k + lane] = -INFINITY;
-      p.top_ids[n * p.k + lane] = -1;
-    }
-    return;
+    p.entropy[n] = 0.f;
   }
+  for (int i = first; i < p.k; i += step) {
+    p.top_lp[n * p.k + i] = -INFINITY;
+    p.top_ids[n * p.k + i] = -1;
+  }
+}
+
+// Rows of up to 64 entries (the 35-token head): 8 lanes per row, entry 8 e + lane in register e, 8 rows per wave.  Every
+// entry's rank is counted against all others (the other lanes' registers come by DPP, lane ^ 1 .. 7), so one pass gives the
+// given token's rank and the place of each of the top k, whatever k is, with no selection rounds and no LDS: 8 E^2
+// compares per 8 rows.
+template <typename T, int E>
+__global__ void __launch_bounds__(256) scores_short_kernel(ScoreArgs p) {
+  const int sub = threadIdx.x & 7;
+  const int64_t n = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const bool in = n < p.n;
+  const int64_t row = !in ? -1 : p.rows ? p.rows[n] : n;
+  const bool here = row >= 0 && row < p.x_rows;
+  if (in && !here) write_none(p, n, sub, 8);
+  if (!here) return;                     // whole groups of 8 lanes: the DPP exchanges below stay inside a group
   const T* x = static_cast<const T*>(p.x) + row * p.stride;
   const int t = p.tokens ? p.tokens[n] : -1;
-  const bool given = t >= 0 && t < p.vocab;
-  const float xt = given ? load_elem(x + t) : 0.f;
-  float m = -INFINITY;
-  for (int v = lane; v < p.vocab; v += 64) m = fmaxf(m, load_elem(x + v));
-  for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+  float v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = 8 * e + sub < p.vocab ? load_elem(x + 8 * e + sub) : -INFINITY;
+  float m = -3.402823466e38f;            // finite, so that -inf - m is -inf and a row of -inf sums up to 0
+#pragma unroll
+  for (int e = 0; e < E; ++e) m = fmaxf(m, v[e]);
+  m = fmaxf(m, xor_lane<1>(m));
+  m = fmaxf(m, xor_lane<2>(m));
+  m = fmaxf(m, xor_lane<7>(m));
   float s = 0.f, u = 0.f;
-  int above = 0;
-  for (int v = lane; v < p.vocab; v += 64) {
-    const float xv = load_elem(x + v);
-    const float z = xv - m, e = expf(z);
-    if (xv > -INFINITY || !(xv == xv)) {
-      s += e;
-      u += e > 0.f ? e * z : (z == z ? 0.f : z);
-    }
-    above += xv > xt || (xv == xt && v < t);
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const float z = v[e] - m, ex = exp_neg(z);
+    s += ex;
+    u = fmaf(ex, fmaxf(z, -200.f), u);   // e^-200 is 0 in fp32: the bound keeps 0 x -inf out
   }
-  for (int o = 32; o; o >>= 1) {
-    s += __shfl_xor(s, o);
-    u += __shfl_xor(u, o);
-    above += __shfl_xor(above, o);
-  }
-  const bool left = !(s == 0.f);
+  s += xor_lane<1>(s);
+  u += xor_lane<1>(u);
+  s += xor_lane<2>(s);
+  u += xor_lane<2>(u);
+  s += xor_lane<7>(s);
+  u += xor_lane<7>(u);
+  const bool left = s != 0.f;            // a NaN counts as something left
   const float ls = logf(s);
-  if (lane == 0) {
-    if (p.logprob) p.logprob[n] = given ? (left ? xt - m - ls : -INFINITY) : 0.f;
-    if (p.rank) p.rank[n] = given ? above : -1;
+  if (sub == 0) {
     p.entropy[n] = left ? ls - u / s : 0.f;
+    if (p.tokens && !(t >= 0 && t < p.vocab)) {
+      p.logprob[n] = 0.f;
+      p.rank[n] = -1;
+    }
   }
-  uint64_t last = ~0ull;
-  for (int i = 0; i < p.k; ++i) {
-    uint64_t best = 0;
-    for (int v = lane; v < p.vocab; v += 64) {
-      const uint64_t key = order_key(load_elem(x + v), v);
-      if (key < last && key > best) best = key;
+  if (!p.k && !p.tokens) return;
+  int o[E], above[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    o[e] = 8 * e + sub < p.vocab ? order_of(v[e]) : -0x7fffffff - 1;    // entries that are none are below all
+    above[e] = 0;
+  }
+#pragma unroll
+  for (int e = 0; e < E; ++e)
+#pragma unroll
+    for (int f = 0; f < E; ++f)
+      if (f != e) above[e] += f < e ? o[f] >= o[e] : o[f] > o[e];
+  auto against = [&](const int (&w)[E], int lower) {   // lower: 1 where the other lane is below this one
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+#pragma unroll
+      for (int f = 0; f < E; ++f) above[e] += f < e ? w[f] >= o[e] : f > e ? w[f] > o[e] : w[f] + lower > o[e];
+    }
+  };
+  auto with = [&](auto x_) {
+    constexpr int X = decltype(x_)::value;
+    int w[E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) w[e] = xor_lane<X>(o[e]);
+    against(w, (sub ^ X) < sub);
+  };
+  with(std::integral_constant<int, 1>{});
+  with(std::integral_constant<int, 2>{});
+  with(std::integral_constant<int, 3>{});
+  with(std::integral_constant<int, 4>{});
+  with(std::integral_constant<int, 5>{});
+  with(std::integral_constant<int, 6>{});
+  with(std::integral_constant<int, 7>{});
+#pragma unroll
+  for (int e = 0; e < E; ++e) {
+    const int i = 8 * e + sub;
+    if (i >= p.vocab) continue;
+    const float lp = left ? v[e] - m - ls : -INFINITY;
+    if (i == t && p.tokens) {
+      p.logprob[n] = lp;
+      p.rank[n] = above[e];
+    }
+    if (above[e] < p.k) {
+      p.top_lp[n * p.k + above[e]] = lp;
+      p.top_ids[n * p.k + above[e]] = i;
+    }
+  }
+}
+
+// The 64 best keys of a wave, one per lane in descending order (0: none).
+struct Best {
+  uint64_t key;
+  uint64_t floor;                        // the k-th best; keys at or below it do not matter
+
+  __device__ __forceinline__ void clear() { key = floor = 0; }
+  // the wave's keys, one per lane, as the first list: a bitonic sort
+  __device__ __forceinline__ void sort(uint64_t mine, int lane, int k) {
+    key = mine;
+    merge<2>(lane);
+    merge<4>(lane);
+    merge<8>(lane);
+    merge<16>(lane);
+    merge<32>(lane);
+    merge<64>(lane);
+    floor = read_lane(key, k - 1);
+  }
+  // one key per lane: those above the floor go in one after the other
+  __device__ __forceinline__ void take(uint64_t mine, int lane, int k) {
+    uint64_t todo = __ballot(mine > floor);
+    while (todo) {
+      const uint64_t c = read_lane(mine, __builtin_ctzll(todo));
+      const int at = __builtin_popcountll(__ballot(key > c));
+      const uint64_t moved = ((uint64_t)(uint32_t)__builtin_amdgcn_mov_dpp((int)(key >> 32), 0x138, 0xf, 0xf, true) << 32) |
+                             (uint32_t)__builtin_amdgcn_mov_dpp((int)(uint32_t)key, 0x138, 0xf, 0xf, true);   // wave_shr 1
+      key = lane < at ? key : lane == at ? c : moved;
+      floor = read_lane(key, k - 1);
+      todo &= todo - 1;
+      todo &= __ballot(mine > floor);
+    }
+  }
+
+ private:
+  template <int N>
+  __device__ __forceinline__ void merge(int lane) {   // sorted runs of N / 2 -> sorted runs of N
+    flip<N>(lane);
+    if constexpr (N >= 64) step<16>(lane);
+    if constexpr (N >= 32) step<8>(lane);
+    if constexpr (N >= 16) step<4>(lane);
+    if constexpr (N >= 8) step<2>(lane);
+    if constexpr (N >= 4) step<1>(lane);
+  }
+  template <int N>
+  __device__ __forceinline__ void flip(int lane) {
+    const uint64_t other = xor_lane<N - 1>(key);
+    key = ((lane & (N / 2)) == 0) == (key > other) ? key : other;
+  }
+  template <int D>
+  __device__ __forceinline__ void step(int lane) {
+    const uint64_t other = xor_lane<D>(key);
+    key = ((lane & D) == 0) == (key > other) ? key : other;
+  }
+};
+
+// 16 bytes of a row
+template <typename T>
+struct Vec {
+  static constexpr int N = 16 / sizeof(T);
+  union {
+    uint4 raw;
+    T e[N];
+  };
+  __device__ Vec() {}
+};
+
+// One wave's part of a row, entries in ascending order.  The maximum is the wave's, so every e^(x - m) is at most 1 and all
+// terms of the entropy's sum have one sign; a step that brings no new maximum and nothing above the k-th best entry (one
+// compare of the lane's largest against the floor) adds up its terms and nothing else.
+struct Part {
+  float m = -3.402823466e38f, s = 0.f, u = 0.f;
+  int above = 0;
+  float floor = -INFINITY;               // value of the k-th best, or the maximum for k = 0
+  bool full = false;                     // k entries seen
+  Best best;
+
+  template <int N>
+  __device__ __forceinline__ void step(const float (&x)[N], int i0, int valid, int lane, int k, float xt, int t, int base, int span) {
+    float top = x[0];
+#pragma unroll
+    for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
+    if (!full || __ballot(top > floor)) news<N>(x, i0, valid, lane, k, top);
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+      const float z = x[j] - m, e = exp_neg(z);
+      s += e;
+      u = fmaf(e, fmaxf(z, -200.f), u);
+    }
+    // entries above x_t; equal ones count below index t.  base .. base + span: the wave's entries of this step
+    if (t >= base + span) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) above += j < valid && x[j] >= xt;
+    } else if (t < base) {
+#pragma unroll
+      for (int j = 0; j < N; ++j) above += x[j] > xt;
+    } else {
+#pragma unroll
+      for (int j = 0; j < N; ++j) above += j < valid && (x[j] > xt || (x[j] == xt && i0 + j < t));
+    }
+  }
+
+  template <int N>
+  __device__ __forceinline__ void news(const float (&x)[N], int i0, int valid, int lane, int k, float top) {
+    float w = top;
+    w = fmaxf(w, xor_lane<1>(w));
+    w = fmaxf(w, xor_lane<2>(w));
+    w = fmaxf(w, xor_lane<7>(w));
+    w = fmaxf(w, xor_lane<15>(w));
+    w = fmaxf(fmaxf(read_lane(w, 0), read_lane(w, 16)), fmaxf(read_lane(w, 32), read_lane(w, 48)));
+    if (w > m) {
+      // s and u to the new maximum: e^(x - w) = e^(x - m) e^d, (x - w) = (x - m) + d; d bounded as in the sums
+      const float d = fmaxf(m - w, -200.f), f = exp_neg(d);
+      u = f * fmaf(d, s, u);
+      s *= f;
+      m = w;
+    }
+    if (k == 0) {
+      floor = m;
+      full = true;
+      return;
+    }
+    uint64_t key[N];
+#pragma unroll
+    for (int j = 0; j < N; ++j) key[j] = j < valid ? key_of(x[j], i0 + j) : 0;
+    if (best.floor == 0 && read_lane(best.key, 0) == 0) {
+      // nothing held yet: the lanes' largest first, which sets a floor close to the final one
+      uint64_t mine = key[0];
+      int at = 0;
+#pragma unroll
+      for (int j = 1; j < N; ++j)
+        if (key[j] > mine) {
+          mine = key[j];
+          at = j;
+        }
+      best.sort(mine, lane, k);
+#pragma unroll
+      for (int j = 0; j < N; ++j) key[j] = j == at ? 0 : key[j];
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) best.take(key[j], lane, k);
+    full = best.floor != 0;
+    if (full) floor = key_value(best.floor);
+  }
+};
+
+// Longer rows: W waves per row, each a contiguous part of it in 16-byte loads from the first aligned entry on (the entries in
+// front of it and behind the last whole vector are single loads of the first and the last wave), joined in LDS.
+template <typename T, int W, int ROWS>
+__global__ void __launch_bounds__(64 * W * ROWS) scores_long_kernel(ScoreArgs p) {
+  constexpr int N = Vec<T>::N, kAhead = 4;
+  __shared__ float part_f[W * ROWS][3];
+  __shared__ int part_i[W * ROWS];
+  __shared__ uint64_t part_k[W * ROWS][W > 1 ? TONE_SCORES_MAX_K : 1];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = W > 1 ? wave % W : 0;
+  const int64_t n = (int64_t)blockIdx.x * ROWS + wave / W;
+  const bool in = n < p.n;
+  const int64_t row = !in ? -1 : p.rows ? p.rows[n] : n;
+  const bool here = row >= 0 && row < p.x_rows;
+  if (in && !here && wr == 0) write_none(p, n, lane, 64);
+  if constexpr (W == 1) {
+    if (!here) return;
+  }
+  Part a;
+  a.best.clear();
+  int t = -1;
+  float xt = 0.f;
+  if (here) {
+    const T* x = static_cast<const T*>(p.x) + row * p.stride;
+    t = p.tokens ? p.tokens[n] : -1;
+    if (t < 0 || t >= p.vocab) t = -1;
+    if (t >= 0) xt = load_elem(x + t);
+    const int head = min(p.vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+    const int vecs = (p.vocab - head) / N, each = (vecs + W - 1) / W;
+    const int v0 = min(vecs, wr * each), v1 = min(vecs, v0 + each);
+    const uint4* base = reinterpret_cast<const uint4*>(x + head);
+    for (int c = v0; c < v1; c += 64 * kAhead) {
+      Vec<T> v[kAhead];
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int i = c + 64 * q + lane;
+        if (i < v1) v[q].raw = base[i];
+      }
+#pragma unroll
+      for (int q = 0; q < kAhead; ++q) {
+        const int b = c + 64 * q;
+        if (b >= v1) break;
+        const bool ok = b + lane < v1;
+        float f[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[j] = ok ? load_elem(&v[q].e[j]) : -INFINITY;
+        a.step<N>(f, head + (b + lane) * N, ok ? N : 0, lane, p.k, xt, t, head + b * N, min(64, v1 - b) * N);
+      }
+    }
+    const int tail = head + vecs * N;
+    if (wr == W - 1 && tail < p.vocab) {
+      const int i = tail + lane;
+      const float one[1] = {i < p.vocab ? load_elem(x + i) : -INFINITY};
+      a.step<1>(one, i, i < p.vocab, lane, p.k, xt, t, tail, p.vocab - tail);
+    }
+    if (wr == 0 && head) {
+      const float one[1] = {lane < head ? load_elem(x + lane) : -INFINITY};
+      a.full = false;                    // lower indices than what is held: equal values have to be looked at
+      a.step<1>(one, lane, lane < head, lane, p.k, xt, t, 0, head);
     }
     for (int o = 32; o; o >>= 1) {
-      const uint64_t other = __shfl_xor((unsigned long long)best, o);
-      if (other > best) best = other;
-    }
-    last = best;
-    if (lane == 0) {
-      p.top_lp[n * p.k + i] = left ? key_value(best) - m - ls : -INFINITY;
-      p.top_ids[n * p.k + i] = (int32_t)~(uint32_t)best;
+      a.s += __shfl_xor(a.s, o);
+      a.u += __shfl_xor(a.u, o);
+      a.above += __shfl_xor(a.above, o);
     }
   }
+  if constexpr (W > 1) {
+    if (lane == 0) {
+      part_f[wave][0] = a.m;
+      part_f[wave][1] = a.s;
+      part_f[wave][2] = a.u;
+      part_i[wave] = a.above;
+    }
+    if (lane < p.k) part_k[wave][lane] = a.best.key;
+    __syncthreads();
+    if (wr != 0 || !here) return;
+    float m = a.m;
+    for (int w = 1; w < W; ++w) m = fmaxf(m, part_f[wave + w][0]);
+    float s = 0.f, u = 0.f;
+    a.above = 0;
+    for (int w = 0; w < W; ++w) {
+      const float d = fmaxf(part_f[wave + w][0] - m, -200.f), f = exp_neg(d);
+      u += f * fmaf(d, part_f[wave + w][1], part_f[wave + w][2]);
+      s += f * part_f[wave + w][1];
+      a.above += part_i[wave + w];
+    }
+    a.m = m;
+    a.s = s;
+    a.u = u;
+    if (p.k)
+      for (int w = 1; w < W; ++w) a.best.take(lane < p.k ? part_k[wave + w][lane] : 0, lane, p.k);
+  }
+  const bool left = a.s != 0.f;
+  const float ls = logf(a.s);
+  if (lane == 0) {
+    p.entropy[n] = left ? ls - a.u / a.s : 0.f;
+    if (p.tokens) {
+      p.logprob[n] = t < 0 ? 0.f : left ? xt - a.m - ls : -INFINITY;
+      p.rank[n] = t < 0 ? -1 : a.above;
+    }
+  }
+  if (lane < p.k) {
+    p.top_lp[n * p.k + lane] = left ? key_value(a.best.key) - a.m - ls : -INFINITY;
+    p.top_ids[n * p.k + lane] = key_index(a.best.key);
+  }
+}
+
+template <typename T, int E>
+void short_as(const ScoreArgs& p, hipStream_t st) {
+  hipLaunchKernelGGL((scores_short_kernel<T, E>), dim3((unsigned)((p.n + 31) / 32)), dim3(256), 0, st, p);
+}
+
+template <typename T>
+hipError_t launch_as(const ScoreArgs& p, hipStream_t st) {
+  if (p.vocab <= 64) {
+    switch ((p.vocab + 7) / 8) {
+      case 1: short_as<T, 1>(p, st); break;
+      case 2: short_as<T, 2>(p, st); break;
+      case 3: short_as<T, 3>(p, st); break;
+      case 4: short_as<T, 4>(p, st); break;
+      case 5: short_as<T, 5>(p, st); break;
+      case 6: short_as<T, 6>(p, st); break;
+      case 7: short_as<T, 7>(p, st); break;
+      default: short_as<T, 8>(p, st);
+    }
+    return hipGetLastError();
+  }
+  const int64_t steps = (p.vocab / Vec<T>::N + 63) / 64;     // 64-lane loads a row takes
+  if (steps >= 16 && p.n < 1024) hipLaunchKernelGGL((scores_long_kernel<T, 16, 1>), dim3((unsigned)p.n), dim3(1024), 0, st, p);
+  else if (steps >= 8) hipLaunchKernelGGL((scores_long_kernel<T, 4, 1>), dim3((unsigned)p.n), dim3(256), 0, st, p);
+  else hipLaunchKernelGGL((scores_long_kernel<T, 1, 4>), dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, p);
+  return hipGetLastError();
 }
 
 hipError_t launch_scores(const ScoreArgs& p, int type, hipStream_t st) {
-  const dim3 grid((unsigned)((p.n + 3) / 4));
   switch (type) {
-    case TONE_TYPE_FP32: hipLaunchKernelGGL(scores_kernel<float>, grid, dim3(256), 0, st, p); break;
-    case TONE_TYPE_FP16: hipLaunchKernelGGL(scores_kernel<__half>, grid, dim3(256), 0, st, p); break;
-    default: hipLaunchKernelGGL(scores_kernel<Bf16>, grid, dim3(256), 0, st, p);
+    case TONE_TYPE_FP32: return launch_as<float>(p, st);
+    case TONE_TYPE_FP16: return launch_as<__half>(p, st);
+    default: return launch_as<Bf16>(p, st);
   }
-  return hipGetLastError();
 }
 
 }  // namespace
@@ -121,11 +472,9 @@ using namespace tone;
 
 extern "C" {
 
-int64_t tone_token_scores_workspace(int64_t n, int vocab, int k) { return n < 0 || vocab <= 0 || k < 0 ? -1 : 0; }
-
 int tone_token_scores(int device, const void* x, int type, int64_t stride, int64_t x_rows, const int64_t* rows, int64_t n,
                       int vocab, const int32_t* tokens, int k, float* logprob, float* entropy, int32_t* rank,
-                      float* top_logprob, int32_t* top_ids, void* workspace, int64_t workspace_bytes, void* stream) {
+                      float* top_logprob, int32_t* top_ids, void* stream) {
   const char* what = "tone_token_scores";
   if (n < 0 || x_rows < 0 || vocab <= 0 || vocab > (1 << 24)) return refuse(what, "n, x_rows or vocab out of range");
   if (!known_type(type)) return refuse(what, "unknown element type");
@@ -135,9 +484,8 @@ int tone_token_scores(int device, const void* x, int type, int64_t stride, int64
   if (tokens && (!logprob || !rank)) return refuse(what, "tokens without logprob or rank");
   if (!rows && x_rows < n) return refuse(what, "fewer rows in x than outputs");
   if (stride < vocab && x_rows > 1) return refuse(what, "row stride < vocab");
-  if ((n + 3) / 4 > INT32_MAX) return refuse(what, "too many rows for one launch");
-  const int64_t need = tone_token_scores_workspace(n, vocab, k);
-  if (workspace_bytes < need || (need && !workspace)) return refuse(what, "workspace smaller than tone_token_scores_workspace");
+  if (!aligned(x, type)) return refuse(what, "x not aligned to its element type");
+  if (n > INT32_MAX) return refuse(what, "too many rows for one launch");
   ScoreArgs p{x, stride, x_rows, rows, n, vocab, k, tokens, tokens ? logprob : nullptr, entropy, tokens ? rank : nullptr,
               top_logprob, top_ids};
   return launch_on(device, what, [&] { return launch_scores(p, type, static_cast<hipStream_t>(stream)); });

@@ -28,6 +28,9 @@ __device__ __forceinline__ void store_elem(Bf16* p, float v) { *p = static_cast<
 
 inline bool known_type(int t) { return t == TONE_TYPE_FP32 || t == TONE_TYPE_FP16 || t == TONE_TYPE_BF16; }
 
+// whether a pointer lies on a whole element of its type
+inline bool aligned(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type == TONE_TYPE_FP32 ? 3 : 1)) == 0; }
+
 // The calling thread's device for the life of an entry point, the former one afterwards.
 class OnDevice {
  public:

@@ -255,10 +255,8 @@ def token_scores(x, tokens=None, k: int = 0, rows=None, stream=None) -> TokenSco
         if k:
             top = torch.empty(shape + (k,), dtype=torch.float32, device=dev)
             ids = torch.empty(shape + (k,), dtype=torch.int32, device=dev)
-        need = lib.tone_token_scores_workspace(n, vocab, k)
-        ws = torch.empty(need, dtype=torch.uint8, device=dev) if need else None
         _lib.check(lib.tone_token_scores(dev.index, x.data_ptr(), typ, stride, x_rows, _ptr(rows), n, vocab, _ptr(tokens), k,
-                                         _ptr(lp), entropy.data_ptr(), _ptr(rank), _ptr(top), _ptr(ids), _ptr(ws), need, st),
+                                         _ptr(lp), entropy.data_ptr(), _ptr(rank), _ptr(top), _ptr(ids), st),
                    "tone_token_scores")
     return TokenScores(lp, rank, entropy, top, ids)
 

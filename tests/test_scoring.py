@@ -186,8 +186,8 @@ def test_c_frames_slots_and_put_refuse():
 def test_c_token_scores_refuses():
     lib = _lib.load()
 
-    def call(x=P, typ=0, stride=5, x_rows=2, rows=None, n=2, vocab=5, tokens=P, k=2, lp=P, ent=P, top=P, ws=None, wb=0):
-        return lib.tone_token_scores(0, x, typ, stride, x_rows, rows, n, vocab, tokens, k, lp, ent, P, top, P, ws, wb, None)
+    def call(x=P, typ=0, stride=5, x_rows=2, rows=None, n=2, vocab=5, tokens=P, k=2, lp=P, ent=P, top=P):
+        return lib.tone_token_scores(0, x, typ, stride, x_rows, rows, n, vocab, tokens, k, lp, ent, P, top, P, None)
     _refused(call(x=None), "null")
     _refused(call(ent=None), "null")
     _refused(call(top=None), "null")
@@ -198,11 +198,9 @@ def test_c_token_scores_refuses():
     _refused(call(x_rows=1), "fewer rows")
     _refused(call(stride=4), "stride")
     _refused(call(n=-1), "range")
-    assert lib.tone_token_scores_workspace(-1, 5, 2) == -1
-    need = lib.tone_token_scores_workspace(1, 131072, 20)
-    if need:
-        _refused(call(n=1, vocab=131072, stride=131072, k=20), "workspace")
-        _refused(call(n=1, vocab=131072, stride=131072, k=20, ws=P, wb=need - 1), "workspace")
+    _refused(call(n=1 << 32, x_rows=1 << 32), "one launch")
+    _refused(call(x=ctypes.c_void_p(4098)), "aligned")
+    _refused(call(x=ctypes.c_void_p(4097), typ=2), "aligned")
 
 
 def test_c_ctc_align_refuses():
@@ -231,5 +229,5 @@ def test_c_empty_calls_do_nothing():
     lib = _lib.load()
     assert lib.tone_frames_slots(0, None, 3, 4, 3, 8, 4, None, None, None, None, 0, None, 2, None) == 0
     assert lib.tone_frames_put(0, None, 0, 5, None, 0, 5, None, 0, 5, 9, None) == 0
-    assert lib.tone_token_scores(0, None, 0, 5, 0, None, 0, 5, None, 0, None, None, None, None, None, None, 0, None) == 0
+    assert lib.tone_token_scores(0, None, 0, 5, 0, None, 0, 5, None, 0, None, None, None, None, None, None) == 0
     assert lib.tone_ctc_align(0, None, 0, 5, 0, 0, None, 0, 6, 5, 4, None, 3, None, None, None, None, None, None, None, 0, None) == 0
