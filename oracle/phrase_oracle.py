@@ -80,7 +80,7 @@ def align(frames, tokens, blank):
     def emit(t, s):
         if not 0 <= lab[s] < vocab or (s % 2 and lab[s] == blank):
             return -np.inf
-        return frames[t, lab[s]] if np.isfinite(frames[t, lab[s]]) else -np.inf
+        return frames[t, lab[s]] if abs(frames[t, lab[s]]) < 6e4 else -np.inf      # (NaN compares false)
 
     if f == 0:
         ok = not tokens
