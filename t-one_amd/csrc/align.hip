@@ -39,47 +39,36 @@ struct AlignArgs {
   float *score, *total;                 // total: or nullptr
   int32_t *labels, *spans;              // [batch][frames], [batch][most][2]
   uint32_t* words;                      // [batch][groups][W][64]
-  int columns, direct;                  // columns staged per frame; direct: column = label, else 0 = blank, 1 + i = token i
+  int columns, direct;                  // columns staged per frame: the labels (direct), or 0 = blank, 1 + i = token i
   int ahead;                            // frames per stage
 };
 
 constexpr float kClosed = 6e4f;         // entries of this size and more (masks of lowest values) count as -inf
-constexpr int kZero = -(1 << 30);       // exponents of probability 0 end here ...
-constexpr int kShut = kZero / 2;        // ... after a factor of 0; what passes one stays below kZero / 4 and is taken for 0
 constexpr int kRefresh = 32;            // frames between two refreshes of the waves' overlap
-constexpr int kStage = 8;               // loads of the next stage a lane has in flight during a stage
+constexpr int kLoaders = 4;             // waves that stage the frames
+constexpr int kBatch = 8;               // loads a loader lane has in flight
+// exponents of probability 0: a factor of 0 takes kShut off, what passed one stays below kNone and counts as 0.  They are
+// held above kZero every 32 frames, and 32 factors of 0 from there do not leave 31 bits.
+constexpr int kShut = -(1 << 25), kNone = -(1 << 24), kZero = -(1 << 29);
 
 template <int W_, int R_>
 struct Shape {
   static constexpr int W = W_, R = R_;
-  static constexpr int HL = W > 1 ? (2 * kRefresh + R - 1) / R : 0;   // lanes that repeat the wave below
-  static constexpr int N = (64 - HL) * R;                              // states a wave adds
+  static constexpr int HL = W > 1 ? 2 * kRefresh / R : 0;   // lanes that repeat the wave below
+  static constexpr int N = (64 - HL) * R;                    // states a wave adds
   static constexpr int kStates = (W - 1) * N + 64 * R;
   static constexpr int kBits = R / 2 * 3;
-  static constexpr int F = 32 / kBits;                                 // frames per word
+  static constexpr int F = R == 2 ? 8 : R == 4 ? 4 : 2;      // frames per word
+  static_assert(F * kBits <= 32 && kRefresh % F == 0 && 2 * kRefresh % R == 0, "whole words and lanes");
 };
 
-__device__ __forceinline__ double shift_in(double v, double edge) {   // lane i: lane i - 1's value, lane 0: edge
-  const int64_t a = __double_as_longlong(v), e = __double_as_longlong(edge);
-  const int lo = __builtin_amdgcn_update_dpp((int)e, (int)a, 0x138, 0xf, 0xf, false);   // wave_shr 1
-  const int hi = __builtin_amdgcn_update_dpp((int)(e >> 32), (int)(a >> 32), 0x138, 0xf, 0xf, false);
-  return __longlong_as_double(((int64_t)hi << 32) | (uint32_t)lo);
-}
+// lane i: lane i - 1's value (wave_shr 1); lane 0 keeps `edge`'s
 __device__ __forceinline__ int shift_in(int v, int edge) { return __builtin_amdgcn_update_dpp(edge, v, 0x138, 0xf, 0xf, false); }
 __device__ __forceinline__ float shift_in(float v, float edge) {
   return __int_as_float(shift_in(__float_as_int(v), __float_as_int(edge)));
 }
-
-// the larger of two numbers that are no NaN (fmax puts a quieting v_max in front of each operand)
-__device__ __forceinline__ double larger(double a, double b) {
-  double r;
-  asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-  return r;
-}
-// one bit more at the low end: word + word + carry, one v_addc behind the compare
-__device__ __forceinline__ void push(uint32_t& word, bool bit) {
-  unsigned out;
-  word = __builtin_addc(word, word, (unsigned)bit, &out);
+__device__ __forceinline__ double shift_in(double v, double edge) {
+  return __hiloint2double(shift_in(__double2hiint(v), __double2hiint(edge)), shift_in(__double2loint(v), __double2loint(edge)));
 }
 
 // a probability e^v as mantissa in [0.7, 1.42) and exponent: v log2 e in two terms, so the mantissa is off by a few 2^-24
@@ -95,270 +84,252 @@ __device__ __forceinline__ Prob prob_of(float v) {
   return {__builtin_amdgcn_exp2f(f), (int)n};
 }
 
-// The frames of a sequence, staged `ahead` at a time: stage() issues the loads of the next ones, put() writes what came.
-template <class SH, bool SUM>
+// What is staged: [2][ahead][columns + 1] entries of 8 bytes, a double (best path) or a Prob (sum); the last column is closed.
 struct Frames {
   const AlignArgs p;
-  const int b, n, lane, wave;
+  const int b, n;
   const int32_t* tok;
-  char* buf;                            // [2][ahead][columns + 1]: the last column is closed
-  int64_t row, row_after;               // lane f: row of frame f of the stage under way / of the one behind it
-  float got[kStage];
-
-  static constexpr int kEntry = SUM ? 8 : 4;
+  char* buf;
 
   __device__ Frames(const AlignArgs& p_, int b_, int n_, char* buf_)
-      : p(p_), b(b_), n(n_), lane(threadIdx.x & 63), wave(__builtin_amdgcn_readfirstlane(threadIdx.x >> 6)), tok(p_.tokens + (int64_t)b_ * p_.most), buf(buf_) {}
+      : p(p_), b(b_), n(n_), tok(p_.tokens + (int64_t)b_ * p_.most), buf(buf_) {}
 
-  __device__ __forceinline__ int per_frame() const { return (p.columns + 1) * kEntry; }
-  __device__ __forceinline__ char* at(int stage, int f) const { return buf + ((stage & 1) * p.ahead + f) * per_frame(); }
-  __device__ __forceinline__ int column(int i, int len) const {        // of token i of the sequence
+  __device__ __forceinline__ char* at(int stage, int f) const { return buf + ((stage & 1) * p.ahead + f) * ((p.columns + 1) * 8); }
+  __device__ __forceinline__ int column(int i, int len) const {        // byte offset of token i of the sequence
     if (i >= len) return 0;                                            // a state behind the last: anything
     const int t = tok[i];
-    return t < 0 || t >= p.vocab || t == p.blank ? p.columns : p.direct ? t : i + 1;
+    return 8 * (t < 0 || t >= p.vocab || t == p.blank ? p.columns : p.direct ? t : i + 1);
   }
-  __device__ __forceinline__ int blank_column() const { return p.direct ? p.blank : 0; }
-  __device__ __forceinline__ void rows_from(int t0) {
-    row_after = -1;
-    if (p.rows && lane < p.ahead && t0 + lane < n) row_after = p.rows[(int64_t)b * p.frames + t0 + lane];
-  }
+  __device__ __forceinline__ int blank_column() const { return p.direct ? 8 * p.blank : 0; }
   __device__ __forceinline__ float value(int64_t off) const {
-    float v;
-    if (p.type == TONE_TYPE_FP32) v = load_elem(static_cast<const float*>(p.x) + off);
-    else if (p.type == TONE_TYPE_FP16) v = load_elem(static_cast<const __half*>(p.x) + off);
-    else v = load_elem(static_cast<const Bf16*>(p.x) + off);
-    return v;
+    if (p.type == TONE_TYPE_FP32) return load_elem(static_cast<const float*>(p.x) + off);
+    if (p.type == TONE_TYPE_FP16) return load_elem(static_cast<const __half*>(p.x) + off);
+    return load_elem(static_cast<const Bf16*>(p.x) + off);
   }
-  // The wave's part of a stage is the frames wave, wave + W, ... in blocks of 64 columns (the closed one among them), item by
-  // item in that order.  The first kStage items are under way during the stage before; only wide frames have more.
-  __device__ __forceinline__ float item(int t0, int f, int c0) const {
-    const int c = c0 + lane;
-    int64_t off = (int64_t)b * p.batch_stride + (int64_t)(t0 + f) * p.stride;
-    bool here = c < p.columns;
-    if (p.rows) {
-      const int64_t r = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), f) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, f);
-      here = here && r >= 0 && r < p.x_rows;
-      off = r * p.stride;
-    }
-    if (!here) return -INFINITY;
-    const int label = p.direct ? c : c == 0 ? p.blank : tok[c - 1];
-    return label >= 0 && label < p.vocab ? value(off + label) : -INFINITY;
-  }
-  __device__ __forceinline__ void write(int stage, int f, int c0, float v) const {
-    const int c = c0 + lane;
-    v = fabsf(v) < kClosed ? v : -INFINITY;
-    if (c > p.columns) return;
-    if constexpr (SUM) reinterpret_cast<Prob*>(at(stage, f))[c] = prob_of(v);
-    else reinterpret_cast<float*>(at(stage, f))[c] = v;
-  }
-  __device__ __forceinline__ void load(int t0) {
-    row = row_after;
-    rows_from(t0 + p.ahead);
-    int f = wave, c0 = 0;
+  // frames t0 ... of the sequence: items of one frame and 64 columns, dealt to the loader waves
+  template <bool SUM>
+  __device__ __forceinline__ void fill(int stage, int t0, int loader, int lane) const {
+    const int blocks = p.columns / 64 + 1, frames = min(p.ahead, n - t0), items = frames * blocks;
+    for (int i0 = loader; i0 < items; i0 += kLoaders * kBatch) {
+      int64_t row[kBatch];
+      float v[kBatch];
 #pragma unroll
-    for (int j = 0; j < kStage; ++j) {
-      if (f < p.ahead && t0 + f < n) got[j] = item(t0, f, c0);
-      next(f, c0);
-    }
-  }
-  __device__ __forceinline__ void put(int stage, int t0) {
-    int f = wave, c0 = 0;
+      for (int j = 0; j < kBatch; ++j) {
+        const int f = min(frames - 1, (i0 + j * kLoaders) / blocks);
+        row[j] = p.rows ? p.rows[(int64_t)b * p.frames + t0 + f] : t0 + f;
+      }
 #pragma unroll
-    for (int j = 0; j < kStage; ++j) {
-      if (f < p.ahead && t0 + f < n) write(stage, f, c0, got[j]);
-      next(f, c0);
-    }
-    while (f < p.ahead && t0 + f < n) {
-      write(stage, f, c0, item(t0, f, c0));
-      next(f, c0);
-    }
-  }
-  __device__ __forceinline__ void next(int& f, int& c0) const {
-    c0 += 64;
-    if (c0 > p.columns) {
-      c0 = 0;
-      f += SH::W;
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kLoaders, f = i / blocks, c = (i - f * blocks) * 64 + lane;
+        const bool here = i < items && c < p.columns && (!p.rows || (row[j] >= 0 && row[j] < p.x_rows));
+        int label = c;
+        if (!p.direct) label = here && c ? tok[c - 1] : p.blank;
+        v[j] = -INFINITY;
+        if (here && label >= 0 && label < p.vocab) v[j] = value((p.rows ? 0 : (int64_t)b * p.batch_stride) + row[j] * p.stride + label);
+      }
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j) {
+        const int i = i0 + j * kLoaders, f = i / blocks, c = (i - f * blocks) * 64 + lane;
+        if (i >= items || c > p.columns) continue;
+        const float w = fabsf(v[j]) < kClosed ? v[j] : -INFINITY;
+        if constexpr (SUM) reinterpret_cast<Prob*>(at(stage, f))[c] = prob_of(w);
+        else reinterpret_cast<double*>(at(stage, f))[c] = w;
+      }
     }
   }
 };
 
-// one frame of the best path: the lane's states to the next frame's, highest first (each needs the ones below as they were)
+// The lane's states, and one frame: the highest first, since each needs the ones below it as they were.
 template <class SH>
-struct BestStep {
+struct Best {
+  static constexpr int Q = SH::R / 2;
   double a[SH::R];
-  double closed[SH::R / 2];             // 0 where token q may follow the token before it directly, else -inf
-  int col[SH::R / 2];                   // byte offsets
+  double below;                         // the state below the lane's first; lane 0: -inf
+  int col[Q];
+  bool apart[Q];                        // token q may follow the token before it directly
   uint32_t word;
 
-  __device__ __forceinline__ void step(const char* frame, int blank, double edge) {
-    const double eb = *reinterpret_cast<const float*>(frame + blank);
-    double et[SH::R / 2];
+  struct Row {
+    double blank, tok[Q];
+  };
+  __device__ __forceinline__ void read(Row& r, const char* frame, int blank) const {
+    r.blank = *reinterpret_cast<const double*>(frame + blank);
 #pragma unroll
-    for (int q = 0; q < SH::R / 2; ++q) et[q] = *reinterpret_cast<const float*>(frame + col[q]);
-    const double below = shift_in(a[SH::R - 1], edge);
+    for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const double*>(frame + col[q]);
+  }
+  __device__ __forceinline__ void begin(const Row& r, int base) {
 #pragma unroll
-    for (int q = SH::R / 2 - 1; q >= 0; --q) {
-      const double stay = a[2 * q + 1], one = a[2 * q], two = (q ? a[q ? 2 * q - 1 : 0] : below) + closed[q];
-      const double m = larger(stay, one);
-      push(word, one > stay);
-      push(word, two > m);
-      a[2 * q + 1] = larger(m, two) + et[q];
-      const double from = q ? a[q ? 2 * q - 1 : 0] : below;
-      push(word, from > one);
-      a[2 * q] = larger(one, from) + eb;
+    for (int i = 0; i < SH::R; ++i) a[i] = -INFINITY;
+    below = -INFINITY;
+    word = 0;
+    if (base == 0) {
+      a[0] = r.blank;
+      a[1] = r.tok[0];
+    }
+  }
+  __device__ __forceinline__ void step(const Row& r) {
+    below = shift_in(a[SH::R - 1], below);
+#pragma unroll
+    for (int q = Q - 1; q >= 0; --q) {
+      const double stay = a[2 * q + 1], one = a[2 * q], from = q ? a[q ? 2 * q - 1 : 0] : below;
+      // not apart: a NaN, which no compare prefers and v_max_f64 passes over
+      const double two = __hiloint2double(apart[q] ? __double2hiint(from) : 0x7ff80000, __double2loint(from));
+      double m, token, blank;
+      uint64_t c0, c1, c2;
+      // one by hand: (a) v_max_f64 without the quieting of operands that fmax brings, (b) each compare's mask pushed into
+      // the word by one add with carry, two instructions at least behind the compare as gfx950 demands of masks
+      asm("v_cmp_gt_f64_e64 %[c1], %[one], %[stay]\n\t"
+          "v_cmp_gt_f64_e64 %[c0], %[from], %[one]\n\t"
+          "v_max_f64 %[m], %[stay], %[one]\n\t"
+          "v_max_f64 %[blank], %[one], %[from]\n\t"
+          "v_cmp_gt_f64_e64 %[c2], %[two], %[m]\n\t"
+          "v_max_f64 %[token], %[m], %[two]\n\t"
+          "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c1]\n\t"
+          "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c2]\n\t"
+          "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c0]"
+          : [word] "+v"(word), [m] "=&v"(m), [blank] "=&v"(blank), [token] "=&v"(token), [c0] "=&s"(c0), [c1] "=&s"(c1), [c2] "=&s"(c2)
+          : [stay] "v"(stay), [one] "v"(one), [two] "v"(two), [from] "v"(from)
+          : "vcc");
+      a[2 * q + 1] = token + r.tok[q];
+      a[2 * q] = blank + r.blank;
     }
   }
 };
 
-// the same for the sum over paths
 template <class SH>
-struct SumStep {
-  float m[SH::R];
-  int e[SH::R];
-  int closed[SH::R / 2];                // 0 or kShut
-  int col[SH::R / 2];
+struct Sum {
+  static constexpr int Q = SH::R / 2;
+  float m[SH::R], below_m;
+  int e[SH::R], below_e;
+  int col[Q];
+  int shut[Q];                          // 0, or kShut where token q must not follow the token before it directly
 
-  __device__ __forceinline__ void step(const char* frame, int blank, float edge_m, int edge_e) {
-    const Prob pb = *reinterpret_cast<const Prob*>(frame + blank);
-    Prob pt[SH::R / 2];
+  struct Row {
+    Prob blank, tok[Q];
+  };
+  __device__ __forceinline__ void read(Row& r, const char* frame, int blank) const {
+    r.blank = *reinterpret_cast<const Prob*>(frame + blank);
 #pragma unroll
-    for (int q = 0; q < SH::R / 2; ++q) pt[q] = *reinterpret_cast<const Prob*>(frame + col[q]);
-    const float below_m = shift_in(m[SH::R - 1], edge_m);
-    const int below_e = shift_in(e[SH::R - 1], edge_e);
+    for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const Prob*>(frame + col[q]);
+  }
+  __device__ __forceinline__ void begin(const Row& r, int base) {
 #pragma unroll
-    for (int q = SH::R / 2 - 1; q >= 0; --q) {
+    for (int i = 0; i < SH::R; ++i) {
+      m[i] = 1.f;
+      e[i] = kZero;
+    }
+    below_m = 1.f;
+    below_e = kZero;
+    if (base == 0) {
+      m[0] = r.blank.m;
+      e[0] = r.blank.e;
+      m[1] = r.tok[0].m;
+      e[1] = r.tok[0].e;
+    }
+  }
+  __device__ __forceinline__ void step(const Row& r) {
+    below_m = shift_in(m[SH::R - 1], below_m);
+    below_e = shift_in(e[SH::R - 1], below_e);
+#pragma unroll
+    for (int q = Q - 1; q >= 0; --q) {
       const float fm = q ? m[q ? 2 * q - 1 : 0] : below_m;
       const int fe = q ? e[q ? 2 * q - 1 : 0] : below_e;
       {
-        const int e2 = fe + closed[q], hi = max(max(e[2 * q + 1], e[2 * q]), e2);
+        const int e2 = fe + shut[q], hi = max(max(e[2 * q + 1], e[2 * q]), e2);
         const float sum = (ldexpf(m[2 * q + 1], e[2 * q + 1] - hi) + ldexpf(m[2 * q], e[2 * q] - hi)) + ldexpf(fm, e2 - hi);
-        m[2 * q + 1] = sum * pt[q].m;
-        e[2 * q + 1] = max(hi + pt[q].e, kZero);
+        m[2 * q + 1] = sum * r.tok[q].m;
+        e[2 * q + 1] = hi + r.tok[q].e;
       }
       const int hi = max(e[2 * q], fe);
-      m[2 * q] = (ldexpf(m[2 * q], e[2 * q] - hi) + ldexpf(fm, fe - hi)) * pb.m;
-      e[2 * q] = max(hi + pb.e, kZero);
+      m[2 * q] = (ldexpf(m[2 * q], e[2 * q] - hi) + ldexpf(fm, fe - hi)) * r.blank.m;
+      e[2 * q] = hi + r.blank.e;
     }
   }
-  // a frame multiplies a mantissa by 0.7 to 4.3, so 32 frames stay far inside fp32
+  // a frame multiplies a mantissa by 0.7 to 4.3: 32 frames stay far inside fp32
   __device__ __forceinline__ void renormalize() {
 #pragma unroll
     for (int r = 0; r < SH::R; ++r) {
-      const int x = __builtin_amdgcn_frexp_expf(m[r]);
+      e[r] = max(e[r] + __builtin_amdgcn_frexp_expf(m[r]), kZero);
       m[r] = __builtin_amdgcn_frexp_mantf(m[r]);
-      e[r] = max(e[r] + x, kZero);
     }
   }
 };
 
-// Runs `step(stage, frame)` for all frames of the sequence: stages the frames, and refreshes the overlap of the waves.
-template <class SH, bool SUM, class Step, class Refresh>
-__device__ __forceinline__ void over_frames(Frames<SH, SUM>& fr, bool active, Step&& step, Refresh&& refresh) {
-  const int n = fr.n, ahead = fr.p.ahead;
-  fr.rows_from(0);
-  fr.load(0);
-  fr.put(0, 0);
+// Takes `st` through the frames of a sequence (n > 0).  word(g) after the last frame of every group g of F frames and after
+// the last one, refresh(write, half) every kRefresh frames.  The loader waves fill the next stage meanwhile.
+template <class SH, bool SUM, class State, class Word, class Refresh>
+__device__ __forceinline__ void over_frames(const Frames& fr, State& st, int wave, int lane, int base, bool active, Word&& word, Refresh&& refresh) {
+  constexpr int F = SH::F;
+  const int n = fr.n, ahead = fr.p.ahead, blank = fr.blank_column(), pitch = (fr.p.columns + 1) * 8;
+  if (wave >= SH::W) fr.fill<SUM>(0, 0, wave - SH::W, lane);
   __syncthreads();
   for (int t0 = 0, stage = 0; t0 < n; t0 += ahead, ++stage) {
     const bool more = t0 + ahead < n;
-    if (more) fr.load(t0 + ahead);
-    const int m = min(ahead, n - t0);
-    if (active)
-      for (int f = 0; f < m; ++f) step(stage, f, t0 + f);
-    if (more) {
-      fr.put(stage + 1, t0 + ahead);
-      const bool now = ((t0 + ahead) & (kRefresh - 1)) == 0;
-      if (now) refresh(true, ((t0 + ahead) / kRefresh) & 1);
-      __syncthreads();
-      if (now) refresh(false, ((t0 + ahead) / kRefresh) & 1);
+    const int half = ((t0 + ahead) / kRefresh) & 1;
+    const bool now = more && ((t0 + ahead) & (kRefresh - 1)) == 0;
+    if (wave >= SH::W) {
+      if (more) fr.fill<SUM>(stage + 1, t0 + ahead, wave - SH::W, lane);
+    } else if (active) {
+      const int m = min(ahead, n - t0);
+      const char* frame = fr.at(stage, 0);
+      typename State::Row r, next;
+      st.read(r, frame, blank);
+      int f = 0;
+      if (t0 == 0) {
+        st.begin(r, base);
+        f = 1;
+        frame += pitch;
+        if (m > 1) st.read(r, frame, blank);
+        if (F == 1 || n == 1) word(0);
+      }
+      while (f < m) {
+        // up to the end of the word, the next frame's entries under way
+        const int end = min(m, (f & ~(F - 1)) + F);
+        if (end - f == F) {
+#pragma unroll
+          for (int i = 0; i < F; ++i) {
+            frame += pitch;
+            if (i + 1 < F || end < m) st.read(next, frame, blank);
+            st.step(r);
+            r = next;
+          }
+          f = end;
+        } else {
+          for (; f < end; ++f) {
+            frame += pitch;
+            if (f + 1 < m) st.read(next, frame, blank);
+            st.step(r);
+            r = next;
+          }
+        }
+        if ((f & (F - 1)) == 0 || t0 + f == n) word((t0 + f - 1) / F);
+      }
+      if (now) refresh(true, half);
     }
+    if (more) __syncthreads();
+    if (now && active && wave < SH::W) refresh(false, half);
   }
 }
 
+// The path from its last state, by one wave.  `at` counts the states as the words hold them: 64 R of wave 0, of wave 1, ...
 template <class SH>
-__device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
-  constexpr int W = SH::W, R = SH::R, HL = SH::HL;
-  __shared__ double s_end[2];
-  __shared__ double s_over[2][W][W > 1 ? HL * R : 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
-  const bool active = wave * SH::N <= 2 * L;
-  const int64_t groups = (p.frames + SH::F - 1) / SH::F;
-  uint32_t* words = p.words + (int64_t)b * groups * W * 64;
-  int32_t* labels = p.labels + (int64_t)b * p.frames;
-  int32_t* spans = p.spans + (int64_t)b * p.most * 2;
-  const int32_t* tok = p.tokens + (int64_t)b * p.most;
-  if (threadIdx.x < 2) s_end[threadIdx.x] = n == 0 && L == 0 && threadIdx.x == 0 ? 0.0 : -INFINITY;   // [0]: last blank, [1]: last token
-  if (n > 0) {
-    Frames<SH, false> fr(p, b, n, lds);
-    BestStep<SH> st;
-    st.word = 0;
-#pragma unroll
-    for (int r = 0; r < R; ++r) st.a[r] = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < R / 2; ++q) {
-      const int i = (base >> 1) + q;
-      st.col[q] = fr.column(i, L) * 4;
-      st.closed[q] = i > 0 && i < L && tok[i] == tok[i - 1] ? -INFINITY : 0.0;
-    }
-    const int blank = fr.blank_column() * 4;
-    int held = 0;
-    uint32_t* out = words + wave * 64 + lane;
-    // before the first frame: a state in front of the first, from which blank 0 (one on) and token 0 (two on) are reached
-    double edge = wave == 0 ? 0.0 : -INFINITY;
-    over_frames<SH, false>(
-        fr, active,
-        [&](int stage, int f, int t) {
-          st.step(fr.at(stage, f), blank, edge);
-          edge = -INFINITY;
-          if (++held == SH::F || t == n - 1) {
-            *out = st.word;
-            out += W * 64;
-            st.word = 0;
-            held = 0;
-          }
-        },
-        [&](bool write, int half) {
-          if constexpr (W > 1) {
-            if (write) {
-              if (lane >= 64 - HL)
-#pragma unroll
-                for (int r = 0; r < R; ++r) s_over[half][wave][(lane - (64 - HL)) * R + r] = st.a[r];
-            } else if (wave > 0 && lane < HL) {
-#pragma unroll
-              for (int r = 0; r < R; ++r) st.a[r] = s_over[half][wave - 1][lane * R + r];
-            }
-          }
-        });
-    __syncthreads();                     // s_end's first values are in place
-    if (active && (wave == 0 || lane >= HL)) {
-#pragma unroll
-      for (int r = 0; r < R; ++r) {
-        if (base + r == 2 * L) s_end[0] = st.a[r];
-        if (base + r == 2 * L - 1) s_end[1] = st.a[r];
-      }
-    }
-    __threadfence_block();
-  }
-  __syncthreads();
-  const double at_blank = s_end[0], at_token = s_end[1], score = fmax(at_blank, at_token);
-  const bool alive = score > -INFINITY;
-  for (int t = (alive ? n : 0) + threadIdx.x; t < p.frames; t += 64 * W) labels[t] = -1;
-  for (int i = (alive ? 2 * L : 0) + threadIdx.x; i < 2 * p.most; i += 64 * W) spans[i] = -1;
-  if (threadIdx.x == 0) p.score[b] = (float)score;
-  if (!alive || n == 0 || wave > 0) return;
-  // the path from its end: the state is uniform, wave w_'s lane l_'s state r_
-  int s = at_token > at_blank ? 2 * L - 1 : 2 * L, w_ = 0, l_, r_;
+__device__ __forceinline__ void trace(const AlignArgs& p, int s, int n, const uint32_t* words, const int32_t* tok, int32_t* labels, int32_t* spans) {
+  constexpr int W = SH::W, R = SH::R, F = SH::F, kAhead = W > 4 ? 4 : 8, kLane = R == 2 ? 1 : R == 4 ? 2 : 3;
+  constexpr int kOver = SH::HL * R;
+  // steps back by the state's bits: even states (blank) bit 0; odd ones bit 2 over bit 1 (token: c1, c2): 2 if c2 else c1
+  constexpr uint32_t kSteps = 0xa5a04444u;
+  static_assert(R <= 8, "kLane");
+  const int lane = threadIdx.x & 63;
+  int at;
   {
-    int rest = s;
+    int w = 0, rest = s;
     while (rest >= 64 * R) {
       rest -= SH::N;
-      ++w_;
+      ++w;
     }
-    l_ = rest / R;
-    r_ = rest - l_ * R;
+    at = w * 64 * R + rest;
   }
-  int t = n - 1, path = 0, above = -1;
-  constexpr int kAhead = 8;
+  int path = 0, above = -1;
   uint32_t cur[kAhead][W], nxt[kAhead][W];
   auto fetch = [&](uint32_t (&to)[kAhead][W], int g0) {     // groups g0, g0 - 1, ...
 #pragma unroll
@@ -366,37 +337,29 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
 #pragma unroll
       for (int w = 0; w < W; ++w) to[i][w] = g0 - i >= 0 ? words[((int64_t)(g0 - i) * W + w) * 64 + lane] : 0;
   };
-  int g = t / SH::F;
+  int g = (n - 1) / F;
   fetch(cur, g);
   while (g >= 0) {
     fetch(nxt, g - kAhead);
 #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
       if (g - i < 0) continue;
-      const int first = (g - i) * SH::F;
-      int at = 0;                        // bits of the frames behind t in the word
-      for (; t >= first; --t, at += SH::kBits) {
-        uint32_t word = __builtin_amdgcn_readlane(cur[i][0], l_);
+      const int first = (g - i) * F, last = min(n - 1, first + F - 1);
+      int drop = 0;                      // bits of the frames behind t in the word
+      for (int t = last; t >= first; --t, drop += SH::kBits) {
+        uint32_t word = __builtin_amdgcn_readlane(cur[i][0], (at >> kLane) & 63);
 #pragma unroll
         for (int w = 1; w < W; ++w)
-          if (w_ == w) word = __builtin_amdgcn_readlane(cur[i][w], l_);
-        const uint32_t bits = word >> (at + 3 * (r_ >> 1));
-        const int how = r_ & 1 ? (bits & 2 ? 2 : (bits >> 2) & 1) : bits & 1;
+          if (at >= w * 64 * R) word = __builtin_amdgcn_readlane(cur[i][w], (at >> kLane) & 63);
         path = lane == (t & 63) ? s : path;
+        const uint32_t bits = (word >> (drop + 3 * ((at >> 1) & (R / 2 - 1)))) & 7;
+        const int how = (kSteps >> (2 * bits + 16 * (at & 1))) & 3;
         const int now = s;
         s -= how;
-        r_ -= how;
-        if (r_ < 0) {
-          r_ += R;
-          --l_;
-          if (W > 1 && w_ > 0 && l_ < HL) {
-            --w_;
-            l_ += 64 - HL;
-          }
-        }
+        at -= how;
+        if (W > 1 && at >= 64 * R && (at & (64 * R - 1)) < kOver) at -= kOver;    // the wave below has it
         if ((t & 63) == 0) {             // frames t .. t + 63 are known, and the state before them
-          const int mine = t + lane, before = t ? s : -1;
-          const int prev = shift_in(path, before);
+          const int mine = t + lane, prev = shift_in(path, t ? s : -1);
           int next = __shfl_down(path, 1);
           if (lane == 63) next = above;
           if (mine == n - 1) next = -1;
@@ -418,84 +381,122 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
 }
 
 template <class SH>
+__device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
+  constexpr int W = SH::W, R = SH::R, HL = SH::HL, kThreads = 64 * (W + kLoaders);
+  __shared__ double s_end[2];
+  __shared__ double s_over[2][W][W > 1 ? HL * R : 1];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
+  const bool active = wave < W && wave * SH::N <= 2 * L;
+  uint32_t* words = p.words + (int64_t)b * ((p.frames + SH::F - 1) / SH::F) * W * 64;
+  int32_t* labels = p.labels + (int64_t)b * p.frames;
+  int32_t* spans = p.spans + (int64_t)b * p.most * 2;
+  const int32_t* tok = p.tokens + (int64_t)b * p.most;
+  if (threadIdx.x < 2) s_end[threadIdx.x] = n == 0 && L == 0 && threadIdx.x == 0 ? 0.0 : -INFINITY;   // [0]: last blank, [1]: last token
+  if (n > 0) {
+    const Frames fr(p, b, n, lds);
+    Best<SH> st;
+#pragma unroll
+    for (int q = 0; q < R / 2; ++q) {
+      const int i = (base >> 1) + q;
+      st.col[q] = wave < W ? fr.column(i, L) : 0;
+      st.apart[q] = !(wave < W && i > 0 && i < L && tok[i] == tok[i - 1]);
+    }
+    uint32_t* out = words + wave * 64 + lane;
+    over_frames<SH, false>(
+        fr, st, wave, lane, base, active,
+        [&](int g) {
+          out[(int64_t)g * (W * 64)] = st.word;
+          st.word = 0;
+        },
+        [&](bool write, int half) {
+          if constexpr (W > 1) {
+            if (write) {
+              if (lane >= 64 - HL)
+#pragma unroll
+                for (int r = 0; r < R; ++r) s_over[half][wave][(lane - (64 - HL)) * R + r] = st.a[r];
+            } else if (wave > 0 && lane < HL) {
+#pragma unroll
+              for (int r = 0; r < R; ++r) st.a[r] = s_over[half][wave - 1][lane * R + r];
+            }
+          }
+        });
+    if (active && (wave == 0 || lane >= HL)) {
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (base + r == 2 * L) s_end[0] = st.a[r];
+        if (base + r == 2 * L - 1) s_end[1] = st.a[r];
+      }
+    }
+    __threadfence_block();
+  }
+  __syncthreads();
+  const double at_blank = s_end[0], at_token = s_end[1], score = fmax(at_blank, at_token);
+  const bool alive = score > -INFINITY;
+  for (int t = (alive ? n : 0) + threadIdx.x; t < p.frames; t += kThreads) labels[t] = -1;
+  for (int i = (alive ? 2 * L : 0) + threadIdx.x; i < 2 * p.most; i += kThreads) spans[i] = -1;
+  if (threadIdx.x == 0) p.score[b] = (float)score;
+  if (alive && n > 0 && wave == 0) trace<SH>(p, at_token > at_blank ? 2 * L - 1 : 2 * L, n, words, tok, labels, spans);
+}
+
+template <class SH>
 __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
   constexpr int W = SH::W, R = SH::R, HL = SH::HL;
-  __shared__ float s_end_m[2];
-  __shared__ int s_end_e[2];
-  __shared__ float s_over_m[2][W][W > 1 ? HL * R : 1];
-  __shared__ int s_over_e[2][W][W > 1 ? HL * R : 1];
+  __shared__ Prob s_end[2];
+  __shared__ Prob s_over[2][W][W > 1 ? HL * R : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
-  const bool active = wave * SH::N <= 2 * L;
+  const bool active = wave < W && wave * SH::N <= 2 * L;
   const int32_t* tok = p.tokens + (int64_t)b * p.most;
   if (n == 0) {
     if (threadIdx.x == 0) p.total[b] = L == 0 ? 0.f : -INFINITY;
     return;
   }
-  if (threadIdx.x < 2) {
-    s_end_m[threadIdx.x] = 0.f;
-    s_end_e[threadIdx.x] = kZero;
-  }
-  Frames<SH, true> fr(p, b, n, lds);
-  SumStep<SH> st;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    st.m[r] = 1.f;
-    st.e[r] = kZero;
-  }
+  if (threadIdx.x < 2) s_end[threadIdx.x] = {0.f, kZero};
+  const Frames fr(p, b, n, lds);
+  Sum<SH> st;
 #pragma unroll
   for (int q = 0; q < R / 2; ++q) {
     const int i = (base >> 1) + q;
-    st.col[q] = fr.column(i, L) * 8;
-    st.closed[q] = i > 0 && i < L && tok[i] == tok[i - 1] ? kShut : 0;
+    st.col[q] = wave < W ? fr.column(i, L) : 0;
+    st.shut[q] = wave < W && i > 0 && i < L && tok[i] == tok[i - 1] ? kShut : 0;
   }
-  const int blank = fr.blank_column() * 8;
-  int edge = wave == 0 ? 0 : kZero;
   over_frames<SH, true>(
-      fr, active,
-      [&](int stage, int f, int t) {
-        st.step(fr.at(stage, f), blank, 1.f, edge);
-        edge = kZero;
-        if ((t & (kRefresh - 1)) == kRefresh - 1) st.renormalize();
+      fr, st, wave, lane, base, active,
+      [&](int g) {
+        if ((g & (kRefresh / SH::F - 1)) == kRefresh / SH::F - 1) st.renormalize();
       },
       [&](bool write, int half) {
         if constexpr (W > 1) {
           if (write) {
             if (lane >= 64 - HL)
 #pragma unroll
-              for (int r = 0; r < R; ++r) {
-                s_over_m[half][wave][(lane - (64 - HL)) * R + r] = st.m[r];
-                s_over_e[half][wave][(lane - (64 - HL)) * R + r] = st.e[r];
-              }
+              for (int r = 0; r < R; ++r) s_over[half][wave][(lane - (64 - HL)) * R + r] = {st.m[r], st.e[r]};
           } else if (wave > 0 && lane < HL) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-              st.m[r] = s_over_m[half][wave - 1][lane * R + r];
-              st.e[r] = s_over_e[half][wave - 1][lane * R + r];
+              const Prob v = s_over[half][wave - 1][lane * R + r];
+              st.m[r] = v.m;
+              st.e[r] = v.e;
             }
           }
         }
       });
-  __syncthreads();
   if (active && (wave == 0 || lane >= HL)) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
       for (int i = 0; i < 2; ++i)
-        if (base + r == 2 * L - i) {
-          s_end_m[i] = st.m[r];
-          s_end_e[i] = st.e[r];
-        }
+        if (base + r == 2 * L - i) s_end[i] = {st.m[r], st.e[r]};
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int hi = max(s_end_e[0], s_end_e[1]);
-    const float sum = ldexpf(s_end_m[0], s_end_e[0] - hi) + ldexpf(s_end_m[1], s_end_e[1] - hi);
-    p.total[b] = hi < kZero / 4 ? -INFINITY : (float)((double)hi * 0.693147180559945309 + (double)logf(sum));
+    const int hi = max(s_end[0].e, s_end[1].e);
+    const float sum = ldexpf(s_end[0].m, s_end[0].e - hi) + ldexpf(s_end[1].m, s_end[1].e - hi);
+    p.total[b] = hi < kNone ? -INFINITY : (float)((double)hi * 0.693147180559945309 + (double)logf(sum));
   }
 }
 
 // workgroup b: the best path of sequence b; batch + b: the sum of all
 template <int W, int R>
-__global__ void __launch_bounds__(64 * W) align_kernel(AlignArgs p) {
+__global__ void __launch_bounds__(64 * (W + kLoaders)) align_kernel(AlignArgs p) {
   extern __shared__ char lds[];
   using SH = Shape<W, R>;
   const bool sum = (int)blockIdx.x >= p.batch;
@@ -509,30 +510,30 @@ template <int W, int R>
 hipError_t launch_as(AlignArgs p, hipStream_t st) {
   p.direct = p.vocab <= p.most + 1;
   p.columns = p.direct ? p.vocab : p.most + 1;
-  // frames per stage: as many as kStage loads per lane hold, a divisor of the refresh interval
+  // frames per stage: a divisor of the refresh interval, two stages beside the rest of the LDS
   p.ahead = kRefresh;
-  while (p.ahead > W && p.ahead / W * ((p.columns + 64) / 64) > kStage) p.ahead /= 2;
-  const size_t lds = (size_t)2 * p.ahead * (p.columns + 1) * (p.total ? 8 : 4);
+  while (p.ahead > 1 && 16 * p.ahead * (p.columns + 1) > 128 * 1024) p.ahead /= 2;
+  const size_t lds = (size_t)16 * p.ahead * (p.columns + 1);
   auto* fn = align_kernel<W, R>;
   if (lds > 32 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(fn, dim3(p.total ? 2 * p.batch : p.batch), dim3(64 * W), lds, st, p);
+  hipLaunchKernelGGL(fn, dim3(p.total ? 2 * p.batch : p.batch), dim3(64 * (W + kLoaders)), lds, st, p);
   return hipGetLastError();
 }
 
-// The fewest states per lane that hold the sequences: a step's time grows with them (see the table in launch_align).
-template <class F>
-auto by_tokens(int most, F&& f) {
+// the fewest states per lane and waves that hold the sequences
+template <class Fn>
+auto by_tokens(int most, Fn&& fn) {
   const int states = 2 * most + 1;
-  if (states <= Shape<1, 2>::kStates) return f(Shape<1, 2>{});
-  if (states <= Shape<4, 2>::kStates) return f(Shape<4, 2>{});
-  if (states <= Shape<4, 4>::kStates) return f(Shape<4, 4>{});
-  if (states <= Shape<4, 8>::kStates) return f(Shape<4, 8>{});
-  return f(Shape<4, 18>{});
+  if (states <= Shape<1, 2>::kStates) return fn(Shape<1, 2>{});
+  if (states <= Shape<4, 2>::kStates) return fn(Shape<4, 2>{});
+  if (states <= Shape<4, 4>::kStates) return fn(Shape<4, 4>{});
+  if (states <= Shape<8, 4>::kStates) return fn(Shape<8, 4>{});
+  return fn(Shape<8, 8>{});
 }
-static_assert(Shape<4, 18>::kStates >= 2 * TONE_ALIGN_MAX_TOKENS + 1, "the longest sequences fit");
+static_assert(Shape<8, 8>::kStates >= 2 * TONE_ALIGN_MAX_TOKENS + 1, "the longest sequences fit");
 
 hipError_t launch_align(const AlignArgs& p, hipStream_t st) {
   return by_tokens(p.most, [&](auto sh) { return launch_as<decltype(sh)::W, decltype(sh)::R>(p, st); });

@@ -24,7 +24,7 @@ from . import _lib
 from . import config as C
 
 MAX_K = 64              # TONE_SCORES_MAX_K
-MAX_TOKENS = 2000       # TONE_ALIGN_MAX_TOKENS
+MAX_TOKENS = 1800       # TONE_ALIGN_MAX_TOKENS
 STATUS = {1: "out of pages", 2: "a stream's table row is full", 4: "bad request", 8: "bad queue cursors"}   # TONE_FRAMES_*
 
 
