@@ -12,10 +12,13 @@
 // of W waves, R consecutive ones per lane: a step moves one 64-bit value from lane to lane (DPP) and needs no LDS and no
 // barrier.  With W > 1 the waves' ranges overlap: a wave's first HL lanes repeat the last ones of the wave below, whose
 // values they lack go wrong by at most two states per frame from the left edge on, and are set right from that wave through
-// LDS every 32 frames.  The frames' log probabilities are staged in LDS some frames ahead, the columns being the vocabulary,
-// or only the sequence's own labels where those are fewer.  Which predecessor was taken is one bit (blank) or two (token)
-// per state, F frames of a lane to a word of the workspace; the path is read back by one wave, a lane's word at a time
-// (v_readlane) with the state in scalar registers, so no load waits for the state it belongs to.
+// LDS every 32 frames.  Waves of their own stage the frames' log probabilities in LDS some frames ahead, the columns being
+// the vocabulary, or only the sequence's own labels where those are fewer.
+//
+// Which predecessor was taken is one bit (blank) or two (token) per state, F frames of a lane to a word of the workspace.
+// Each state also carries where its path was 32 frames ago, so the path is first found at every 32nd frame, one look-up
+// each, and then between them by all waves at once: a wave loads the words of its 32 frames and walks them with the state in
+// scalar registers (v_readlane), so no load waits for the state it belongs to.
 //
 // The sum over paths runs in a workgroup of its own, beside the one that finds the best path.  Each state is a 32-bit mantissa
 // and a 32-bit exponent of 2 (never a logarithm: no exp and log per state and frame, and no underflow, however unlikely a
@@ -38,13 +41,14 @@ struct AlignArgs {
   const int32_t *token_lens, *frame_lens;
   float *score, *total;                 // total: or nullptr
   int32_t *labels, *spans;              // [batch][frames], [batch][most][2]
-  uint32_t* words;                      // [batch][groups][W][64]
+  uint32_t* words;                      // [batch][groups][W][64], groups of F frames
+  uint16_t* came;                       // [batch][legs][states], legs of kRefresh frames: the state at the frame before the leg
   int columns, direct;                  // columns staged per frame: the labels (direct), or 0 = blank, 1 + i = token i
   int ahead;                            // frames per stage
 };
 
 constexpr float kClosed = 6e4f;         // entries of this size and more (masks of lowest values) count as -inf
-constexpr int kRefresh = 32;            // frames between two refreshes of the waves' overlap
+constexpr int kRefresh = 32;            // frames of a leg: between two refreshes of the waves' overlap, and two marks of the path
 constexpr int kLoaders = 4;             // waves that stage the frames
 constexpr int kBatch = 8;               // loads a loader lane has in flight
 // exponents of probability 0: a factor of 0 takes kShut off, what passed one stays below kNone and counts as 0.  They are
@@ -145,6 +149,7 @@ struct Best {
   static constexpr int Q = SH::R / 2;
   double a[SH::R];
   double below;                         // the state below the lane's first; lane 0: -inf
+  int o[SH::R], below_o;                // the paths' states at the frame before the leg
   int col[Q];
   bool apart[Q];                        // token q may follow the token before it directly
   uint32_t word;
@@ -161,20 +166,29 @@ struct Best {
 #pragma unroll
     for (int i = 0; i < SH::R; ++i) a[i] = -INFINITY;
     below = -INFINITY;
+    below_o = 0;
     word = 0;
+    mark(base);
     if (base == 0) {
       a[0] = r.blank;
       a[1] = r.tok[0];
     }
   }
+  __device__ __forceinline__ void mark(int base) {
+#pragma unroll
+    for (int i = 0; i < SH::R; ++i) o[i] = base + i;
+  }
   __device__ __forceinline__ void step(const Row& r) {
     below = shift_in(a[SH::R - 1], below);
+    below_o = shift_in(o[SH::R - 1], below_o);
 #pragma unroll
     for (int q = Q - 1; q >= 0; --q) {
       const double stay = a[2 * q + 1], one = a[2 * q], from = q ? a[q ? 2 * q - 1 : 0] : below;
       // not apart: a NaN, which no compare prefers and v_max_f64 passes over
       const double two = __hiloint2double(apart[q] ? __double2hiint(from) : 0x7ff80000, __double2loint(from));
+      const int o_from = q ? o[q ? 2 * q - 1 : 0] : below_o;
       double m, token, blank;
+      int o_token, o_blank;
       uint64_t c0, c1, c2;
       // one by hand: (a) v_max_f64 without the quieting of operands that fmax brings, (b) each compare's mask pushed into
       // the word by one add with carry, two instructions at least behind the compare as gfx950 demands of masks
@@ -184,14 +198,19 @@ struct Best {
           "v_max_f64 %[blank], %[one], %[from]\n\t"
           "v_cmp_gt_f64_e64 %[c2], %[two], %[m]\n\t"
           "v_max_f64 %[token], %[m], %[two]\n\t"
+          "v_cndmask_b32_e64 %[o_token], %[o_stay], %[o_one], %[c1]\n\t"
+          "v_cndmask_b32_e64 %[o_blank], %[o_one], %[o_from], %[c0]\n\t"
           "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c1]\n\t"
           "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c2]\n\t"
-          "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c0]"
-          : [word] "+v"(word), [m] "=&v"(m), [blank] "=&v"(blank), [token] "=&v"(token), [c0] "=&s"(c0), [c1] "=&s"(c1), [c2] "=&s"(c2)
-          : [stay] "v"(stay), [one] "v"(one), [two] "v"(two), [from] "v"(from)
+          "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c0]\n\t"
+          "v_cndmask_b32_e64 %[o_token], %[o_token], %[o_from], %[c2]"
+          : [o_token] "=&v"(o_token), [o_blank] "=&v"(o_blank), [word] "+v"(word), [m] "=&v"(m), [blank] "=&v"(blank), [token] "=&v"(token), [c0] "=&s"(c0), [c1] "=&s"(c1), [c2] "=&s"(c2)
+          : [o_stay] "v"(o[2 * q + 1]), [o_one] "v"(o[2 * q]), [o_from] "v"(o_from), [stay] "v"(stay), [one] "v"(one), [two] "v"(two), [from] "v"(from)
           : "vcc");
       a[2 * q + 1] = token + r.tok[q];
       a[2 * q] = blank + r.blank;
+      o[2 * q + 1] = o_token;
+      o[2 * q] = o_blank;
     }
   }
 };
@@ -311,83 +330,71 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int wav
   }
 }
 
-// The path from its last state, by one wave.  `at` counts the states as the words hold them: 64 R of wave 0, of wave 1, ...
+// The path over the frames t0 .. t1 of one leg from its state `s` at t1, by one wave.  `at` is the state's place in the words:
+// 64 R states of the wave below, then 64 R of the one that holds s (or that one alone, where it is wave 0).
 template <class SH>
-__device__ __forceinline__ void trace(const AlignArgs& p, int s, int n, const uint32_t* words, const int32_t* tok, int32_t* labels, int32_t* spans) {
-  constexpr int W = SH::W, R = SH::R, F = SH::F, kAhead = W > 4 ? 4 : 8, kLane = R == 2 ? 1 : R == 4 ? 2 : 3;
+__device__ __forceinline__ void trace(const AlignArgs& p, int s, int t0, int t1, int n, const uint32_t* words, const int32_t* tok, int32_t* labels,
+                                      int32_t* spans) {
+  constexpr int W = SH::W, R = SH::R, F = SH::F, G = kRefresh / F, V = W > 1 ? 2 : 1, kLane = R == 2 ? 1 : R == 4 ? 2 : 3;
   constexpr int kOver = SH::HL * R;
   // steps back by the state's bits: even states (blank) bit 0; odd ones bit 2 over bit 1 (token: c1, c2): 2 if c2 else c1
   constexpr uint32_t kSteps = 0xa5a04444u;
   static_assert(R <= 8, "kLane");
   const int lane = threadIdx.x & 63;
-  int at;
-  {
-    int w = 0, rest = s;
-    while (rest >= 64 * R) {
-      rest -= SH::N;
-      ++w;
-    }
-    at = w * 64 * R + rest;
+  int w = 0, at = s;
+  while (at >= 64 * R) {
+    at -= SH::N;
+    ++w;
   }
-  int path = 0, above = -1;
-  uint32_t cur[kAhead][W], nxt[kAhead][W];
-  auto fetch = [&](uint32_t (&to)[kAhead][W], int g0) {     // groups g0, g0 - 1, ...
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-      for (int w = 0; w < W; ++w) to[i][w] = g0 - i >= 0 ? words[((int64_t)(g0 - i) * W + w) * 64 + lane] : 0;
-  };
-  int g = (n - 1) / F;
-  fetch(cur, g);
-  while (g >= 0) {
-    fetch(nxt, g - kAhead);
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i) {
-      if (g - i < 0) continue;
-      const int first = (g - i) * F, last = min(n - 1, first + F - 1);
-      int drop = 0;                      // bits of the frames behind t in the word
-      for (int t = last; t >= first; --t, drop += SH::kBits) {
-        uint32_t word = __builtin_amdgcn_readlane(cur[i][0], (at >> kLane) & 63);
-#pragma unroll
-        for (int w = 1; w < W; ++w)
-          if (at >= w * 64 * R) word = __builtin_amdgcn_readlane(cur[i][w], (at >> kLane) & 63);
-        path = lane == (t & 63) ? s : path;
-        const uint32_t bits = (word >> (drop + 3 * ((at >> 1) & (R / 2 - 1)))) & 7;
-        const int how = (kSteps >> (2 * bits + 16 * (at & 1))) & 3;
-        const int now = s;
-        s -= how;
-        at -= how;
-        if (W > 1 && at >= 64 * R && (at & (64 * R - 1)) < kOver) at -= kOver;    // the wave below has it
-        if ((t & 63) == 0) {             // frames t .. t + 63 are known, and the state before them
-          const int mine = t + lane, prev = shift_in(path, t ? s : -1);
-          int next = __shfl_down(path, 1);
-          if (lane == 63) next = above;
-          if (mine == n - 1) next = -1;
-          if (mine < n) {
-            labels[mine] = path & 1 ? tok[path >> 1] : p.blank;
-            if ((path & 1) && prev != path) spans[path & ~1] = mine;
-            if ((path & 1) && next != path) spans[path | 1] = mine + 1;
-          }
-          above = now;
-        }
-      }
-    }
-    g -= kAhead;
-#pragma unroll
-    for (int i = 0; i < kAhead; ++i)
-#pragma unroll
-      for (int w = 0; w < W; ++w) cur[i][w] = nxt[i][w];
+  if (w > 0) {
+    at += 64 * R;
+    --w;
   }
+  const int g0 = t0 / F, last = t1 / F;
+  uint32_t words_of[G][V];
+#pragma unroll
+  for (int i = 0; i < G; ++i)
+#pragma unroll
+    for (int v = 0; v < V; ++v)
+      words_of[i][v] = g0 + i <= last ? words[((int64_t)(g0 + i) * W + min(w + v, W - 1)) * 64 + lane] : 0;
+  int path = 0;
+#pragma unroll
+  for (int i = G - 1; i >= 0; --i) {
+    const int first = (g0 + i) * F;
+    int drop = 0;                        // bits of the frames behind t in the word
+    for (int t = min(t1, first + F - 1); t >= first; --t, drop += SH::kBits) {
+      uint32_t word = __builtin_amdgcn_readlane(words_of[i][0], (at >> kLane) & 63);
+      if (V > 1 && at >= 64 * R) word = __builtin_amdgcn_readlane(words_of[i][V - 1], (at >> kLane) & 63);
+      path = lane == t - t0 ? s : path;
+      const uint32_t bits = (word >> (drop + 3 * ((at >> 1) & (R / 2 - 1)))) & 7;
+      const int how = (kSteps >> (2 * bits + 16 * (at & 1))) & 3;
+      s -= how;
+      at -= how;
+      if (W > 1 && at >= 64 * R && at < 64 * R + kOver) at -= kOver;      // the wave below has it
+    }
+  }
+  // s: the state at the frame before t0.  A token begins where the state before is another one, and ends there as well
+  const int t = t0 + lane, prev = shift_in(path, t0 ? s : -1);
+  if (t > t1) return;
+  labels[t] = path & 1 ? tok[path >> 1] : p.blank;
+  if (prev != path) {
+    if (path & 1) spans[path & ~1] = t;
+    if (prev >= 0 && (prev & 1)) spans[prev | 1] = t;
+  }
+  if (t == n - 1 && (path & 1)) spans[path | 1] = n;
 }
 
 template <class SH>
 __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
   constexpr int W = SH::W, R = SH::R, HL = SH::HL, kThreads = 64 * (W + kLoaders);
+  constexpr int kLegs = 256;             // legs traced between two barriers
   __shared__ double s_end[2];
+  __shared__ int s_state[kLegs];
   __shared__ double s_over[2][W][W > 1 ? HL * R : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
   const bool active = wave < W && wave * SH::N <= 2 * L;
   uint32_t* words = p.words + (int64_t)b * ((p.frames + SH::F - 1) / SH::F) * W * 64;
+  uint16_t* came = p.came + (int64_t)b * ((p.frames + kRefresh - 1) / kRefresh) * SH::kStates;
   int32_t* labels = p.labels + (int64_t)b * p.frames;
   int32_t* spans = p.spans + (int64_t)b * p.most * 2;
   const int32_t* tok = p.tokens + (int64_t)b * p.most;
@@ -407,6 +414,15 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
         [&](int g) {
           out[(int64_t)g * (W * 64)] = st.word;
           st.word = 0;
+          constexpr int G = kRefresh / SH::F;
+          if ((g & (G - 1)) == G - 1 || g == (n - 1) / SH::F) {            // the end of a leg, or of the sequence
+            if (wave == 0 || lane >= HL) {
+              uint32_t* to = reinterpret_cast<uint32_t*>(came + (int64_t)(g / G) * SH::kStates + base);
+#pragma unroll
+              for (int q = 0; q < R / 2; ++q) to[q] = st.o[2 * q] | st.o[2 * q + 1] << 16;
+            }
+            st.mark(base);
+          }
         },
         [&](bool write, int half) {
           if constexpr (W > 1) {
@@ -435,7 +451,21 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
   for (int t = (alive ? n : 0) + threadIdx.x; t < p.frames; t += kThreads) labels[t] = -1;
   for (int i = (alive ? 2 * L : 0) + threadIdx.x; i < 2 * p.most; i += kThreads) spans[i] = -1;
   if (threadIdx.x == 0) p.score[b] = (float)score;
-  if (alive && n > 0 && wave == 0) trace<SH>(p, at_token > at_blank ? 2 * L - 1 : 2 * L, n, words, tok, labels, spans);
+  if (!alive || n == 0) return;
+  int s = at_token > at_blank ? 2 * L - 1 : 2 * L;
+  for (int leg = (n - 1) / kRefresh; leg >= 0; leg -= kLegs) {              // s: the state at the end of `leg`
+    const int low = max(0, leg - kLegs + 1);
+    if (wave == 0) {
+      for (int k = leg; k >= low; --k) {
+        if (lane == 0) s_state[leg - k] = s;
+        if (k > 0) s = __builtin_amdgcn_readfirstlane(came[(int64_t)k * SH::kStates + s]);
+      }
+    }
+    __syncthreads();
+    for (int k = leg - wave; k >= low; k -= W + kLoaders)
+      trace<SH>(p, __builtin_amdgcn_readfirstlane(s_state[leg - k]), k * kRefresh, min(n, (k + 1) * kRefresh) - 1, n, words, tok, labels, spans);
+    __syncthreads();
+  }
 }
 
 template <class SH>
@@ -539,10 +569,14 @@ hipError_t launch_align(const AlignArgs& p, hipStream_t st) {
   return by_tokens(p.most, [&](auto sh) { return launch_as<decltype(sh)::W, decltype(sh)::R>(p, st); });
 }
 
-int64_t align_workspace(int batch, int frames, int most) {
-  return by_tokens(most, [&](auto sh) -> int64_t {
+// bytes of the words, and of the states at the legs' beginnings behind them
+struct Workspace {
+  int64_t words, came;
+};
+Workspace align_workspace(int batch, int frames, int most) {
+  return by_tokens(most, [&](auto sh) -> Workspace {
     using SH = decltype(sh);
-    return (int64_t)batch * ((frames + SH::F - 1) / SH::F) * SH::W * 64 * 4;
+    return {(int64_t)batch * ((frames + SH::F - 1) / SH::F) * SH::W * 64 * 4, (int64_t)batch * ((frames + kRefresh - 1) / kRefresh) * SH::kStates * 2};
   });
 }
 
@@ -555,7 +589,8 @@ extern "C" {
 
 int64_t tone_ctc_align_workspace(int batch, int frames, int tokens) {
   if (batch < 0 || frames < 0 || tokens < 0 || tokens > TONE_ALIGN_MAX_TOKENS) return -1;
-  return align_workspace(batch, frames, tokens);
+  const Workspace w = align_workspace(batch, frames, tokens);
+  return w.words + w.came;
 }
 
 int tone_ctc_align(int device, const void* x, int type, int64_t stride, int64_t batch_stride, int64_t x_rows,
@@ -575,7 +610,8 @@ int tone_ctc_align(int device, const void* x, int type, int64_t stride, int64_t 
   const int64_t need = tone_ctc_align_workspace(batch, frames, max_tokens);
   if (workspace_bytes < need || (need && !workspace)) return refuse(what, "workspace smaller than tone_ctc_align_workspace");
   AlignArgs p{x, type, stride, batch_stride, x_rows, rows, batch, frames, vocab, blank, tokens, max_tokens, token_lens, frame_lens,
-              score, total, labels, spans, static_cast<uint32_t*>(workspace), 0, 0, 0};
+              score, total, labels, spans, static_cast<uint32_t*>(workspace),
+              reinterpret_cast<uint16_t*>(static_cast<char*>(workspace) + align_workspace(batch, frames, max_tokens).words), 0, 0, 0};
   return launch_on(device, what, [&] { return launch_align(p, static_cast<hipStream_t>(stream)); });
 }
 
