@@ -105,43 +105,69 @@ struct Frames {
     return 8 * (t < 0 || t >= p.vocab || t == p.blank ? p.columns : p.direct ? t : i + 1);
   }
   __device__ __forceinline__ int blank_column() const { return p.direct ? 8 * p.blank : 0; }
-  __device__ __forceinline__ float value(int64_t off) const {
-    if (p.type == TONE_TYPE_FP32) return load_elem(static_cast<const float*>(p.x) + off);
-    if (p.type == TONE_TYPE_FP16) return load_elem(static_cast<const __half*>(p.x) + off);
-    return load_elem(static_cast<const Bf16*>(p.x) + off);
-  }
-  // frames t0 ... of the sequence: items of one frame and 64 columns, dealt to the loader waves
-  template <bool SUM>
-  __device__ __forceinline__ void fill(int stage, int t0, int loader, int lane) const {
-    const int blocks = p.columns / 64 + 1, frames = min(p.ahead, n - t0), items = frames * blocks;
-    for (int i0 = loader; i0 < items; i0 += kLoaders * kBatch) {
-      int64_t row[kBatch];
-      float v[kBatch];
+};
+
+// A loader wave: frames loader, loader + kLoaders, ... of each stage, 64 columns at a time.  What is in flight is the data of
+// the stage after the next and the rows of the one after that, so a stage waits for neither; only frames of many columns
+// have more than kBatch loads, and those behind are loaded as they are written.
+template <bool SUM>
+__device__ __forceinline__ void load_frames(const Frames& fr, int loader, int lane) {
+  const AlignArgs& p = fr.p;
+  const int n = fr.n, ahead = p.ahead, per = max(1, ahead / kLoaders), shift = 31 - __builtin_clz(per), items = (p.columns / 64 + 1) * per;
+  const bool wide = p.type == TONE_TYPE_FP32;
+  const char* x = static_cast<const char*>(p.x) + (p.rows ? 0 : (int64_t)fr.b * p.batch_stride * (wide ? 4 : 2));
+  const int64_t* rows = p.rows ? p.rows + (int64_t)fr.b * p.frames : nullptr;
+  int64_t row = -1, row_next = -1;               // lane f: row of frame f of a stage
+  uint32_t raw[kBatch];
+  bool have[kBatch];
+  auto frame = [&](int i) { return loader + kLoaders * (i & (per - 1)); };
+  auto load = [&](int i, uint32_t& to) -> bool {
+    const int f = frame(i), c = (i >> shift) * 64 + lane;
+    const int64_t r = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), f) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, f);
+    int label = c;
+    if (!p.direct) label = c && c < p.columns ? fr.tok[c - 1] : p.blank;
+    const bool ok = c < p.columns && label >= 0 && label < p.vocab && r >= 0 && (!rows || r < p.x_rows);
+    const int64_t off = ok ? r * p.stride + label : 0;
+    if (ok) to = wide ? *reinterpret_cast<const uint32_t*>(x + 4 * off) : *reinterpret_cast<const uint16_t*>(x + 2 * off);
+    return ok;
+  };
+  auto write = [&](int stage, int i, uint32_t bits, bool ok) {
+    const int c = (i >> shift) * 64 + lane;
+    if (c > p.columns) return;
+    float v = __uint_as_float(p.type == TONE_TYPE_BF16 ? bits << 16 : bits);
+    if (p.type == TONE_TYPE_FP16) v = __half2float(__ushort_as_half((uint16_t)bits));
+    if (!ok || !(fabsf(v) < kClosed)) v = -INFINITY;
+    if constexpr (SUM) reinterpret_cast<Prob*>(fr.at(stage, frame(i)))[c] = prob_of(v);
+    else reinterpret_cast<double*>(fr.at(stage, frame(i)))[c] = v;
+  };
+  for (int t0 = -3 * ahead, stage = -3; t0 < n; t0 += ahead, ++stage) {
+    if (t0 + ahead >= 0 && t0 + ahead < n) {
+      const int m = n - (t0 + ahead);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (j < items && frame(j) < min(m, ahead)) write(stage + 1, j, raw[j], have[j]);
+      for (int i = kBatch; i < items; ++i)       // `row` is still that stage's
+        if (frame(i) < min(m, ahead)) {
+          uint32_t bits = 0;
+          const bool ok = load(i, bits);
+          write(stage + 1, i, bits, ok);
+        }
+    }
+    row = row_next;
+    if (t0 + 2 * ahead >= 0) {
+      const int m = n - (t0 + 2 * ahead);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        const int f = min(frames - 1, (i0 + j * kLoaders) / blocks);
-        row[j] = p.rows ? p.rows[(int64_t)b * p.frames + t0 + f] : t0 + f;
-      }
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int i = i0 + j * kLoaders, f = i / blocks, c = (i - f * blocks) * 64 + lane;
-        const bool here = i < items && c < p.columns && (!p.rows || (row[j] >= 0 && row[j] < p.x_rows));
-        int label = c;
-        if (!p.direct) label = here && c ? tok[c - 1] : p.blank;
-        v[j] = -INFINITY;
-        if (here && label >= 0 && label < p.vocab) v[j] = value((p.rows ? 0 : (int64_t)b * p.batch_stride) + row[j] * p.stride + label);
-      }
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j) {
-        const int i = i0 + j * kLoaders, f = i / blocks, c = (i - f * blocks) * 64 + lane;
-        if (i >= items || c > p.columns) continue;
-        const float w = fabsf(v[j]) < kClosed ? v[j] : -INFINITY;
-        if constexpr (SUM) reinterpret_cast<Prob*>(at(stage, f))[c] = prob_of(w);
-        else reinterpret_cast<double*>(at(stage, f))[c] = w;
+        have[j] = false;
+        if (j < items && frame(j) < min(m, ahead)) have[j] = load(j, raw[j]);
       }
     }
+    row_next = -1;
+    const int t = t0 + 3 * ahead + lane;
+    if (lane < ahead && t < n) row_next = rows ? rows[t] : t;
+    if (t0 + ahead >= 0 && t0 + ahead < n) __syncthreads();      // as the stepping waves: before stage 0, and between stages
   }
-};
+}
 
 // The lane's states, and one frame: the highest first, since each needs the ones below it as they were.
 template <class SH>
@@ -162,13 +188,15 @@ struct Best {
 #pragma unroll
     for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const double*>(frame + col[q]);
   }
-  __device__ __forceinline__ void begin(const Row& r, int base) {
+  __device__ __forceinline__ void clear(int base) {
 #pragma unroll
     for (int i = 0; i < SH::R; ++i) a[i] = -INFINITY;
     below = -INFINITY;
     below_o = 0;
     word = 0;
     mark(base);
+  }
+  __device__ __forceinline__ void first(const Row& r, int base) {      // the first frame
     if (base == 0) {
       a[0] = r.blank;
       a[1] = r.tok[0];
@@ -231,7 +259,7 @@ struct Sum {
 #pragma unroll
     for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const Prob*>(frame + col[q]);
   }
-  __device__ __forceinline__ void begin(const Row& r, int base) {
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < SH::R; ++i) {
       m[i] = 1.f;
@@ -239,6 +267,8 @@ struct Sum {
     }
     below_m = 1.f;
     below_e = kZero;
+  }
+  __device__ __forceinline__ void first(const Row& r, int base) {      // the first frame
     if (base == 0) {
       m[0] = r.blank.m;
       e[0] = r.blank.e;
@@ -275,36 +305,32 @@ struct Sum {
 };
 
 // Takes `st` through the frames of a sequence (n > 0).  word(g) after the last frame of every group g of F frames and after
-// the last one, refresh(write, half) every kRefresh frames.  The loader waves fill the next stage meanwhile.
+// the last one, refresh(write, half) every kRefresh frames.  The loader waves fill the next stage meanwhile.  A wave steps
+// only where a path can be: before frame s / 2 none has reached its first state s, and from the frame on from which its last
+// state cannot reach the end any more its values are of no use (nor are those that would be drawn from them).
 template <class SH, bool SUM, class State, class Word, class Refresh>
-__device__ __forceinline__ void over_frames(const Frames& fr, State& st, int wave, int lane, int base, bool active, Word&& word, Refresh&& refresh) {
+__device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, int wave, int lane, Word&& word, Refresh&& refresh) {
   constexpr int F = SH::F;
   const int n = fr.n, ahead = fr.p.ahead, blank = fr.blank_column(), pitch = (fr.p.columns + 1) * 8;
-  if (wave >= SH::W) fr.fill<SUM>(0, 0, wave - SH::W, lane);
+  if (wave >= SH::W) {
+    load_frames<SUM>(fr, wave - SH::W, lane);
+    return;
+  }
+  const int low = wave * SH::N, high = low + 64 * SH::R - 1;
   __syncthreads();
   for (int t0 = 0, stage = 0; t0 < n; t0 += ahead, ++stage) {
     const bool more = t0 + ahead < n;
     const int half = ((t0 + ahead) / kRefresh) & 1;
     const bool now = more && ((t0 + ahead) & (kRefresh - 1)) == 0;
-    if (wave >= SH::W) {
-      if (more) fr.fill<SUM>(stage + 1, t0 + ahead, wave - SH::W, lane);
-    } else if (active) {
-      const int m = min(ahead, n - t0);
+    const int m = min(ahead, n - t0);
+    if (low <= 2 * L && low <= 2 * (t0 + m) - 1 && (int64_t)high + 2 * (int64_t)(n - 1 - t0) >= 2 * L - 1) {
       const char* frame = fr.at(stage, 0);
       typename State::Row r, next;
       st.read(r, frame, blank);
-      int f = 0;
-      if (t0 == 0) {
-        st.begin(r, base);
-        f = 1;
-        frame += pitch;
-        if (m > 1) st.read(r, frame, blank);
-        if (F == 1 || n == 1) word(0);
-      }
-      while (f < m) {
+      for (int f = 0; f < m;) {
         // up to the end of the word, the next frame's entries under way
-        const int end = min(m, (f & ~(F - 1)) + F);
-        if (end - f == F) {
+        const int end = min(m, f + F);
+        if (t0 + f > 0 && end - f == F) {
 #pragma unroll
           for (int i = 0; i < F; ++i) {
             frame += pitch;
@@ -317,16 +343,17 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int wav
           for (; f < end; ++f) {
             frame += pitch;
             if (f + 1 < m) st.read(next, frame, blank);
-            st.step(r);
+            if (t0 + f == 0) st.first(r, low + lane * SH::R);
+            else st.step(r);
             r = next;
           }
         }
-        if ((f & (F - 1)) == 0 || t0 + f == n) word((t0 + f - 1) / F);
+        word((t0 + f - 1) / F);
       }
-      if (now) refresh(true, half);
     }
+    if (now) refresh(true, half);
     if (more) __syncthreads();
-    if (now && active && wave < SH::W) refresh(false, half);
+    if (now) refresh(false, half);
   }
 }
 
@@ -392,7 +419,6 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
   __shared__ int s_state[kLegs];
   __shared__ double s_over[2][W][W > 1 ? HL * R : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
-  const bool active = wave < W && wave * SH::N <= 2 * L;
   uint32_t* words = p.words + (int64_t)b * ((p.frames + SH::F - 1) / SH::F) * W * 64;
   uint16_t* came = p.came + (int64_t)b * ((p.frames + kRefresh - 1) / kRefresh) * SH::kStates;
   int32_t* labels = p.labels + (int64_t)b * p.frames;
@@ -409,8 +435,9 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
       st.apart[q] = !(wave < W && i > 0 && i < L && tok[i] == tok[i - 1]);
     }
     uint32_t* out = words + wave * 64 + lane;
+    st.clear(base);
     over_frames<SH, false>(
-        fr, st, wave, lane, base, active,
+        fr, st, L, wave, lane,
         [&](int g) {
           out[(int64_t)g * (W * 64)] = st.word;
           st.word = 0;
@@ -436,7 +463,7 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
             }
           }
         });
-    if (active && (wave == 0 || lane >= HL)) {
+    if (wave < W && (wave == 0 || lane >= HL)) {
 #pragma unroll
       for (int r = 0; r < R; ++r) {
         if (base + r == 2 * L) s_end[0] = st.a[r];
@@ -474,7 +501,6 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
   __shared__ Prob s_end[2];
   __shared__ Prob s_over[2][W][W > 1 ? HL * R : 1];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
-  const bool active = wave < W && wave * SH::N <= 2 * L;
   const int32_t* tok = p.tokens + (int64_t)b * p.most;
   if (n == 0) {
     if (threadIdx.x == 0) p.total[b] = L == 0 ? 0.f : -INFINITY;
@@ -489,8 +515,9 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
     st.col[q] = wave < W ? fr.column(i, L) : 0;
     st.shut[q] = wave < W && i > 0 && i < L && tok[i] == tok[i - 1] ? kShut : 0;
   }
+  st.clear();
   over_frames<SH, true>(
-      fr, st, wave, lane, base, active,
+      fr, st, L, wave, lane,
       [&](int g) {
         if ((g & (kRefresh / SH::F - 1)) == kRefresh / SH::F - 1) st.renormalize();
       },
@@ -510,7 +537,7 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
           }
         }
       });
-  if (active && (wave == 0 || lane >= HL)) {
+  if (wave < W && (wave == 0 || lane >= HL)) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
       for (int i = 0; i < 2; ++i)
