@@ -88,7 +88,9 @@ __device__ __forceinline__ Prob prob_of(float v) {
   return {__builtin_amdgcn_exp2f(f), (int)n};
 }
 
-// What is staged: [2][ahead][columns + 1] entries of 8 bytes, a double (best path) or a Prob (sum); the last column is closed.
+// What is staged: [2][columns + 1][ahead + 2] entries of 8 bytes, a double (best path) or a Prob (sum); the last column is
+// closed.  A column's frames lie together, so a lane reads two of them at once and the frame is an offset in the instruction;
+// the two entries of padding spread the columns over the banks.
 struct Frames {
   const AlignArgs p;
   const int b, n;
@@ -98,13 +100,14 @@ struct Frames {
   __device__ Frames(const AlignArgs& p_, int b_, int n_, char* buf_)
       : p(p_), b(b_), n(n_), tok(p_.tokens + (int64_t)b_ * p_.most), buf(buf_) {}
 
-  __device__ __forceinline__ char* at(int stage, int f) const { return buf + ((stage & 1) * p.ahead + f) * ((p.columns + 1) * 8); }
+  __device__ __forceinline__ int pitch() const { return (p.ahead + 2) * 8; }
+  __device__ __forceinline__ char* stage(int i) const { return buf + (i & 1) * (p.columns + 1) * pitch(); }
   __device__ __forceinline__ int column(int i, int len) const {        // byte offset of token i of the sequence
     if (i >= len) return 0;                                            // a state behind the last: anything
     const int t = tok[i];
-    return 8 * (t < 0 || t >= p.vocab || t == p.blank ? p.columns : p.direct ? t : i + 1);
+    return pitch() * (t < 0 || t >= p.vocab || t == p.blank ? p.columns : p.direct ? t : i + 1);
   }
-  __device__ __forceinline__ int blank_column() const { return p.direct ? 8 * p.blank : 0; }
+  __device__ __forceinline__ int blank_column() const { return p.direct ? pitch() * p.blank : 0; }
 };
 
 // A loader wave: frames loader, loader + kLoaders, ... of each stage, 64 columns at a time.  What is in flight is the data of
@@ -137,8 +140,9 @@ __device__ __forceinline__ void load_frames(const Frames& fr, int loader, int la
     float v = __uint_as_float(p.type == TONE_TYPE_BF16 ? bits << 16 : bits);
     if (p.type == TONE_TYPE_FP16) v = __half2float(__ushort_as_half((uint16_t)bits));
     if (!ok || !(fabsf(v) < kClosed)) v = -INFINITY;
-    if constexpr (SUM) reinterpret_cast<Prob*>(fr.at(stage, frame(i)))[c] = prob_of(v);
-    else reinterpret_cast<double*>(fr.at(stage, frame(i)))[c] = v;
+    char* to = fr.stage(stage) + c * fr.pitch() + 8 * frame(i);
+    if constexpr (SUM) *reinterpret_cast<Prob*>(to) = prob_of(v);
+    else *reinterpret_cast<double*>(to) = v;
   };
   for (int t0 = -3 * ahead, stage = -3; t0 < n; t0 += ahead, ++stage) {
     if (t0 + ahead >= 0 && t0 + ahead < n) {
@@ -180,13 +184,20 @@ struct Best {
   bool apart[Q];                        // token q may follow the token before it directly
   uint32_t word;
 
+  struct Rows {                         // of two frames
+    double2 blank, tok[Q];
+  };
   struct Row {
     double blank, tok[Q];
-  };
-  __device__ __forceinline__ void read(Row& r, const char* frame, int blank) const {
-    r.blank = *reinterpret_cast<const double*>(frame + blank);
+    __device__ __forceinline__ Row(const Rows& r, int i) : blank(i ? r.blank.y : r.blank.x) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const double*>(frame + col[q]);
+      for (int q = 0; q < Q; ++q) tok[q] = i ? r.tok[q].y : r.tok[q].x;
+    }
+  };
+  __device__ __forceinline__ void read(Rows& r, const char* frame, int blank) const {
+    r.blank = *reinterpret_cast<const double2*>(frame + blank);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const double2*>(frame + col[q]);
   }
   __device__ __forceinline__ void clear(int base) {
 #pragma unroll
@@ -251,13 +262,23 @@ struct Sum {
   int col[Q];
   int shut[Q];                          // 0, or kShut where token q must not follow the token before it directly
 
+  struct alignas(16) Two {
+    Prob x, y;
+  };
+  struct Rows {
+    Two blank, tok[Q];
+  };
   struct Row {
     Prob blank, tok[Q];
-  };
-  __device__ __forceinline__ void read(Row& r, const char* frame, int blank) const {
-    r.blank = *reinterpret_cast<const Prob*>(frame + blank);
+    __device__ __forceinline__ Row(const Rows& r, int i) : blank(i ? r.blank.y : r.blank.x) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const Prob*>(frame + col[q]);
+      for (int q = 0; q < Q; ++q) tok[q] = i ? r.tok[q].y : r.tok[q].x;
+    }
+  };
+  __device__ __forceinline__ void read(Rows& r, const char* frame, int blank) const {
+    r.blank = *reinterpret_cast<const Two*>(frame + blank);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) r.tok[q] = *reinterpret_cast<const Two*>(frame + col[q]);
   }
   __device__ __forceinline__ void clear() {
 #pragma unroll
@@ -311,7 +332,7 @@ struct Sum {
 template <class SH, bool SUM, class State, class Word, class Refresh>
 __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, int wave, int lane, Word&& word, Refresh&& refresh) {
   constexpr int F = SH::F;
-  const int n = fr.n, ahead = fr.p.ahead, blank = fr.blank_column(), pitch = (fr.p.columns + 1) * 8;
+  const int n = fr.n, ahead = fr.p.ahead, blank = fr.blank_column();
   if (wave >= SH::W) {
     load_frames<SUM>(fr, wave - SH::W, lane);
     return;
@@ -324,31 +345,32 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, 
     const bool now = more && ((t0 + ahead) & (kRefresh - 1)) == 0;
     const int m = min(ahead, n - t0);
     if (low <= 2 * L && low <= 2 * (t0 + m) - 1 && (int64_t)high + 2 * (int64_t)(n - 1 - t0) >= 2 * L - 1) {
-      const char* frame = fr.at(stage, 0);
-      typename State::Row r, next;
+      const char* frame = fr.stage(stage);
+      typename State::Rows r, next;
       st.read(r, frame, blank);
-      for (int f = 0; f < m;) {
-        // up to the end of the word, the next frame's entries under way
-        const int end = min(m, f + F);
-        if (t0 + f > 0 && end - f == F) {
+      for (int f = 0; f < m; f += F) {
+        // the next two frames' entries under way (they are in the stage, also where the sequence has ended)
+        if (t0 + f > 0 && f + F <= m) {
 #pragma unroll
-          for (int i = 0; i < F; ++i) {
-            frame += pitch;
-            if (i + 1 < F || end < m) st.read(next, frame, blank);
-            st.step(r);
+          for (int i = 0; i < F; i += 2) {
+            frame += 16;
+            if (i + 2 < F || f + F < m) st.read(next, frame, blank);
+            st.step({r, 0});
+            st.step({r, 1});
             r = next;
           }
-          f = end;
         } else {
-          for (; f < end; ++f) {
-            frame += pitch;
-            if (f + 1 < m) st.read(next, frame, blank);
-            if (t0 + f == 0) st.first(r, low + lane * SH::R);
-            else st.step(r);
+#pragma unroll 1
+          for (int i = 0; i < F; i += 2) {
+            frame += 16;
+            if (f + i + 2 < m) st.read(next, frame, blank);
+            if (t0 + f + i == 0) st.first({r, 0}, low + lane * SH::R);
+            else if (f + i < m) st.step({r, 0});
+            if (f + i + 1 < m) st.step({r, 1});
             r = next;
           }
         }
-        word((t0 + f - 1) / F);
+        word((t0 + f) / F);
       }
     }
     if (now) refresh(true, half);
@@ -554,7 +576,7 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
 // workgroup b: the best path of sequence b; batch + b: the sum of all
 template <int W, int R>
 __global__ void __launch_bounds__(64 * (W + kLoaders)) align_kernel(AlignArgs p) {
-  extern __shared__ char lds[];
+  extern __shared__ __attribute__((aligned(16))) char lds[];
   using SH = Shape<W, R>;
   const bool sum = (int)blockIdx.x >= p.batch;
   const int b = sum ? blockIdx.x - p.batch : blockIdx.x;
@@ -569,8 +591,9 @@ hipError_t launch_as(AlignArgs p, hipStream_t st) {
   p.columns = p.direct ? p.vocab : p.most + 1;
   // frames per stage: a divisor of the refresh interval, two stages beside the rest of the LDS
   p.ahead = kRefresh;
-  while (p.ahead > 1 && 16 * p.ahead * (p.columns + 1) > 128 * 1024) p.ahead /= 2;
-  const size_t lds = (size_t)16 * p.ahead * (p.columns + 1);
+  while (p.ahead > 2 && 16 * (p.ahead + 2) * (p.columns + 1) > 128 * 1024) p.ahead /= 2;
+  static_assert(16 * (2 + 2) * (TONE_ALIGN_MAX_TOKENS + 2) <= 128 * 1024, "two frames of the longest sequences fit");
+  const size_t lds = (size_t)16 * (p.ahead + 2) * (p.columns + 1);
   auto* fn = align_kernel<W, R>;
   if (lds > 32 * 1024) {
     const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
