@@ -176,7 +176,7 @@ int tone_session_debug_read(tone_session *s, const char *buffer, void *host_dst,
 /* status bits of tone_frames_plan (device memory): 0, or the whole call changed nothing */
 #define TONE_FRAMES_NO_PAGES 1     /* more pages to take than were free before the call           */
 #define TONE_FRAMES_ROW_FULL 2     /* a stream would hold more than `width` pages                 */
-#define TONE_FRAMES_BAD_REQUEST 4  /* negative or decreasing counts, add > max_add, row ids       */
+#define TONE_FRAMES_BAD_REQUEST 4  /* negative or decreasing counts, a frame past 2^31 - 2, add > max_add, row ids */
 #define TONE_FRAMES_BAD_QUEUE 8    /* the cursors describe no queue of n_pages pages              */
 
 /* Move `batch` streams from the frames [first, length) they hold to [max(first, keep), length + add), 0 <= keep <=

@@ -15,12 +15,27 @@
 namespace tone {
 namespace {
 
+// n / d for 0 <= n < 2^31 by one multiplication: m = ceil(2^(31 + l) / d), 2^l >= d (m < 2^32; exact over that range)
+struct Divisor {
+  uint32_t d, m;
+  int s;
+  explicit Divisor(uint32_t d_) : d(d_), s(0) {
+    while ((1ull << s) < d) ++s;
+    m = (uint32_t)(((1ull << (31 + s)) + d - 1) / d);
+    s += 31 - 32;
+  }
+  __device__ __forceinline__ uint32_t operator()(uint32_t n) const {
+    return d == 1 ? n : __umulhi(n, m) >> s;
+  }
+};
+
 struct PlanArgs {
   int32_t* table;                       // [n_rows][width], rows `stride` entries apart
   int64_t stride;
   int n_rows, width;
   int32_t* queue;                       // [n_pages]
   int n_pages, page;
+  Divisor by_page;
   const int64_t* cursors_in;            // head, tail of the queue
   int64_t* cursors_out;
   const int32_t *rows_in, *rows_out, *first, *length, *keep, *add;   // [batch]
@@ -34,6 +49,7 @@ struct SlotArgs {
   const int32_t* table;
   int64_t stride;
   int n_rows, width, n_pages, page;
+  Divisor by_page;
   const int32_t *rows, *first, *begin, *count;   // [batch]
   int batch;
   int64_t* slots;                       // [batch][max_count]
@@ -52,25 +68,26 @@ struct PutArgs {
   int64_t pool_stride, pool_rows;
 };
 
-constexpr int kPlanThreads = 256;
-constexpr int kPlanRows = 32;          // requests a workgroup writes, at most
+constexpr int kPlanWaves = 16;          // of a workgroup, shared by its requests
 
 struct Request {
-  int64_t kept, end;                   // the frames held after the call
-  int64_t lo0, hi0, lo1, hi1;          // pages held before / after
-  int64_t from;                        // first page taken
+  int first, length, kept, end;         // frames held before: [first, length), after: [kept, end)
+  int lo0, hi0, lo1, hi1;               // pages held before / after
+  int from;                             // first page taken
   int take, drop;
   bool bad, wide;
 };
 
 __device__ __forceinline__ Request read_request(const PlanArgs& p, int b) {
   Request r;
-  const int64_t first = p.first[b], length = p.length[b], keep = p.keep[b], add = p.add[b], P = p.page;
-  const int ri = p.rows_in[b], ro = p.rows_out[b];
-  r.kept = first > keep ? first : keep;
-  r.end = length + add;
-  r.bad = first < 0 || first > length || add < 0 || add > p.max_add || keep < 0 || keep > r.end || ri < 0 || ri >= p.n_rows ||
-          ro < 0 || ro >= p.n_rows || ri == ro;
+  const int first = p.first[b], length = p.length[b], keep = p.keep[b], add = p.add[b], ri = p.rows_in[b], ro = p.rows_out[b];
+  const int64_t end = (int64_t)length + add;
+  r.first = first;
+  r.length = length;
+  r.kept = max(first, keep);
+  r.end = (int)end;
+  r.bad = first < 0 || first > length || add < 0 || add > p.max_add || keep < 0 || end > INT32_MAX || keep > end || ri < 0 ||
+          ri >= p.n_rows || ro < 0 || ro >= p.n_rows || ri == ro;
   if (r.bad) {
     r.lo0 = r.hi0 = r.lo1 = r.hi1 = r.from = 0;
     r.take = r.drop = 0;
@@ -78,48 +95,46 @@ __device__ __forceinline__ Request read_request(const PlanArgs& p, int b) {
     return r;
   }
   const bool had = first < length, has = r.kept < r.end;
-  // frame numbers are 31 bits, the end 32: unsigned 32-bit divisions
-  const uint32_t u = (uint32_t)P;
-  r.lo0 = (uint32_t)first / u;
-  r.hi0 = had ? ((uint32_t)length - 1u) / u + 1 : r.lo0;
-  r.lo1 = (uint32_t)r.kept / u;
-  r.hi1 = has ? ((uint32_t)r.end - 1u) / u + 1 : r.lo1;
-  r.from = had && r.hi0 > r.lo1 ? r.hi0 : r.lo1;
-  r.take = has ? (int)(r.hi1 - r.from) : 0;
-  r.drop = had ? (int)((has && r.lo1 < r.hi0 ? r.lo1 : r.hi0) - r.lo0) : 0;
+  r.lo0 = p.by_page(first);
+  r.hi0 = had ? p.by_page(length - 1) + 1 : r.lo0;
+  r.lo1 = p.by_page(r.kept);
+  r.hi1 = has ? p.by_page(r.end - 1) + 1 : r.lo1;
+  r.from = had ? max(r.hi0, r.lo1) : r.lo1;
+  r.take = has ? r.hi1 - r.from : 0;
+  r.drop = had ? (has ? min(r.lo1, r.hi0) : r.hi0) - r.lo0 : 0;
   r.wide = r.hi1 - r.lo1 > p.width || r.hi0 - r.lo0 > p.width;
   return r;
 }
 
-// One launch: every workgroup adds up the pages of all requests (16 bytes each, out of L2) to place its own ones, instead of
-// a scan kernel in front of a writing kernel.  blockIdx.x: up to kPlanRows requests; blockIdx.y: a share of their slots.
-__global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs p, int rows_per) {
-  __shared__ int64_t part[kPlanThreads / 64][4];
-  __shared__ int s_take[kPlanRows], s_drop[kPlanRows];
+// One launch: every workgroup adds up the pages of all requests (24 bytes each, out of L2) to place its own ones, instead of a
+// scan kernel in front of a writing kernel.  blockIdx.x: kPlanWaves / per requests of `per` waves each, so that a request's
+// chain of dependent loads (its row, its pages, its slots) is walked by all of them at once; blockIdx.y: a share of the slots.
+__global__ void __launch_bounds__(64 * kPlanWaves) plan_kernel(PlanArgs p, int per) {
+  __shared__ int64_t part[kPlanWaves][4];
+  __shared__ int s_take[kPlanWaves], s_drop[kPlanWaves];
   __shared__ int s_flags;
-  const int tid = threadIdx.x, r0 = blockIdx.x * rows_per, r1 = min(p.batch, r0 + rows_per);
+  const int tid = threadIdx.x, wave = tid >> 6, rows = kPlanWaves / per, r0 = blockIdx.x * rows, r1 = min(p.batch, r0 + rows);
   if (tid == 0) s_flags = 0;
   __syncthreads();
-  int64_t take = 0, take0 = 0, drop = 0, drop0 = 0;      // of all requests / of those before r0
+  int64_t v[4] = {0, 0, 0, 0};          // taken by all / by those before r0; released likewise
   int flags = 0;
-  for (int b = tid; b < p.batch; b += kPlanThreads) {
+  for (int b = tid; b < p.batch; b += 64 * kPlanWaves) {
     const Request r = read_request(p, b);
     flags |= (r.wide ? TONE_FRAMES_ROW_FULL : 0) | (r.bad ? TONE_FRAMES_BAD_REQUEST : 0);
-    take += r.take;
-    drop += r.drop;
+    v[0] += r.take;
+    v[2] += r.drop;
     if (b < r0) {
-      take0 += r.take;
-      drop0 += r.drop;
+      v[1] += r.take;
+      v[3] += r.drop;
     } else if (b < r1) {
       s_take[b - r0] = r.take;
       s_drop[b - r0] = r.drop;
     }
   }
-  int64_t v[4] = {take, take0, drop, drop0};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     for (int o = 32; o; o >>= 1) v[i] += __shfl_xor(v[i], o);
-    if ((tid & 63) == 0) part[tid >> 6][i] = v[i];
+    if ((tid & 63) == 0) part[wave][i] = v[i];
   }
   if (flags) atomicOr(&s_flags, flags);
   __syncthreads();
@@ -127,7 +142,7 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs p, int rows
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] = 0;
-    for (int w = 0; w < kPlanThreads / 64; ++w) v[i] += part[w][i];
+    for (int w = 0; w < kPlanWaves; ++w) v[i] += part[w][i];
   }
   const int64_t head = p.cursors_in[0], tail = p.cursors_in[1];
   // free + released <= n_pages holds for every state these calls produce; anything else is not a queue of this pool
@@ -138,51 +153,51 @@ __global__ void __launch_bounds__(kPlanThreads) plan_kernel(PlanArgs p, int rows
     p.cursors_out[1] = tail + (flags ? 0 : v[2]);
     p.status[0] = flags;
   }
-  const int64_t h0 = flags ? 0 : head % p.n_pages, q0 = flags ? 0 : tail % p.n_pages;
-  int64_t at_take = h0 + v[1], at_drop = q0 + v[3];
-  const int seg = (p.max_add + gridDim.y - 1) / gridDim.y, s0 = blockIdx.y * seg, s1 = min(p.max_add, s0 + seg);
-  for (int b = r0; b < r1; ++b) {
-    const Request r = read_request(p, b);
-    int64_t* slots = p.slots + (int64_t)b * p.max_add;
-    if (flags) {
-      for (int j = s0 + tid; j < s1; j += kPlanThreads) slots[j] = -1;
-      const int ri = p.rows_in[b], ro = p.rows_out[b];
-      if (blockIdx.y == 0 && ri >= 0 && ri < p.n_rows && ro >= 0 && ro < p.n_rows)
-        for (int j = tid; j < p.width; j += kPlanThreads) p.table[ro * p.stride + j] = p.table[ri * p.stride + j];
-      continue;
+  const int mine = wave / per, b = r0 + mine, at = (wave - mine * per) * 64 + (tid & 63), step = 64 * per;
+  if (b >= r1) return;
+  const int seg = (p.max_add + gridDim.y - 1) / gridDim.y, s0 = min(p.max_add, (int)blockIdx.y * seg), s1 = min(p.max_add, s0 + seg);
+  int64_t* slots = p.slots + (int64_t)b * p.max_add;
+  const int ri = p.rows_in[b], ro = p.rows_out[b];
+  if (flags) {
+    for (int j = s0 + at; j < s1; j += step) slots[j] = -1;
+    if (blockIdx.y == 0 && ri >= 0 && ri < p.n_rows && ro >= 0 && ro < p.n_rows && ri != ro)
+      for (int j = at; j < p.width; j += step) p.table[ro * p.stride + j] = p.table[ri * p.stride + j];
+    return;
+  }
+  const Request r = read_request(p, b);
+  // positions in the queue, modulo n_pages once: both are below 2 n_pages, as taken <= free and free + released <= n_pages
+  int64_t take = head % p.n_pages + v[1], drop = tail % p.n_pages + v[3];
+  for (int i = 0; i < mine; ++i) {
+    take += s_take[i];
+    drop += s_drop[i];
+  }
+  const int32_t* before = p.table + ri * p.stride;
+  // page of logical page lp: kept from the old row, or the next entry of the queue
+  auto page_of = [&](int lp) -> int32_t {
+    if (lp < r.hi0 && r.hi0 > r.lo0) return before[lp - r.lo0];
+    int64_t i = take + (lp - r.from);
+    if (i >= p.n_pages) i -= p.n_pages;
+    return p.queue[i];
+  };
+  if (blockIdx.y == 0) {
+    int32_t* after = p.table + ro * p.stride;
+    for (int j = at; j < p.width; j += step) after[j] = r.lo1 + j < r.hi1 ? page_of(r.lo1 + j) : -1;
+    for (int j = at; j < r.drop; j += step) {
+      int64_t i = drop + j;
+      if (i >= p.n_pages) i -= p.n_pages;
+      p.queue[i] = before[j];
     }
-    const int32_t* before = p.table + p.rows_in[b] * p.stride;
-    // page of logical page lp: kept from the old row, or the next entry of the queue
-    auto page_of = [&](int64_t lp) -> int32_t {
-      if (lp < r.hi0 && r.hi0 > r.lo0) return before[lp - r.lo0];
-      int64_t i = at_take + (lp - r.from);
-      if (i >= p.n_pages) i -= p.n_pages;      // at_take < 2 n_pages: taken <= free <= n_pages
-      return p.queue[i];
-    };
-    if (blockIdx.y == 0) {
-      int32_t* after = p.table + p.rows_out[b] * p.stride;
-      for (int j = tid; j < p.width; j += kPlanThreads) after[j] = r.lo1 + j < r.hi1 ? page_of(r.lo1 + j) : -1;
-      for (int j = tid; j < r.drop; j += kPlanThreads) {
-        int64_t i = at_drop + j;
-        if (i >= p.n_pages) i -= p.n_pages;
-        p.queue[i] = before[j];
-      }
+  }
+  const int new_end = min(s1, r.end - r.length);
+  for (int j = s0 + at; j < s1; j += step) {
+    int64_t slot = -1;
+    const int f = r.length + j;
+    if (j < new_end && f >= r.kept) {
+      const int q = p.by_page(f);
+      const int32_t pg = page_of(q);
+      if (pg >= 0 && pg < p.n_pages) slot = (int64_t)pg * p.page + (f - q * p.page);
     }
-    const int64_t length = p.length[b];
-    const int add = p.add[b];
-    const uint32_t base = (uint32_t)(r.lo1 * p.page), u = (uint32_t)p.page;
-    for (int j = s0 + tid; j < s1; j += kPlanThreads) {
-      const int64_t f = length + j;
-      int64_t slot = -1;
-      if (j < add && f >= r.kept) {
-        const uint32_t off = (uint32_t)f - base, q = off / u;
-        const int32_t pg = page_of(r.lo1 + q);
-        if (pg >= 0 && pg < p.n_pages) slot = (int64_t)pg * u + (off - q * u);
-      }
-      slots[j] = slot;
-    }
-    at_take += s_take[b - r0];
-    at_drop += s_drop[b - r0];
+    slots[j] = slot;
   }
 }
 
@@ -193,55 +208,79 @@ __global__ void __launch_bounds__(256) slots_kernel(SlotArgs p, int segs) {
   const int row = p.rows[b], first = p.first[b], count = p.count[b];
   const int64_t f = (int64_t)p.begin[b] + j;
   int64_t slot = -1;
-  if (row >= 0 && row < p.n_rows && first >= 0 && j < count && f >= first && f <= 0x7fffffff) {
-    const uint32_t u = (uint32_t)p.page, q = (uint32_t)f / u, at = q - (uint32_t)first / u;
-    if (at < (uint32_t)p.width) {
+  if (row >= 0 && row < p.n_rows && first >= 0 && j < count && f >= first && f <= INT32_MAX) {
+    const int q = p.by_page((uint32_t)f), at = q - (int)p.by_page(first);
+    if (at < p.width) {
       const int32_t pg = p.table[row * p.stride + at];
-      if (pg >= 0 && pg < p.n_pages) slot = (int64_t)pg * u + ((uint32_t)f - q * u);
+      if (pg >= 0 && pg < p.n_pages) slot = (int64_t)pg * p.page + ((int)f - q * p.page);
     }
   }
   p.slots[(int64_t)b * p.max_count + j] = slot;
 }
 
-// rows [16 x blockIdx.x, + 16) of src, one element per thread and step
+constexpr int kPutEach = 8;                          // entries a thread has in flight
+constexpr int kPutChunk = 256 * kPutEach;
+
+// Entries kPutChunk * blockIdx.x ... of the rows laid end to end: consecutive lanes copy consecutive entries of a row, all of
+// a thread's loads are issued before its first store, and the rows' slots come from LDS.
 template <typename S, typename D>
 __global__ void __launch_bounds__(256) put_kernel(const S* __restrict__ src, int64_t src_stride, const int64_t* __restrict__ slots,
-                                                  int64_t n, int vocab, D* __restrict__ pool, int64_t pool_stride, int64_t pool_rows) {
-  const int64_t r0 = (int64_t)blockIdx.x * 16;
-  const int rows = (int)min((int64_t)16, n - r0);
-  for (int e = threadIdx.x; e < rows * vocab; e += 256) {
-    const int r = e / vocab, c = e - r * vocab;
-    const int64_t s = slots[r0 + r];
-    if (s >= 0 && s < pool_rows) store_elem(pool + s * pool_stride + c, load_elem(src + (r0 + r) * src_stride + c));
+                                                  int64_t n, Divisor by_vocab, D* __restrict__ pool, int64_t pool_stride, int64_t pool_rows) {
+  __shared__ int64_t s_slot[kPutChunk + 1];
+  const int vocab = by_vocab.d;
+  const int64_t e0 = (int64_t)blockIdx.x * kPutChunk, row0 = e0 / vocab;
+  const int c0 = (int)(e0 - row0 * vocab), entries = (int)min((int64_t)kPutChunk, n * vocab - e0);
+  const int rows = by_vocab(c0 + entries - 1) + 1;   // at most kPutChunk + 1 (vocab 1: kPutChunk)
+  for (int r = threadIdx.x; r < rows; r += 256) s_slot[r] = slots[row0 + r];
+  float v[kPutEach];
+#pragma unroll
+  for (int i = 0; i < kPutEach; ++i) {
+    const int e = i * 256 + threadIdx.x;
+    if (e < entries) {
+      const int r = by_vocab(c0 + e);
+      v[i] = load_elem(src + (row0 + r) * src_stride + (c0 + e - r * vocab));
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < kPutEach; ++i) {
+    const int e = i * 256 + threadIdx.x;
+    if (e < entries) {
+      const int r = by_vocab(c0 + e);
+      const int64_t s = s_slot[r];
+      if (s >= 0 && s < pool_rows) store_elem(pool + s * pool_stride + (c0 + e - r * vocab), v[i]);
+    }
   }
 }
 
 template <typename S>
 hipError_t put_from(const PutArgs& a, hipStream_t st) {
-  const dim3 grid((unsigned)((a.n + 15) / 16));
+  const dim3 grid((unsigned)((a.n * a.vocab + kPutChunk - 1) / kPutChunk));
   const S* src = static_cast<const S*>(a.src);
+  const Divisor by(a.vocab);
   switch (a.pool_type) {
     case TONE_TYPE_FP32:
-      hipLaunchKernelGGL((put_kernel<S, float>), grid, dim3(256), 0, st, src, a.src_stride, a.slots, a.n, a.vocab,
-                         static_cast<float*>(a.pool), a.pool_stride, a.pool_rows);
+      hipLaunchKernelGGL((put_kernel<S, float>), grid, dim3(256), 0, st, src, a.src_stride, a.slots, a.n, by, static_cast<float*>(a.pool),
+                         a.pool_stride, a.pool_rows);
       break;
     case TONE_TYPE_FP16:
-      hipLaunchKernelGGL((put_kernel<S, __half>), grid, dim3(256), 0, st, src, a.src_stride, a.slots, a.n, a.vocab,
-                         static_cast<__half*>(a.pool), a.pool_stride, a.pool_rows);
+      hipLaunchKernelGGL((put_kernel<S, __half>), grid, dim3(256), 0, st, src, a.src_stride, a.slots, a.n, by, static_cast<__half*>(a.pool),
+                         a.pool_stride, a.pool_rows);
       break;
     default:
-      hipLaunchKernelGGL((put_kernel<S, Bf16>), grid, dim3(256), 0, st, src, a.src_stride, a.slots, a.n, a.vocab,
-                         static_cast<Bf16*>(a.pool), a.pool_stride, a.pool_rows);
+      hipLaunchKernelGGL((put_kernel<S, Bf16>), grid, dim3(256), 0, st, src, a.src_stride, a.slots, a.n, by, static_cast<Bf16*>(a.pool),
+                         a.pool_stride, a.pool_rows);
   }
   return hipGetLastError();
 }
 
 hipError_t launch_plan(const PlanArgs& p, hipStream_t st) {
-  // about one workgroup per CU over the requests; long slot rows are shared by several
-  const int rows_per = std::min(kPlanRows, std::max(1, (p.batch + 255) / 256));
-  const int gx = std::max(1, (p.batch + rows_per - 1) / rows_per);   // an empty batch still writes the cursors and the status
-  const int gy = std::max(1, std::min({64, 1024 / std::max(1, gx), (p.max_add + 1023) / 1024}));
-  hipLaunchKernelGGL(plan_kernel, dim3(gx, gy), dim3(kPlanThreads), 0, st, p, rows_per);
+  // a wave per request while that gives every CU a workgroup, more for fewer requests; long slot rows are cut in pieces
+  int per = 1;
+  while (per < kPlanWaves && (int64_t)p.batch * per < 16 * 256) per *= 2;
+  const int rows = kPlanWaves / per, gx = std::max(1, (p.batch + rows - 1) / rows);   // an empty batch still writes the cursors and the status
+  const int gy = std::max(1, std::min(1024 / gx, (p.max_add + 64 * per * 4 - 1) / (64 * per * 4)));
+  hipLaunchKernelGGL(plan_kernel, dim3(gx, gy), dim3(64 * kPlanWaves), 0, st, p, per);
   return hipGetLastError();
 }
 
@@ -279,7 +318,7 @@ int tone_frames_plan(int device, int32_t* table, int64_t table_stride, int n_row
   if (n_rows <= 0 || width <= 0 || n_pages <= 0 || page_size <= 0 || table_stride < width)
     return refuse(what, "rows, width, pages and page size must be positive, table_stride >= width");
   if ((int64_t)width * page_size > INT32_MAX) return refuse(what, "width x page_size exceeds 2^31 - 1 frames");
-  PlanArgs p{table, table_stride, n_rows, width, queue, n_pages, page_size, cursors_in, cursors_out, rows_in, rows_out,
+  PlanArgs p{table, table_stride, n_rows, width, queue, n_pages, page_size, Divisor(page_size), cursors_in, cursors_out, rows_in, rows_out,
              first, length, keep, add, batch, slots, max_add, status};
   return launch_on(device, what, [&] { return launch_plan(p, static_cast<hipStream_t>(stream)); });
 }
@@ -294,7 +333,7 @@ int tone_frames_slots(int device, const int32_t* table, int64_t table_stride, in
   if (n_rows <= 0 || width <= 0 || n_pages <= 0 || page_size <= 0 || table_stride < width)
     return refuse(what, "rows, width, pages and page size must be positive, table_stride >= width");
   if (((int64_t)max_count + 255) / 256 * batch > INT32_MAX) return refuse(what, "batch x max_count too large for one launch");
-  SlotArgs p{table, table_stride, n_rows, width, n_pages, page_size, rows, first, begin, count, batch, slots, max_count};
+  SlotArgs p{table, table_stride, n_rows, width, n_pages, page_size, Divisor(page_size), rows, first, begin, count, batch, slots, max_count};
   return launch_on(device, what, [&] { return launch_slots(p, static_cast<hipStream_t>(stream)); });
 }
 
@@ -307,7 +346,7 @@ int tone_frames_put(int device, const void* src, int src_type, int64_t src_strid
   if (!src || !slots || (!pool && pool_rows)) return refuse(what, "null pointer");
   if (src_stride < vocab || pool_stride < vocab) return refuse(what, "row stride < vocab");
   if (!aligned(src, src_type) || !aligned(pool, pool_type)) return refuse(what, "src or pool not aligned to its element type");
-  if ((n + 15) / 16 > INT32_MAX) return refuse(what, "too many rows for one launch");
+  if (n > ((int64_t)INT32_MAX << 8) / vocab) return refuse(what, "too many rows for one launch");
   PutArgs p{src, src_type, src_stride, slots, n, vocab, pool, pool_type, pool_stride, pool_rows};
   return launch_on(device, what, [&] { return launch_put(p, static_cast<hipStream_t>(stream)); });
 }
