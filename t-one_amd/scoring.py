@@ -16,9 +16,7 @@ current stream of the tensors' device.  Contents are checked on the device: an i
 
 from __future__ import annotations
 
-from typing import NamedTuple, Optional, Sequence
-
-import numpy as np
+from typing import NamedTuple, Optional
 
 from . import _lib
 from . import config as C
@@ -28,12 +26,16 @@ MAX_TOKENS = 1800       # TONE_ALIGN_MAX_TOKENS
 STATUS = {1: "out of pages", 2: "a stream's table row is full", 4: "bad request", 8: "bad queue cursors"}   # TONE_FRAMES_*
 
 
-def _torch():
-    import torch
-    return torch
-
-
 _types: dict = {}
+_mod = None
+
+
+def _torch():
+    global _mod
+    if _mod is None:
+        import torch
+        _mod = torch
+    return _mod
 
 
 def _type(t, name: str) -> int:
@@ -66,20 +68,22 @@ class _On:
     """The stream of one call.  Outputs come from the allocator under that stream; where it is not the current one, the
     inputs are marked as in use on it, so that they may be freed at once after the call."""
 
+    __slots__ = ("raw", "_ctx")
+
     def __init__(self, dev, stream, *inputs):
         torch = _torch()
-        cur = torch.cuda.current_stream(dev)
         self._ctx = None
-        if stream is None or stream == cur:
-            self.raw = cur.cuda_stream
+        if stream is None:
+            self.raw = torch._C._cuda_getCurrentRawStream(dev.index)   # current_stream(dev).cuda_stream without the objects
             return
         if stream.device != dev:
             raise ValueError(f"stream on {stream.device}, tensors on {dev}")
         self.raw = stream.cuda_stream
-        self._ctx = torch.cuda.stream(stream)
-        for t in inputs:
-            if t is not None:
-                t.record_stream(stream)
+        if stream != torch.cuda.current_stream(dev):
+            self._ctx = torch.cuda.stream(stream)
+            for t in inputs:
+                if t is not None:
+                    t.record_stream(stream)
 
     def __enter__(self):
         if self._ctx is not None:
@@ -171,18 +175,25 @@ def frames_slots(table, rows, first, begin, count, *, page_size: int, n_pages: i
     return slots
 
 
-def _rows_of(t, name: str):
-    """(tensor, row stride) of a (..., V) tensor whose leading dimensions are one run of equally spaced rows."""
+def _rows_of(t, name: str) -> int:
+    """Distance of the rows of a (..., V) tensor, whose leading dimensions must be one run of equally spaced rows."""
     if t.dim() < 2 or t.shape[-1] < 1:
         raise ValueError(f"{name} must be (..., vocab), got {tuple(t.shape)}")
+    if t.is_contiguous():
+        return t.shape[-1]
     if t.shape[-1] > 1 and t.stride(-1) != 1:
         raise ValueError(f"{name} must have unit stride along the vocabulary")
-    if t.dim() > 2:
-        step = t.stride(-2)
-        for d in range(t.dim() - 3, -1, -1):
-            if t.shape[d] > 1 and t.stride(d) != step * int(np.prod(t.shape[d + 1 : -1])):
-                raise ValueError(f"{name}'s leading dimensions must be one run of equally spaced rows")
-    return t.stride(-2) if t.shape[-2] > 1 or t.dim() > 2 else max(t.stride(-2), t.shape[-1])
+    step = run = None
+    for d in range(t.dim() - 2, -1, -1):
+        if t.shape[d] == 1:
+            continue
+        if step is None:
+            step, run = t.stride(d), t.stride(d) * t.shape[d]
+        elif t.stride(d) != run:
+            raise ValueError(f"{name}'s leading dimensions must be one run of equally spaced rows")
+        else:
+            run *= t.shape[d]
+    return t.shape[-1] if step is None else step
 
 
 def frames_put(src, slots, pool, stream=None) -> None:
@@ -234,11 +245,11 @@ def token_scores(x, tokens=None, k: int = 0, rows=None, stream=None) -> TokenSco
         if rows.dtype != torch.int64 or not rows.is_contiguous():
             raise ValueError(f"rows must be a contiguous int64 tensor, got {rows.dtype}")
     stride = _rows_of(x, "x")
-    shape = tuple(rows.shape) if rows is not None else tuple(x.shape[:-1])
+    shape = rows.shape if rows is not None else x.shape[:-1]
     x_rows = x.numel() // vocab
-    n = int(np.prod(shape, dtype=np.int64))
-    if tokens is not None and (tokens.dtype != torch.int32 or tuple(tokens.shape) != shape or not tokens.is_contiguous()):
-        raise ValueError(f"tokens must be a contiguous {shape} int32 tensor, got {tuple(tokens.shape)} {tokens.dtype}")
+    n = rows.numel() if rows is not None else x_rows
+    if tokens is not None and (tokens.dtype != torch.int32 or tokens.shape != shape or not tokens.is_contiguous()):
+        raise ValueError(f"tokens must be a contiguous {tuple(shape)} int32 tensor, got {tuple(tokens.shape)} {tokens.dtype}")
     k = int(k)
     if not 0 <= k <= min(vocab, MAX_K):
         raise ValueError(f"k must be in 0 .. min(vocab, {MAX_K}), got {k}")

@@ -114,6 +114,16 @@ def test_frames_put_refuses(change):
         S.frames_put(**a)
 
 
+def test_rows_of_any_leading_shape():
+    x = torch.zeros((6, 10, 8))
+    assert S._rows_of(x, "x") == 8 and S._rows_of(x[:, :, :5], "x") == 8 and S._rows_of(x[:, :1], "x") == 80
+    assert S._rows_of(x[::2, :1, :3], "x") == 160 and S._rows_of(x[:1, ::2], "x") == 16 and S._rows_of(x[:1, :1, :3], "x") == 3
+    assert S._rows_of(torch.zeros((1, 8)).expand(4, 8), "x") == 0 and S._rows_of(torch.zeros((0, 8)), "x") == 8
+    for bad in (x[:, :7], x.transpose(0, 1), x[:, :, ::2]):
+        with pytest.raises(ValueError):
+            S._rows_of(bad, "x")
+
+
 @pytest.mark.parametrize("change", [
     {"x": torch.zeros((2, 5), dtype=torch.int32)}, {"x": torch.zeros(5)}, {"x": torch.zeros((2, 0))}, {"x": torch.zeros((5, 2)).t()},
     {"tokens": torch.zeros(2, dtype=torch.int64)}, {"tokens": torch.zeros(3, dtype=torch.int32)}, {"k": 6}, {"k": -1},
