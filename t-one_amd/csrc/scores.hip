@@ -186,6 +186,17 @@ struct Best {
   uint64_t floor;                        // the k-th best; keys at or below it do not matter
 
   __device__ __forceinline__ void clear() { key = floor = 0; }
+  __device__ __forceinline__ bool any() const { return read_lane(key, 0) != 0; }
+  // another list, in ascending order
+  __device__ __forceinline__ void join(uint64_t other, int lane) {
+    key = key > other ? key : other;
+    step<32>(lane);
+    step<16>(lane);
+    step<8>(lane);
+    step<4>(lane);
+    step<2>(lane);
+    step<1>(lane);
+  }
   // the wave's keys, one per lane, as the first list: a bitonic sort
   __device__ __forceinline__ void sort(uint64_t mine, int lane, int k) {
     key = mine;
@@ -245,44 +256,57 @@ struct Vec {
   __device__ Vec() {}
 };
 
-// One wave's part of a row, entries in ascending order.  The maximum is the wave's, so every e^(x - m) is at most 1 and all
-// terms of the entropy's sum have one sign; a step that brings no new maximum and nothing above the k-th best entry (one
-// compare of the lane's largest against the floor) adds up its terms and nothing else.
+// One wave's part of a row, in batches of Q steps of N entries per lane, in ascending order.  The maximum is the wave's, so
+// every e^(x - m) is at most 1 and all terms of the entropy's sum have one sign; a batch that brings no new maximum and
+// nothing above the k-th best entry (one compare of the lanes' largest against the floor) adds up its terms and nothing else.
 struct Part {
   float m = -3.402823466e38f, s = 0.f, u = 0.f;
-  int above = 0;
+  int above = 0;                         // uniform
   float floor = -INFINITY;               // value of the k-th best, or the maximum for k = 0
   bool full = false;                     // k entries seen
   Best best;
 
-  template <int N>
-  __device__ __forceinline__ void step(const float (&x)[N], int i0, int valid, int lane, int k, float xt, int t, int base, int span) {
-    float top = x[0];
+  // x[q][j]: entry base + q * span + lane * N + j; those of lanes from valid[q] on are none (-inf)
+  template <int Q, int N>
+  __device__ __forceinline__ void batch(const float (&x)[Q][N], int base, const int (&valid)[Q], int lane, int k, float xt, int t) {
+    float top[Q], most;
 #pragma unroll
-    for (int j = 1; j < N; ++j) top = fmaxf(top, x[j]);
-    if (!full || __ballot(top > floor)) news<N>(x, i0, valid, lane, k, top);
+    for (int q = 0; q < Q; ++q) {
+      top[q] = x[q][0];
 #pragma unroll
-    for (int j = 0; j < N; ++j) {
-      const float z = x[j] - m, e = exp_neg(z);
-      s += e;
-      u = fmaf(e, fmaxf(z, -200.f), u);
+      for (int j = 1; j < N; ++j) top[q] = fmaxf(top[q], x[q][j]);
+      most = q ? fmaxf(most, top[q]) : top[q];
     }
-    // entries above x_t; equal ones count below index t.  base .. base + span: the wave's entries of this step
-    if (t >= base + span) {
+    if (!full || __ballot(most > floor)) news<Q, N>(x, top, most, base, valid, lane, k);
 #pragma unroll
-      for (int j = 0; j < N; ++j) above += j < valid && x[j] >= xt;
-    } else if (t < base) {
+    for (int q = 0; q < Q; ++q)
 #pragma unroll
-      for (int j = 0; j < N; ++j) above += x[j] > xt;
-    } else {
+      for (int j = 0; j < N; ++j) {
+        const float z = x[q][j] - m, e = exp_neg(z);
+        s += e;
+        u = fmaf(e, fmaxf(z, -200.f), u);   // as in the short form
+      }
+    // entries above x_t; equal ones count below index t
 #pragma unroll
-      for (int j = 0; j < N; ++j) above += j < valid && (x[j] > xt || (x[j] == xt && i0 + j < t));
+    for (int q = 0; q < Q; ++q) {
+      const int b = base + q * 64 * N;
+      if (t >= b + 64 * N) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) above += __builtin_popcountll(__ballot(x[q][j] >= xt && lane < valid[q]));
+      } else if (t < b) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) above += __builtin_popcountll(__ballot(x[q][j] > xt));
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          above += __builtin_popcountll(__ballot(lane < valid[q] && (x[q][j] > xt || (x[q][j] == xt && b + lane * N + j < t))));
+      }
     }
   }
 
-  template <int N>
-  __device__ __forceinline__ void news(const float (&x)[N], int i0, int valid, int lane, int k, float top) {
-    float w = top;
+  template <int Q, int N>
+  __device__ __forceinline__ void news(const float (&x)[Q][N], const float (&top)[Q], float most, int base, const int (&valid)[Q], int lane, int k) {
+    float w = most;
     w = fmaxf(w, xor_lane<1>(w));
     w = fmaxf(w, xor_lane<2>(w));
     w = fmaxf(w, xor_lane<7>(w));
@@ -300,25 +324,31 @@ struct Part {
       full = true;
       return;
     }
-    uint64_t key[N];
-#pragma unroll
-    for (int j = 0; j < N; ++j) key[j] = j < valid ? key_of(x[j], i0 + j) : 0;
-    if (best.floor == 0 && read_lane(best.key, 0) == 0) {
+    int best_at = -1;
+    if (!best.any()) {
       // nothing held yet: the lanes' largest first, which sets a floor close to the final one
-      uint64_t mine = key[0];
-      int at = 0;
+      uint64_t mine = 0;
 #pragma unroll
-      for (int j = 1; j < N; ++j)
-        if (key[j] > mine) {
-          mine = key[j];
-          at = j;
+      for (int q = 0; q < Q; ++q)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const uint64_t key = lane < valid[q] ? key_of(x[q][j], base + (q * 64 + lane) * N + j) : 0;
+          if (key > mine) {
+            mine = key;
+            best_at = q * N + j;
+          }
         }
       best.sort(mine, lane, k);
-#pragma unroll
-      for (int j = 0; j < N; ++j) key[j] = j == at ? 0 : key[j];
     }
 #pragma unroll
-    for (int j = 0; j < N; ++j) best.take(key[j], lane, k);
+    for (int q = 0; q < Q; ++q) {
+      const float low = best.floor ? key_value(best.floor) : -INFINITY;
+      if (best.floor && __ballot(top[q] >= low) == 0) continue;      // (a NaN is above no floor, but fills a list)
+#pragma unroll
+      for (int j = 0; j < N; ++j)
+        if (!best.floor || __ballot(x[q][j] >= low))
+          best.take(lane < valid[q] && q * N + j != best_at ? key_of(x[q][j], base + (q * 64 + lane) * N + j) : 0, lane, k);
+    }
     full = best.floor != 0;
     if (full) floor = key_value(best.floor);
   }
@@ -328,66 +358,65 @@ struct Part {
 // front of it and behind the last whole vector are single loads of the first and the last wave), joined in LDS.
 template <typename T, int W, int ROWS>
 __global__ void __launch_bounds__(64 * W * ROWS) scores_long_kernel(ScoreArgs p) {
-  constexpr int N = Vec<T>::N, kAhead = 4;
+  constexpr int N = Vec<T>::N, Q = 4;
   __shared__ float part_f[W * ROWS][3];
   __shared__ int part_i[W * ROWS];
-  __shared__ uint64_t part_k[W * ROWS][W > 1 ? TONE_SCORES_MAX_K : 1];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wr = W > 1 ? wave % W : 0;
-  const int64_t n = (int64_t)blockIdx.x * ROWS + wave / W;
+  __shared__ uint64_t part_k[W > 1 ? W / 2 : 1][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wr = W > 1 ? wave : 0;
+  const int64_t n = (int64_t)blockIdx.x * ROWS + (W > 1 ? 0 : wave);
   const bool in = n < p.n;
   const int64_t row = !in ? -1 : p.rows ? p.rows[n] : n;
   const bool here = row >= 0 && row < p.x_rows;
-  if (in && !here && wr == 0) write_none(p, n, lane, 64);
-  if constexpr (W == 1) {
-    if (!here) return;
+  if (!here) {                           // the whole workgroup, or (W = 1) the wave alone
+    if (in && wr == 0) write_none(p, n, lane, 64);
+    return;
   }
   Part a;
   a.best.clear();
-  int t = -1;
-  float xt = 0.f;
-  if (here) {
-    const T* x = static_cast<const T*>(p.x) + row * p.stride;
-    t = p.tokens ? p.tokens[n] : -1;
-    if (t < 0 || t >= p.vocab) t = -1;
-    if (t >= 0) xt = load_elem(x + t);
-    const int head = min(p.vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
-    const int vecs = (p.vocab - head) / N, each = (vecs + W - 1) / W;
-    const int v0 = min(vecs, wr * each), v1 = min(vecs, v0 + each);
-    const uint4* base = reinterpret_cast<const uint4*>(x + head);
-    for (int c = v0; c < v1; c += 64 * kAhead) {
-      Vec<T> v[kAhead];
+  const T* x = static_cast<const T*>(p.x) + row * p.stride;
+  int t = p.tokens ? p.tokens[n] : -1;
+  if (t < 0 || t >= p.vocab) t = -1;
+  const float xt = t >= 0 ? load_elem(x + t) : 0.f;
+  const int head = min(p.vocab, (int)((16 - ((uintptr_t)x & 15)) & 15) / (int)sizeof(T));
+  const int vecs = (p.vocab - head) / N, each = (vecs + W - 1) / W;
+  const int v0 = min(vecs, wr * each), v1 = min(vecs, v0 + each);
+  const uint4* base = reinterpret_cast<const uint4*>(x + head);
+  Vec<T> v[Q];
+  auto load = [&](int c) {
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q) {
-        const int i = c + 64 * q + lane;
-        if (i < v1) v[q].raw = base[i];
-      }
+    for (int q = 0; q < Q; ++q) {
+      const int i = c + 64 * q + lane;
+      if (i < v1) v[q].raw = base[i];
+    }
+  };
+  load(v0);
+  for (int c = v0; c < v1; c += 64 * Q) {
+    float f[Q][N];
+    int valid[Q];
 #pragma unroll
-      for (int q = 0; q < kAhead; ++q) {
-        const int b = c + 64 * q;
-        if (b >= v1) break;
-        const bool ok = b + lane < v1;
-        float f[N];
+    for (int q = 0; q < Q; ++q) {
+      valid[q] = v1 - (c + 64 * q);
 #pragma unroll
-        for (int j = 0; j < N; ++j) f[j] = ok ? load_elem(&v[q].e[j]) : -INFINITY;
-        a.step<N>(f, head + (b + lane) * N, ok ? N : 0, lane, p.k, xt, t, head + b * N, min(64, v1 - b) * N);
-      }
+      for (int j = 0; j < N; ++j) f[q][j] = lane < valid[q] ? load_elem(&v[q].e[j]) : -INFINITY;
     }
-    const int tail = head + vecs * N;
-    if (wr == W - 1 && tail < p.vocab) {
-      const int i = tail + lane;
-      const float one[1] = {i < p.vocab ? load_elem(x + i) : -INFINITY};
-      a.step<1>(one, i, i < p.vocab, lane, p.k, xt, t, tail, p.vocab - tail);
-    }
-    if (wr == 0 && head) {
-      const float one[1] = {lane < head ? load_elem(x + lane) : -INFINITY};
-      a.full = false;                    // lower indices than what is held: equal values have to be looked at
-      a.step<1>(one, lane, lane < head, lane, p.k, xt, t, 0, head);
-    }
-    for (int o = 32; o; o >>= 1) {
-      a.s += __shfl_xor(a.s, o);
-      a.u += __shfl_xor(a.u, o);
-      a.above += __shfl_xor(a.above, o);
-    }
+    load(c + 64 * Q);
+    a.batch<Q, N>(f, head + c * N, valid, lane, p.k, xt, t);
+  }
+  const int tail = head + vecs * N;
+  if (wr == W - 1 && tail < p.vocab) {
+    const int valid[1] = {p.vocab - tail};
+    const float one[1][1] = {{lane < valid[0] ? load_elem(x + tail + lane) : -INFINITY}};
+    a.batch<1, 1>(one, tail, valid, lane, p.k, xt, t);
+  }
+  if (wr == 0 && head) {
+    const int valid[1] = {head};
+    const float one[1][1] = {{lane < head ? load_elem(x + lane) : -INFINITY}};
+    a.full = false;                      // lower indices than what is held: equal values have to be looked at
+    a.batch<1, 1>(one, 0, valid, lane, p.k, xt, t);
+  }
+  for (int o = 32; o; o >>= 1) {
+    a.s += __shfl_xor(a.s, o);
+    a.u += __shfl_xor(a.u, o);
   }
   if constexpr (W > 1) {
     if (lane == 0) {
@@ -396,24 +425,32 @@ __global__ void __launch_bounds__(64 * W * ROWS) scores_long_kernel(ScoreArgs p)
       part_f[wave][2] = a.u;
       part_i[wave] = a.above;
     }
-    if (lane < p.k) part_k[wave][lane] = a.best.key;
-    __syncthreads();
-    if (wr != 0 || !here) return;
+    // the waves' lists in pairs: of two lists in descending order, the larger of each entry and the other's mirror image
+    // are the 64 best, in an order that log2(64) exchanges sort
+#pragma unroll
+    for (int w = W / 2; w >= 1; w /= 2) {
+      if (p.k) {
+        if (wave >= w && wave < 2 * w) part_k[wave - w][63 - lane] = a.best.key;
+        __syncthreads();
+        if (wave < w) a.best.join(part_k[wave][lane], lane);
+        if (w > 1) __syncthreads();
+      }
+    }
+    if (!p.k) __syncthreads();
+    if (wr != 0) return;
     float m = a.m;
-    for (int w = 1; w < W; ++w) m = fmaxf(m, part_f[wave + w][0]);
+    for (int w = 1; w < W; ++w) m = fmaxf(m, part_f[w][0]);
     float s = 0.f, u = 0.f;
     a.above = 0;
     for (int w = 0; w < W; ++w) {
-      const float d = fmaxf(part_f[wave + w][0] - m, -200.f), f = exp_neg(d);
-      u += f * fmaf(d, part_f[wave + w][1], part_f[wave + w][2]);
-      s += f * part_f[wave + w][1];
-      a.above += part_i[wave + w];
+      const float d = fmaxf(part_f[w][0] - m, -200.f), f = exp_neg(d);
+      u += f * fmaf(d, part_f[w][1], part_f[w][2]);
+      s += f * part_f[w][1];
+      a.above += part_i[w];
     }
     a.m = m;
     a.s = s;
     a.u = u;
-    if (p.k)
-      for (int w = 1; w < W; ++w) a.best.take(lane < p.k ? part_k[wave + w][lane] : 0, lane, p.k);
   }
   const bool left = a.s != 0.f;
   const float ls = logf(a.s);
