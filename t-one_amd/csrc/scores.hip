@@ -38,10 +38,8 @@ __device__ __forceinline__ int order_of(float v) {
 __device__ __forceinline__ uint64_t key_of(float v, int i) {
   return ((uint64_t)((uint32_t)order_of(v) ^ 0x80000000u) << 32) | (uint32_t)~i;
 }
-__device__ __forceinline__ float key_value(uint64_t key) {
-  const int o = (int)((uint32_t)(key >> 32) ^ 0x80000000u);
-  return __int_as_float(o < 0 ? o ^ 0x7fffffff : o);
-}
+__device__ __forceinline__ float value_of(int order) { return __int_as_float(order < 0 ? order ^ 0x7fffffff : order); }
+__device__ __forceinline__ float key_value(uint64_t key) { return value_of((int)((uint32_t)(key >> 32) ^ 0x80000000u)); }
 __device__ __forceinline__ int key_index(uint64_t key) { return (int)~(uint32_t)key; }
 
 // lane ^ X of a 16-lane row without LDS (DPP); X = 16 or 32: ds_bpermute
@@ -68,6 +66,16 @@ __device__ __forceinline__ uint64_t read_lane(uint64_t v, int lane) {
 }
 __device__ __forceinline__ float read_lane(float v, int lane) {
   return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), lane));
+}
+
+// a commutative operation over the wave's 64 lanes, in a fixed order; uniform
+template <class Op>
+__device__ __forceinline__ float over_wave(float v, Op&& op) {
+  v = op(v, xor_lane<1>(v));
+  v = op(v, xor_lane<2>(v));
+  v = op(v, xor_lane<7>(v));
+  v = op(v, xor_lane<15>(v));
+  return op(op(read_lane(v, 0), read_lane(v, 16)), op(read_lane(v, 32), read_lane(v, 48)));
 }
 
 // what a row that is none gives
@@ -265,31 +273,39 @@ struct Part {
   float floor = -INFINITY;               // value of the k-th best, or the maximum for k = 0
   bool full = false;                     // k entries seen
   Best best;
+  int* shared;                           // the largest floor of the row's waves, as order_of
 
   // x[q][j]: entry base + q * span + lane * N + j; those of lanes from valid[q] on are none (-inf)
   template <int Q, int N>
   __device__ __forceinline__ void batch(const float (&x)[Q][N], int base, const int (&valid)[Q], int lane, int k, float xt, int t) {
     float top[Q], most;
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
+    for (int q = 0; q < Q; ++q) {        // steps of which no lane has an entry are left out here and below
+      if (q && valid[q] <= 0) continue;
       top[q] = x[q][0];
 #pragma unroll
       for (int j = 1; j < N; ++j) top[q] = fmaxf(top[q], x[q][j]);
       most = q ? fmaxf(most, top[q]) : top[q];
     }
-    if (!full || __ballot(most > floor)) news<Q, N>(x, top, most, base, valid, lane, k);
+    const float other = shared ? value_of(*static_cast<volatile int*>(shared)) : -INFINITY;
+    if ((!full || __ballot(most > floor)) && (k == 0 || __ballot(most >= other)))
+      news<Q, N>(x, top, most, other, base, valid, lane, k);
+    else if (__ballot(most > m)) larger(most);
 #pragma unroll
-    for (int q = 0; q < Q; ++q)
+    for (int q = 0; q < Q; ++q) {
+      if (q && valid[q] <= 0) continue;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float z = x[q][j] - m, e = exp_neg(z);
         s += e;
         u = fmaf(e, fmaxf(z, -200.f), u);   // as in the short form
       }
+    }
     // entries above x_t; equal ones count below index t
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int b = base + q * 64 * N;
+      if (t < 0 || (q && valid[q] <= 0)) continue;
       if (t >= b + 64 * N) {
 #pragma unroll
         for (int j = 0; j < N; ++j) above += __builtin_popcountll(__ballot(x[q][j] >= xt && lane < valid[q]));
@@ -304,14 +320,8 @@ struct Part {
     }
   }
 
-  template <int Q, int N>
-  __device__ __forceinline__ void news(const float (&x)[Q][N], const float (&top)[Q], float most, int base, const int (&valid)[Q], int lane, int k) {
-    float w = most;
-    w = fmaxf(w, xor_lane<1>(w));
-    w = fmaxf(w, xor_lane<2>(w));
-    w = fmaxf(w, xor_lane<7>(w));
-    w = fmaxf(w, xor_lane<15>(w));
-    w = fmaxf(fmaxf(read_lane(w, 0), read_lane(w, 16)), fmaxf(read_lane(w, 32), read_lane(w, 48)));
+  __device__ __forceinline__ void larger(float most) {
+    const float w = over_wave(most, [](float p_, float q_) { return fmaxf(p_, q_); });
     if (w > m) {
       // s and u to the new maximum: e^(x - w) = e^(x - m) e^d, (x - w) = (x - m) + d; d bounded as in the sums
       const float d = fmaxf(m - w, -200.f), f = exp_neg(d);
@@ -319,6 +329,12 @@ struct Part {
       s *= f;
       m = w;
     }
+  }
+
+  template <int Q, int N>
+  __device__ __forceinline__ void news(const float (&x)[Q][N], const float (&top)[Q], float most, float other, int base, const int (&valid)[Q], int lane,
+                                       int k) {
+    larger(most);
     if (k == 0) {
       floor = m;
       full = true;
@@ -327,30 +343,35 @@ struct Part {
     int best_at = -1;
     if (!best.any()) {
       // nothing held yet: the lanes' largest first, which sets a floor close to the final one
-      uint64_t mine = 0;
+      best_at = 0;                       // (a lane of NaN: its first entry)
+      float largest = x[0][0];
 #pragma unroll
-      for (int q = 0; q < Q; ++q)
+      for (int q = Q - 1; q >= 0; --q) {
+        if (q && valid[q] <= 0) continue;
 #pragma unroll
-        for (int j = 0; j < N; ++j) {
-          const uint64_t key = lane < valid[q] ? key_of(x[q][j], base + (q * 64 + lane) * N + j) : 0;
-          if (key > mine) {
-            mine = key;
+        for (int j = N - 1; j >= 0; --j)
+          if (x[q][j] == most) {
             best_at = q * N + j;
+            largest = most;
           }
-        }
-      best.sort(mine, lane, k);
+      }
+      best.sort(lane < valid[0] ? key_of(largest, base + (best_at / N * 64 + lane) * N + best_at % N) : 0, lane, k);
     }
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      const float low = best.floor ? key_value(best.floor) : -INFINITY;
-      if (best.floor && __ballot(top[q] >= low) == 0) continue;      // (a NaN is above no floor, but fills a list)
+      // nothing below another wave's floor can be among the row's k best; what equals it can, by its index
+      const float low = fmaxf(best.floor ? key_value(best.floor) : -INFINITY, other);
+      if ((q && valid[q] <= 0) || (best.floor && __ballot(top[q] >= low) == 0)) continue;      // (a NaN is above no floor, but fills a list)
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (!best.floor || __ballot(x[q][j] >= low))
           best.take(lane < valid[q] && q * N + j != best_at ? key_of(x[q][j], base + (q * 64 + lane) * N + j) : 0, lane, k);
     }
     full = best.floor != 0;
-    if (full) floor = key_value(best.floor);
+    if (full) {
+      floor = key_value(best.floor);
+      if (shared && lane == 0) atomicMax(shared, order_of(floor));
+    }
   }
 };
 
@@ -371,8 +392,15 @@ __global__ void __launch_bounds__(64 * W * ROWS) scores_long_kernel(ScoreArgs p)
     if (in && wr == 0) write_none(p, n, lane, 64);
     return;
   }
+  __shared__ int s_floor;
   Part a;
   a.best.clear();
+  a.shared = nullptr;
+  if constexpr (W > 1) {
+    if (threadIdx.x == 0) s_floor = order_of(-INFINITY);
+    __syncthreads();
+    a.shared = &s_floor;
+  }
   const T* x = static_cast<const T*>(p.x) + row * p.stride;
   int t = p.tokens ? p.tokens[n] : -1;
   if (t < 0 || t >= p.vocab) t = -1;
@@ -414,10 +442,8 @@ __global__ void __launch_bounds__(64 * W * ROWS) scores_long_kernel(ScoreArgs p)
     a.full = false;                      // lower indices than what is held: equal values have to be looked at
     a.batch<1, 1>(one, 0, valid, lane, p.k, xt, t);
   }
-  for (int o = 32; o; o >>= 1) {
-    a.s += __shfl_xor(a.s, o);
-    a.u += __shfl_xor(a.u, o);
-  }
+  a.s = over_wave(a.s, [](float p_, float q_) { return p_ + q_; });
+  a.u = over_wave(a.u, [](float p_, float q_) { return p_ + q_; });
   if constexpr (W > 1) {
     if (lane == 0) {
       part_f[wave][0] = a.m;
@@ -487,9 +513,14 @@ hipError_t launch_as(const ScoreArgs& p, hipStream_t st) {
     }
     return hipGetLastError();
   }
-  const int64_t steps = (p.vocab / Vec<T>::N + 63) / 64;     // 64-lane loads a row takes
-  if (steps >= 16 && p.n < 1024) hipLaunchKernelGGL((scores_long_kernel<T, 16, 1>), dim3((unsigned)p.n), dim3(1024), 0, st, p);
-  else if (steps >= 8) hipLaunchKernelGGL((scores_long_kernel<T, 4, 1>), dim3((unsigned)p.n), dim3(256), 0, st, p);
+  // Waves per row, by the 64-lane loads it takes (measured, us, k = 10, with 1 / 4 / 16 waves): few rows are a matter of one
+  // row's time (bf16 65,537: 1 row 79 / 31 / 19, 256 rows 93 / 35 / 22, 400 rows 92 / 40 / 40; 5000: 256 rows 17 / 10 / 11), and
+  // from some 2000 rows on the card is full with one wave each (bf16 5000: 1024 rows 17 / 13 / 34, 2048 19 / 20 / 63, 16,384
+  // 73 / 116 / 462; 32,000: 2048 rows 63 / 58 / 92, 4096 87 / 98 / 177; 1000: 1024 rows 8 / 10 / 41).
+  const int64_t steps = (p.vocab / Vec<T>::N + 63) / 64;
+  if (steps >= 20 && p.n <= 256) hipLaunchKernelGGL((scores_long_kernel<T, 16, 1>), dim3((unsigned)p.n), dim3(1024), 0, st, p);
+  else if (steps >= 4 && p.n <= (steps >= 32 ? 2048 : 1536))
+    hipLaunchKernelGGL((scores_long_kernel<T, 4, 1>), dim3((unsigned)p.n), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((scores_long_kernel<T, 1, 4>), dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, p);
   return hipGetLastError();
 }
