@@ -52,6 +52,28 @@ class TextPhrase:
 
 
 @dataclass
+class TokenScore:
+    """One character of a scored phrase: its frames' times, the mean log probability of the character over them, and at the
+    frame where it is most likely the entropy (nats) and the best tokens there with their log probabilities (the blank: "")."""
+    text: str
+    start_time: float
+    end_time: float
+    logprob: float
+    entropy: float
+    alternatives: list[tuple[str, float]]
+
+
+@dataclass
+class ScoredPhrase(TextPhrase):
+    """A phrase with its text aligned to its frames.  ``score``: log probability of the best alignment, ``total``: of the
+    text, over all alignments; both None, and no tokens, for a text that has characters outside the labels, is too long to
+    align (scoring.MAX_TOKENS) or fits no alignment."""
+    score: Optional[float] = None
+    total: Optional[float] = None
+    tokens: list[TokenScore] = field(default_factory=list)
+
+
+@dataclass
 class FrameSplitterState:
     """Frames carried between steps (the reference keeps the logprob rows, logprob_splitter.py:36-40).
     ``tokens`` is the per-frame payload: greedy tokens (L,) int32, or the logprob rows (L, 35) float32
@@ -117,6 +139,17 @@ def phrase_times(start_frame: int, end_frame: int) -> tuple[float, float]:
     return st, max(st, round(end_frame * C.FRAME_SIZE - shift, 2))
 
 
+def frame_time(frame: int) -> float:
+    """The time of a frame's beginning on the scale of :func:`phrase_times`."""
+    return max(0, round(frame * C.FRAME_SIZE - (C.MEAN_TIME_BIAS + PADDING / C.SAMPLE_RATE), 2))
+
+
+def text_tokens(text: str) -> Optional[list[int]]:
+    """Label ids of a text, None where it has a character that is no label."""
+    ids = [LABELS.find(c) for c in text]
+    return None if -1 in ids else ids
+
+
 def frames_to_phrases(tokens, speech, state, *, is_last=False, decode=greedy_text
                       ) -> tuple[list[TextPhrase], FrameSplitterState]:
     """``decode`` maps a phrase's payload to its text: greedy_text on tokens, or a host decoder's
@@ -143,14 +176,22 @@ class StreamingGreedyPipeline:
     phrases are still cut by the device speech flags, and each finished phrase's logprob rows go to
     ``decoder.forward`` exactly as tone/pipeline.py:146-150 does.  Without it the text is the device's
     greedy tokens (10 ids + 10 bits per stream-chunk cross PCIe).
+
+    ``scores``: number of alternatives per character (0 to 35), or None.  With it the step's logprob rows stay on the device
+    in a paged store (:class:`tone_amd.scoring.FrameStore`: ``score_pages`` pages of 64 frames, by default enough for every
+    slot's longest phrase) until their phrase ends, and each finished phrase comes back as a :class:`ScoredPhrase`: its text --
+    the greedy one or the host decoder's -- aligned to its frames, with times, log probabilities and alternatives.
     """
 
     CHUNK_SIZE = C.AUDIO_CHUNK_SAMPLES   # 300 ms; a session built with chunk_samples=3200 serves 400 ms chunks
 
-    def __init__(self, session, n_slots: int, decoder=None, resident: bool = True):
+    def __init__(self, session, n_slots: int, decoder=None, resident: bool = True, scores: Optional[int] = None,
+                 score_pages: Optional[int] = None):
         import torch
         if n_slots <= 0:
             raise ValueError("n_slots must be positive")
+        if scores is not None and not 0 <= scores <= C.VOCAB:
+            raise ValueError(f"scores must be in 0 .. {C.VOCAB}, got {scores}")
         self.session = session
         self.n_slots = int(n_slots)
         self.CHUNK_SIZE = int(getattr(session, "chunk_samples", C.AUDIO_CHUNK_SAMPLES))
@@ -176,6 +217,13 @@ class StreamingGreedyPipeline:
         self._logp_h = torch.zeros((mb, fr, C.VOCAB), dtype=torch.float32).pin_memory() \
             if decoder is not None else None
         self._last_logp: Optional[np.ndarray] = None
+        self.scores = scores
+        self._store = None
+        if scores is not None:
+            from .scoring import FrameStore
+            # the splitter holds a phrase until it is cut, the silence behind it and the step's frames
+            self._store = FrameStore(self.n_slots, MAX_PHRASE + 2 * (MIN_SILENCE + SPEECH_EXPAND + fr), n_pages=score_pages,
+                                     device=dev.index)
 
     def _fresh_state(self) -> FrameSplitterState:
         if self.decoder is None:
@@ -199,6 +247,8 @@ class StreamingGreedyPipeline:
             raise KeyError(f"slot {slot} is not open")
         del self._open[slot]
         self._free.append(slot)
+        if self._store is not None:
+            self._store.release([slot])
 
     @property
     def open_slots(self) -> list[int]:
@@ -225,6 +275,12 @@ class StreamingGreedyPipeline:
         mb = self.session.max_batch
         info = np.empty((n, self.frames), np.int32)
         logp = np.empty((n, self.frames, C.VOCAB), np.float32) if self.decoder is not None else None
+        kept = None
+        if self._store is not None:
+            # before the step, so that a store out of pages raises with the streams as they were; frames before the
+            # splitter's buffer are of no phrase to come
+            from .scoring import frames_put
+            kept = self._store.reserve(slots, self.frames, keep=[self._open[s].offset for s in slots])
         self.session.set_frame_info(self._info)    # frame_info is session state: claim it every step
         for b0 in range(0, n, mb):
             b1 = min(n, b0 + mb)
@@ -244,6 +300,8 @@ class StreamingGreedyPipeline:
             else:
                 self.session.run_rows(self._sig[:nb], self._rows[0, :nb], self._rows[1, :nb], self._slab,
                                       self._logp, check_rows=False)
+            if kept is not None:
+                frames_put(self._logp[:nb], kept[b0:b1], self._store.pool)
             self._info_h[:nb].copy_(self._info[:nb], non_blocking=True)
             if logp is not None:
                 self._logp_h[:nb].copy_(self._logp[:nb], non_blocking=True)
@@ -272,15 +330,62 @@ class StreamingGreedyPipeline:
         is_last = [False] * n if is_last is None else list(is_last)
         info = self.step_frames(chunks, slots) if n else np.zeros((0, self.frames), np.int32)
         out: list[list[TextPhrase]] = []
+        held = {slot: self._open[slot].offset for slot in slots}
         for i, slot in enumerate(slots):
             toks, speech = decode_frame_info(info[i])
+            if self._store is not None:
+                payload = toks if self.decoder is None else self._last_logp[i]
+                found, self._open[slot] = split_frames(payload, speech, self._open[slot], is_last=is_last[i])
+                decode = greedy_text if self.decoder is None else self.decoder.forward
+                out.append([(ScoredPhrase(decode(t), *phrase_times(s, e)), max(held[slot], s - SPEECH_EXPAND), len(t))
+                            for t, s, e in found])
+                continue
             if self.decoder is None:
                 phrases, self._open[slot] = frames_to_phrases(toks, speech, self._open[slot], is_last=is_last[i])
             else:
                 phrases, self._open[slot] = frames_to_phrases(self._last_logp[i], speech, self._open[slot],
                                                               is_last=is_last[i], decode=self.decoder.forward)
             out.append(phrases)
-        return out
+        return out if self._store is None else self._scored(out, slots)
+
+    def _scored(self, found, slots) -> list[list[TextPhrase]]:
+        """Fill in the phrases' scores: found[i] = [(phrase, first frame, frames)] of stream slots[i]."""
+        import torch
+
+        from .scoring import MAX_TOKENS, ctc_align, token_scores
+        todo = []
+        for slot, phrases in zip(slots, found):
+            for phrase, begin, count in phrases:
+                ids = text_tokens(phrase.text)
+                if ids is not None and len(ids) <= MAX_TOKENS:
+                    todo.append((phrase, slot, begin, count, ids))
+        if todo:
+            most = max(len(ids) for *_, ids in todo)
+            tokens = np.full((len(todo), most), -1, np.int32)
+            lens = np.zeros((2, len(todo)), np.int32)
+            for j, (_, _, _, count, ids) in enumerate(todo):
+                tokens[j, : len(ids)] = ids
+                lens[:, j] = len(ids), count
+            dev = self.session.dev
+            rows = self._store.slots([s for _, s, *_ in todo], [b for _, _, b, *_ in todo], lens[1])
+            lens_d = torch.from_numpy(lens).to(dev)
+            a = ctc_align(self._store.pool, torch.from_numpy(tokens).to(dev), lens_d[0], lens_d[1], rows=rows, total=True)
+            r = token_scores(self._store.pool, a.labels, k=self.scores, rows=rows)
+            spans, logprob, entropy = a.spans.cpu().numpy(), r.logprob.cpu().numpy(), r.entropy.cpu().numpy()
+            score, total = a.score.cpu().numpy(), a.total.cpu().numpy()
+            top_ids, top_lp = (r.top_ids.cpu().numpy(), r.top_logprob.cpu().numpy()) if self.scores else (None, None)
+            for j, (phrase, _, begin, _, ids) in enumerate(todo):
+                if not np.isfinite(score[j]):
+                    continue
+                phrase.score, phrase.total = float(score[j]), float(total[j])
+                for i, t in enumerate(ids):
+                    s, e = (int(v) for v in spans[j, i])
+                    at = s + int(np.argmax(logprob[j, s:e]))
+                    more = [] if top_ids is None else [(LABELS[v] if v < len(LABELS) else "", float(lp))
+                                                       for v, lp in zip(top_ids[j, at].tolist(), top_lp[j, at])]
+                    phrase.tokens.append(TokenScore(LABELS[t], frame_time(begin + s), frame_time(begin + e), float(logprob[j, s:e].mean()),
+                                                    float(entropy[j, at]), more))
+        return [[phrase for phrase, *_ in phrases] for phrases in found]
 
     def forward_offline(self, audio: np.ndarray) -> list[TextPhrase]:
         """tone/pipeline.py:178-200 on one stream: pad 300 ms both sides, pad to whole chunks, decode."""

@@ -4,7 +4,7 @@ The acoustic path answers with a row of log probabilities per 30 ms frame (``Ton
 those rows where they are, on the device, until the phrase they belong to has ended:
 
 * ``frames_plan`` / ``frames_slots`` -- page tables and slot maps from the streams' frame counts, ``frames_put`` -- a step's
-  rows written through such a map; :class:`FrameStore` keeps the buffers and the counts for them;
+  rows written through such a map; :class:`FrameStore` keeps their buffers and counts;
 * ``token_scores`` -- per row the log probability of a given token, its rank, the entropy, the k best tokens;
 * ``ctc_align`` -- the best path of given token sequences, each token's frames, the log probability of all paths.
 
@@ -17,6 +17,8 @@ current stream of the tensors' device.  Contents are checked on the device: an i
 from __future__ import annotations
 
 from typing import NamedTuple, Optional
+
+import numpy as np
 
 from . import _lib
 from . import config as C
@@ -325,3 +327,136 @@ def ctc_align(x, tokens, token_lens, frame_lens, rows=None, blank: int = C.BLANK
                                       tokens.data_ptr(), most, token_lens.data_ptr(), frame_lens.data_ptr(), score.data_ptr(),
                                       _ptr(tot), labels.data_ptr(), spans.data_ptr(), _ptr(ws), need, st), "tone_ctc_align")
     return CtcAlignment(score, tot, labels, spans)
+
+
+# --- a store of frames ------------------------------------------------------------------------------------------------
+
+class FrameStore:
+    """The latest rows of many streams, in pages of one pool on the device.
+
+    Stream i holds its frames [first, length), counted from its start.  :meth:`append` adds a step's rows for any subset of
+    the streams (:meth:`reserve`: only their slots) and lets go of the frames before ``keep``; :meth:`slots` gives the pool rows of a range of frames, for
+    ``token_scores`` / ``ctc_align`` with ``rows=``.  Page tables, slot maps and the free list live on the device; the host
+    keeps the counts, so a call that would run out of pages raises before anything has changed.  The calls on one store
+    belong on one stream (or ordered by events); the pool and the tables are the store's own."""
+
+    def __init__(self, n_streams: int, max_frames: int, *, page_size: int = 64, n_pages: Optional[int] = None, vocab: int = C.VOCAB,
+                 dtype=None, device: int = 0):
+        """``max_frames``: the most a stream holds at once.  ``n_pages``: pages of the pool, by default enough for every
+        stream at its most."""
+        torch = _torch()
+        if n_streams < 1 or max_frames < 1 or page_size < 1 or vocab < 1:
+            raise ValueError("n_streams, max_frames, page_size and vocab must be positive")
+        dtype = torch.float32 if dtype is None else dtype
+        if dtype not in (torch.float32, torch.float16, torch.bfloat16):
+            raise ValueError(f"dtype must be float32, float16 or bfloat16, got {dtype}")
+        self.n_streams, self.max_frames, self.page_size = int(n_streams), int(max_frames), int(page_size)
+        self.width = -(-self.max_frames // self.page_size) + 1          # a range of frames can begin inside a page
+        self.n_pages = int(n_pages) if n_pages is not None else self.n_streams * self.width
+        if self.n_pages < 1:
+            raise ValueError("n_pages must be positive")
+        if not torch.cuda.is_available():
+            raise RuntimeError("FrameStore needs a ROCm GPU (torch.cuda.is_available() is False)")
+        self.dev = torch.device("cuda", int(device))
+        self.pool = torch.zeros((self.n_pages * self.page_size, vocab), dtype=dtype, device=self.dev)
+        self._table = torch.full((2 * self.n_streams, self.width), -1, dtype=torch.int32, device=self.dev)
+        self._queue = torch.arange(self.n_pages, dtype=torch.int32, device=self.dev)
+        self._cursors = torch.tensor([[0, self.n_pages], [0, 0]], dtype=torch.int64, device=self.dev)
+        self._side = 0                                                   # which cursors are current
+        self.first = np.zeros(self.n_streams, np.int64)
+        self.length = np.zeros(self.n_streams, np.int64)
+        self._parity = np.zeros(self.n_streams, np.int64)
+        self.free_pages = self.n_pages
+
+    def _ids(self, ids) -> np.ndarray:
+        ids = np.asarray(ids, np.int64).reshape(-1)
+        if ids.size and (ids.min() < 0 or ids.max() >= self.n_streams):
+            raise ValueError(f"stream ids must be in [0, {self.n_streams})")
+        return ids
+
+    def _upload(self, *columns):
+        """int32 columns as one device tensor, through pinned memory that the copy keeps until it is done."""
+        torch = _torch()
+        n = columns[0].shape[0]
+        host = torch.empty((len(columns), n), dtype=torch.int32, pin_memory=True)
+        view = host.numpy()
+        for row, c in zip(view, columns):
+            row[:] = c
+        return host.to(self.dev, non_blocking=True)
+
+    def _plan(self, ids, keep, add, max_add):
+        if len(set(ids.tolist())) != ids.size:
+            raise ValueError("stream ids must be distinct")
+        first, length, page = self.first[ids], self.length[ids], self.page_size
+        kept, end = np.maximum(first, keep), length + add
+        if (keep < 0).any() or (kept > end).any() or (end >= 2 ** 31).any():
+            raise ValueError("keep must be in 0 .. length + count, and frame numbers below 2^31")
+        if (end - kept > self.max_frames).any():
+            raise ValueError(f"a stream would hold more than max_frames = {self.max_frames} frames")
+        lo0, lo1 = first // page, kept // page
+        hi0, hi1 = np.where(first < length, -(-length // page), lo0), np.where(kept < end, -(-end // page), lo1)
+        had, has = first < length, kept < end
+        take = int(np.where(has, hi1 - np.where(had, np.maximum(hi0, lo1), lo1), 0).sum())
+        drop = int(np.where(had, np.where(has, np.minimum(hi0, lo1), hi0) - lo0, 0).sum())
+        if take > self.free_pages:
+            raise RuntimeError(f"out of pages: {take} needed, {self.free_pages} of {self.n_pages} free")
+        rows = 2 * ids + self._parity[ids]
+        req = self._upload(rows, rows ^ 1, first, length, keep, add)
+        slots, _ = frames_plan(self._table, self._queue, self._cursors[self._side], self._cursors[1 - self._side], *req.unbind(0),
+                               page_size=page, max_add=max_add)
+        self._side = 1 - self._side
+        self.first[ids], self.length[ids] = kept, end
+        self._parity[ids] ^= 1
+        self.free_pages += drop - take
+        return slots
+
+    def reserve(self, ids, frames: int, keep=None, counts=None, stream=None):
+        """Slots int64 (n, frames) for the next counts[i] (default: ``frames``) frames of the streams ``ids`` (distinct), to be
+        written with :func:`frames_put`.  Frames before keep[i] (default: none) are let go; new ones among them get no slot."""
+        torch = _torch()
+        ids = self._ids(ids)
+        add = np.full(ids.size, frames, np.int64) if counts is None else np.asarray(counts, np.int64).reshape(-1)
+        keep = self.first[ids] if keep is None else np.asarray(keep, np.int64).reshape(-1)
+        if add.shape != ids.shape or keep.shape != ids.shape or (add < 0).any() or (add > frames).any():
+            raise ValueError(f"counts must be {ids.size} numbers in 0 .. {frames}, keep {ids.size} frame numbers")
+        with (torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.dev)):
+            return self._plan(ids, keep, add, frames)
+
+    def append(self, rows, ids, keep=None, counts=None, stream=None):
+        """Add ``rows`` (n, T, vocab) to the streams ``ids``: :meth:`reserve` and the copy.  Returns the slots (n, T)."""
+        torch = _torch()
+        ids = self._ids(ids)
+        if rows.dim() != 3 or rows.shape[0] != ids.size or rows.shape[2] != self.pool.shape[1]:
+            raise ValueError(f"rows must be ({ids.size}, T, {self.pool.shape[1]}), got {tuple(rows.shape)}")
+        if rows.device != self.dev:
+            raise ValueError(f"rows on {rows.device}, the store on {self.dev}")
+        _type(rows, "rows")
+        _rows_of(rows, "rows")
+        slots = self.reserve(ids, int(rows.shape[1]), keep, counts, stream)
+        frames_put(rows, slots, self.pool, stream=stream)
+        return slots
+
+    def release(self, ids, stream=None) -> None:
+        """Let go of all frames of the streams ``ids``; they start again at frame 0."""
+        torch = _torch()
+        ids = self._ids(ids)
+        if ids.size == 0:
+            return
+        with (torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.dev)):
+            self._plan(ids, self.length[ids], np.zeros(ids.size, np.int64), 0)
+        self.first[ids] = self.length[ids] = 0
+
+    def slots(self, ids, begin, count, stream=None):
+        """Pool rows int64 (n, max(count)) of the frames begin[i] .. begin[i] + count[i] - 1 of stream ids[i], -1 behind
+        them.  A stream may be named more than once."""
+        torch = _torch()
+        ids = self._ids(ids)
+        begin, count = np.asarray(begin, np.int64).reshape(-1), np.asarray(count, np.int64).reshape(-1)
+        if begin.shape != ids.shape or count.shape != ids.shape:
+            raise ValueError("ids, begin and count must have one entry per range")
+        if (count < 0).any() or (begin < self.first[ids]).any() or (begin + count > self.length[ids]).any():
+            raise ValueError("ranges must lie inside the frames their streams hold")
+        most = int(count.max()) if ids.size else 0
+        with (torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.dev)):
+            req = self._upload(2 * ids + self._parity[ids], self.first[ids], begin, count)
+            return frames_slots(self._table, *req.unbind(0), page_size=self.page_size, n_pages=self.n_pages, max_count=most)

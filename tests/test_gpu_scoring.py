@@ -665,3 +665,193 @@ def test_the_phrase_path():
                 assert r.logprob[i, t].item() == 0.0
             else:
                 assert abs(r.logprob[i, t].item() - data[i, t, labels[i, t]]) <= 1e-5
+
+
+# --- the store and the pipeline ---------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("page,dtype", [(64, "fp32"), (7, "fp16"), (1, "bf16")])
+def test_store_against_a_list_of_rows(page, dtype):
+    """Random appends, ranges read, streams released: every frame a stream holds reads back as it was put."""
+    rng = np.random.default_rng(page)
+    n, t, most = 9, 13, 90
+    store = S().FrameStore(n, most, page_size=page, n_pages=n * (-(-most // page) + 1) - 3, vocab=6, dtype=TYPES[dtype])
+    held = [np.zeros((0, 6)) for _ in range(n)]
+    first = np.zeros(n, int)
+    for step in range(40):
+        ids = rng.permutation(n)[: rng.integers(1, n + 1)]
+        rows = _rows(len(ids) * t, 6, dtype, step).view(len(ids), t, 6)
+        counts = rng.integers(0, t + 1, len(ids)) if step % 2 else None
+        end = first[ids] + [len(held[i]) for i in ids] + (t if counts is None else counts)
+        keep = np.maximum(first[ids], end - rng.integers(0, most + 1, len(ids)))
+        store.append(rows, ids, keep=keep, counts=counts)
+        for j, i in enumerate(ids):
+            new = rows[j, : (t if counts is None else counts[j])].float().cpu().numpy()
+            held[i] = np.concatenate([held[i], new])[keep[j] - first[i] :]
+            first[i] = keep[j]
+        if step % 7 == 3:
+            gone = rng.permutation(n)[:2]
+            store.release(gone)
+            for i in gone:
+                held[i], first[i] = held[i][:0], 0
+        pages = sum(-(-(first[i] + len(held[i])) // page) - first[i] // page for i in range(n) if len(held[i]))
+        assert store.free_pages == store.n_pages - pages
+        ids = rng.integers(0, n, 5)
+        count = np.array([rng.integers(0, len(held[i]) + 1) for i in ids])
+        begin = np.array([first[i] + rng.integers(0, len(held[i]) - c + 1) for i, c in zip(ids, count)])
+        slots = store.slots(ids, begin, count)
+        assert slots.shape == (5, count.max())
+        for j, (i, b, c) in enumerate(zip(ids, begin, count)):
+            assert bool((slots[j, c:] == -1).all())
+            np.testing.assert_array_equal(store.pool[slots[j, :c]].float().cpu().numpy(), held[i][b - first[i] : b - first[i] + c])
+
+
+def test_store_refuses_and_stays_as_it_was():
+    store = S().FrameStore(3, 32, page_size=8, n_pages=6, vocab=5)
+    rows = _rows(30, 5, "fp32", 1).view(3, 10, 5)
+    slots = store.append(rows, [2, 0, 1])                # 2 pages each: all of them
+    before = store.pool.clone(), store._table.clone(), store._queue.clone(), store._cursors.clone(), store.first.copy(), store.length.copy()
+    with pytest.raises(RuntimeError, match="out of pages"):
+        store.append(rows, [0, 1, 2])
+    for bad in (dict(ids=[0, 0, 1]), dict(ids=[0, 1, 3]), dict(ids=[0, 1]), dict(ids=[0, 1, 2], keep=[0, 0, 21]),
+                dict(ids=[0, 1, 2], keep=[-1, 0, 0]), dict(ids=[0, 1, 2], counts=[11, 0, 0]), dict(ids=[0, 1, 2], counts=[1, 1])):
+        with pytest.raises(ValueError):
+            store.append(rows, **bad)
+    with pytest.raises(ValueError):
+        store.append(_rows(90, 5, "fp32", 1).view(3, 30, 5), [0, 1, 2])       # more than a stream holds
+    with pytest.raises(ValueError):
+        store.append(rows.cpu(), [0, 1, 2])
+    with pytest.raises(ValueError):
+        store.slots([0], [5], [6])
+    now = store.pool, store._table, store._queue, store._cursors
+    assert all(torch.equal(a, b) for a, b in zip(before, now)) and (store.first == before[4]).all() and (store.length == before[5]).all()
+    with pytest.raises(RuntimeError, match="out of pages"):                  # pages let go by a call are free from the next on
+        store.append(rows[:2], [0, 1], keep=[16, 20])
+    store.append(rows[1:2], [1], keep=[10], counts=[0])   # none of stream 1
+    assert store.free_pages == 2
+    store.append(rows[:1], [0], keep=[16])                # frames 16 .. 19 of stream 0
+    assert store.free_pages == 3 and torch.equal(store.pool[store.slots([0], [16], [4])[0]], rows[0, 6:])
+    assert torch.equal(store.pool[slots[0]], rows[0])     # stream 2 as it was
+    for bad in (dict(n_streams=0, max_frames=8), dict(n_streams=1, max_frames=0), dict(n_streams=1, max_frames=8, page_size=0),
+                dict(n_streams=1, max_frames=8, n_pages=0), dict(n_streams=1, max_frames=8, dtype=torch.int8)):
+        with pytest.raises(ValueError):
+            S().FrameStore(**bad)
+
+
+def test_store_on_a_stream_of_its_own():
+    store, want = S().FrameStore(2, 64, page_size=8, vocab=5), S().FrameStore(2, 64, page_size=8, vocab=5)
+    side = torch.cuda.Stream()
+    rows = _rows(40, 5, "fp32", 1).view(2, 20, 5)
+    side.wait_stream(torch.cuda.current_stream())
+    for _ in range(3):
+        store.append(rows, [1, 0], stream=side)
+        want.append(rows, [1, 0])
+    slots = store.slots([0, 1], [3, 0], [50, 60], stream=side)
+    side.synchronize()
+    assert torch.equal(slots, want.slots([0, 1], [3, 0], [50, 60])) and torch.equal(store.pool, want.pool)
+
+
+@pytest.fixture(scope="module")
+def session():
+    if not torch.cuda.is_available():
+        pytest.skip("no ROCm GPU")
+    from tone_amd.model import ToneSession
+    from tone_amd.weights import synthetic_weights
+    s = ToneSession(synthetic_weights(0), device=0, precision="fp32", max_batch=2)
+    yield s
+    s.close()
+
+
+def _speech(seed, chunks):
+    """Noise with pauses, so that phrases end inside the audio."""
+    rng = np.random.default_rng(seed)
+    x = np.clip(rng.normal(0, 2500, (chunks, 2400)), -32768, 32767).astype(np.int32)
+    x[chunks // 3 : chunks // 3 + 4] = 0
+    return x
+
+
+class _Fixed:
+    """A host decoder that answers one text whatever it hears."""
+
+    def __init__(self, text):
+        self.text = text
+
+    def forward(self, logprobs):
+        assert logprobs.dtype == np.float32 and logprobs.shape[1] == 35
+        return self.text
+
+
+@pytest.mark.parametrize("text", [None, "да нет", "", "\u0434\u0430!", "\u0430" * 300])
+def test_pipeline_scores_its_phrases(session, text, monkeypatch):
+    """StreamingGreedyPipeline(scores=...): the phrases of the plain pipeline, with the scores that the oracle gives for their
+    text on the same frames; more streams than a device batch, closed at different times."""
+    from tone_amd import pipeline as P
+    decoder = lambda: None if text is None else _Fixed(text)  # noqa: E731
+    chunks = {0: _speech(1, 14), 1: _speech(2, 9), 2: _speech(3, 14)}
+    plain, scored = P.StreamingGreedyPipeline(session, 3, decoder()), P.StreamingGreedyPipeline(session, 3, decoder(), scores=4)
+    # the rows as the pipeline puts them (a step's last bits depend on its batch size, so no replay of one stream gives them)
+    kept, put = [], S().frames_put
+    monkeypatch.setattr(S(), "frames_put", lambda x, slots, pool, stream=None: (kept.append(x.cpu().numpy()), put(x, slots, pool, stream))[1])
+    found, rows_of = {}, {i: [] for i in chunks}
+    for name, pipe in (("plain", plain), ("scored", scored)):
+        slots = {i: pipe.open_stream() for i in chunks}
+        got = {i: [] for i in chunks}
+        for step in range(14):
+            on = [i for i in chunks if step < len(chunks[i])]
+            kept.clear()
+            out = pipe.forward(np.stack([chunks[i][step] for i in on]), [slots[i] for i in on], [step == len(chunks[i]) - 1 for i in on])
+            for j, (i, phrases) in enumerate(zip(on, out)):
+                got[i] += phrases
+                if name == "scored":
+                    rows_of[i].append(np.concatenate(kept)[j])
+            for i in on:
+                if step == len(chunks[i]) - 1:
+                    pipe.close_stream(slots[i])
+        found[name] = got
+    assert scored._store.free_pages == scored._store.n_pages
+    assert sum(len(p) for p in found["plain"].values()) > 2
+    for i, audio in chunks.items():
+        rows = np.concatenate(rows_of[i]).astype(np.float64)
+        shift = 0.33 + 2400 / 8000
+        assert [(p.text, p.start_time, p.end_time) for p in found["scored"][i]] == [(p.text, p.start_time, p.end_time) for p in found["plain"][i]]
+        # the phrases' frames, from the splitter run on the same rows
+        st, spans = P.FrameSplitterState(), []
+        speech = np.exp(rows[:, 33]) + np.exp(rows[:, 34]) <= 0.9
+        for k in range(len(audio)):
+            before = st.offset
+            out, st = P.split_frames(np.arange(10 * k, 10 * k + 10), speech[10 * k : 10 * k + 10], st, is_last=k == len(audio) - 1)
+            spans += [(max(before, s - 3), len(t)) for t, s, _ in out]
+        assert len(spans) == len(found["scored"][i])
+        for p, (begin, count) in zip(found["scored"][i], spans):
+            ids = P.text_tokens(p.text)
+            if ids is None:
+                assert p.score is None and p.tokens == []
+                continue
+            score, total, labels, tok = O.align(rows[begin : begin + count], ids, 34)
+            if labels is None:
+                assert p.score is None and p.total is None and p.tokens == []
+                continue
+            assert p.score == float(np.float32(score)) and abs(p.total - total) <= (count + 1) * 16 * EPS + EPS * abs(total)
+            assert [t.text for t in p.tokens] == list(p.text)
+            for t, (a, b) in zip(p.tokens, tok):
+                assert t.start_time == max(0, round((begin + a) * 0.03 - shift, 2)) and t.end_time == max(0, round((begin + b) * 0.03 - shift, 2))
+                lp = rows[begin + a : begin + b, P.LABELS.index(t.text)]
+                assert abs(t.logprob - lp.mean()) <= 1e-5
+                best = rows[begin + a + int(np.argmax(lp))]
+                order = np.argsort(-best, kind="stable")[:4]
+                assert [v for v, _ in t.alternatives] == [P.LABELS[o] if o < 34 else "" for o in order]
+                assert np.abs(np.array([v for _, v in t.alternatives]) - best[order]).max() <= 1e-5
+                assert abs(t.entropy + (np.exp(best) * best).sum()) <= 1e-4
+
+
+def test_pipeline_out_of_pages_leaves_its_streams_as_they_were(session):
+    from tone_amd import pipeline as P
+    pipe = P.StreamingGreedyPipeline(session, 2, scores=0, score_pages=1)
+    a, b = pipe.open_stream(), pipe.open_stream()
+    chunk = _speech(1, 2)
+    pipe.forward(chunk[:1], [a])
+    state = pipe.state_of(b).clone()
+    with pytest.raises(RuntimeError, match="out of pages"):
+        pipe.forward(chunk[1:], [b])
+    assert torch.equal(pipe.state_of(b), state) and pipe._open[b].offset == 0
+    with pytest.raises(ValueError):
+        P.StreamingGreedyPipeline(session, 2, scores=36)
