@@ -11,6 +11,7 @@
 #include "scoring.h"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace tone {
 namespace {
@@ -35,7 +36,7 @@ struct PlanArgs {
   int n_rows, width;
   int32_t* queue;                       // [n_pages]
   int n_pages, page;
-  Divisor by_page;
+  Divisor by_page, by_pages;            // frames to pages; queue positions to rounds of the queue
   const int64_t* cursors_in;            // head, tail of the queue
   int64_t* cursors_out;
   const int32_t *rows_in, *rows_out, *first, *length, *keep, *add;   // [batch]
@@ -68,7 +69,6 @@ struct PutArgs {
   int64_t pool_stride, pool_rows;
 };
 
-constexpr int kPlanWaves = 16;          // of a workgroup, shared by its requests
 
 struct Request {
   int first, length, kept, end;         // frames held before: [first, length), after: [kept, end)
@@ -107,29 +107,40 @@ __device__ __forceinline__ Request read_request(const PlanArgs& p, int b) {
 }
 
 // One launch: every workgroup adds up the pages of all requests (24 bytes each, out of L2) to place its own ones, instead of a
-// scan kernel in front of a writing kernel.  blockIdx.x: kPlanWaves / per requests of `per` waves each, so that a request's
-// chain of dependent loads (its row, its pages, its slots) is walked by all of them at once; blockIdx.y: a share of the slots.
-__global__ void __launch_bounds__(64 * kPlanWaves) plan_kernel(PlanArgs p, int per) {
-  __shared__ int64_t part[kPlanWaves][4];
-  __shared__ int s_take[kPlanWaves], s_drop[kPlanWaves];
+// scan kernel in front of a writing kernel.  blockIdx.x: WAVES / per requests of `per` waves each, so that a request's chain
+// of dependent loads (its row, its pages, its slots) is walked by all of them at once; blockIdx.y: a share of the slots.
+// What bounds it is that chain: everything that does not depend on the sums is loaded in front of them.
+template <int WAVES>
+__global__ void __launch_bounds__(64 * WAVES) plan_kernel(PlanArgs p, int per) {
+  __shared__ int64_t part[WAVES][4];
+  __shared__ int s_take[WAVES], s_drop[WAVES];
   __shared__ int s_flags;
-  const int tid = threadIdx.x, wave = tid >> 6, rows = kPlanWaves / per, r0 = blockIdx.x * rows, r1 = min(p.batch, r0 + rows);
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), rows = WAVES / per, r0 = blockIdx.x * rows, r1 = min(p.batch, r0 + rows);
+  const int mine = wave / per, own = r0 + mine, at = (wave - mine * per) * 64 + (tid & 63), step = 64 * per;
+  const int64_t head = p.cursors_in[0], tail = p.cursors_in[1];
+  Request r;
+  int ri = -1, ro = -1;
+  if (own < r1) {
+    r = read_request(p, own);
+    ri = p.rows_in[own];
+    ro = p.rows_out[own];
+  }
   if (tid == 0) s_flags = 0;
   __syncthreads();
   int64_t v[4] = {0, 0, 0, 0};          // taken by all / by those before r0; released likewise
   int flags = 0;
-  for (int b = tid; b < p.batch; b += 64 * kPlanWaves) {
-    const Request r = read_request(p, b);
-    flags |= (r.wide ? TONE_FRAMES_ROW_FULL : 0) | (r.bad ? TONE_FRAMES_BAD_REQUEST : 0);
-    v[0] += r.take;
-    v[2] += r.drop;
-    if (b < r0) {
-      v[1] += r.take;
-      v[3] += r.drop;
-    } else if (b < r1) {
-      s_take[b - r0] = r.take;
-      s_drop[b - r0] = r.drop;
-    }
+#pragma unroll 4
+  for (int b = tid; b < p.batch; b += 64 * WAVES) {
+    const Request q = read_request(p, b);
+    flags |= (q.wide ? TONE_FRAMES_ROW_FULL : 0) | (q.bad ? TONE_FRAMES_BAD_REQUEST : 0);
+    v[0] += q.take;
+    v[2] += q.drop;
+    v[1] += b < r0 ? q.take : 0;
+    v[3] += b < r0 ? q.drop : 0;
+  }
+  if (own < r1 && at == 0) {
+    s_take[mine] = r.take;
+    s_drop[mine] = r.drop;
   }
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
@@ -142,9 +153,9 @@ __global__ void __launch_bounds__(64 * kPlanWaves) plan_kernel(PlanArgs p, int p
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     v[i] = 0;
-    for (int w = 0; w < kPlanWaves; ++w) v[i] += part[w][i];
+#pragma unroll
+    for (int w = 0; w < WAVES; ++w) v[i] += part[w][i];
   }
-  const int64_t head = p.cursors_in[0], tail = p.cursors_in[1];
   // free + released <= n_pages holds for every state these calls produce; anything else is not a queue of this pool
   if (head < 0 || tail < head || tail - head + v[2] > p.n_pages) flags |= TONE_FRAMES_BAD_QUEUE;
   else if (v[0] > tail - head) flags |= TONE_FRAMES_NO_PAGES;
@@ -153,20 +164,22 @@ __global__ void __launch_bounds__(64 * kPlanWaves) plan_kernel(PlanArgs p, int p
     p.cursors_out[1] = tail + (flags ? 0 : v[2]);
     p.status[0] = flags;
   }
-  const int mine = wave / per, b = r0 + mine, at = (wave - mine * per) * 64 + (tid & 63), step = 64 * per;
-  if (b >= r1) return;
+  if (own >= r1) return;
   const int seg = (p.max_add + gridDim.y - 1) / gridDim.y, s0 = min(p.max_add, (int)blockIdx.y * seg), s1 = min(p.max_add, s0 + seg);
-  int64_t* slots = p.slots + (int64_t)b * p.max_add;
-  const int ri = p.rows_in[b], ro = p.rows_out[b];
+  int64_t* slots = p.slots + (int64_t)own * p.max_add;
   if (flags) {
     for (int j = s0 + at; j < s1; j += step) slots[j] = -1;
     if (blockIdx.y == 0 && ri >= 0 && ri < p.n_rows && ro >= 0 && ro < p.n_rows && ri != ro)
       for (int j = at; j < p.width; j += step) p.table[ro * p.stride + j] = p.table[ri * p.stride + j];
     return;
   }
-  const Request r = read_request(p, b);
   // positions in the queue, modulo n_pages once: both are below 2 n_pages, as taken <= free and free + released <= n_pages
-  int64_t take = head % p.n_pages + v[1], drop = tail % p.n_pages + v[3];
+  // (a 64-bit remainder takes a microsecond; cursors stay below 2^31 for years of 4096 streams)
+  int64_t take = head <= INT32_MAX ? (int)head - p.by_pages((uint32_t)head) * p.n_pages : head % p.n_pages;
+  int64_t drop = take + (tail - head);
+  if (drop >= p.n_pages) drop -= p.n_pages;
+  take += v[1];
+  drop += v[3];
   for (int i = 0; i < mine; ++i) {
     take += s_take[i];
     drop += s_drop[i];
@@ -275,12 +288,18 @@ hipError_t put_from(const PutArgs& a, hipStream_t st) {
 }
 
 hipError_t launch_plan(const PlanArgs& p, hipStream_t st) {
-  // a wave per request while that gives every CU a workgroup, more for fewer requests; long slot rows are cut in pieces
-  int per = 1;
-  while (per < kPlanWaves && (int64_t)p.batch * per < 16 * 256) per *= 2;
-  const int rows = kPlanWaves / per, gx = std::max(1, (p.batch + rows - 1) / rows);   // an empty batch still writes the cursors and the status
-  const int gy = std::max(1, std::min(1024 / gx, (p.max_add + 64 * per * 4 - 1) / (64 * per * 4)));
-  hipLaunchKernelGGL(plan_kernel, dim3(gx, gy), dim3(64 * kPlanWaves), 0, st, p, per);
+  // Few requests: a workgroup of four waves each.  Many: sixteen waves that share a pass over all requests, one per request
+  // once that fills the card.  Long slot rows are cut in pieces.
+  const auto go = [&](auto waves) {
+    constexpr int W = decltype(waves)::value;
+    int per = 1;
+    while (per < W && (int64_t)p.batch * per < W * 256) per *= 2;
+    const int rows = W / per, gx = std::max(1, (p.batch + rows - 1) / rows);   // an empty batch still writes the cursors and the status
+    const int gy = std::max(1, std::min(2048 / gx, (p.max_add + 64 * per * 4 - 1) / (64 * per * 4)));
+    hipLaunchKernelGGL(plan_kernel<W>, dim3(gx, gy), dim3(64 * W), 0, st, p, per);
+  };
+  if (p.batch <= 512) go(std::integral_constant<int, 4>{});
+  else go(std::integral_constant<int, 16>{});
   return hipGetLastError();
 }
 
@@ -318,7 +337,7 @@ int tone_frames_plan(int device, int32_t* table, int64_t table_stride, int n_row
   if (n_rows <= 0 || width <= 0 || n_pages <= 0 || page_size <= 0 || table_stride < width)
     return refuse(what, "rows, width, pages and page size must be positive, table_stride >= width");
   if ((int64_t)width * page_size > INT32_MAX) return refuse(what, "width x page_size exceeds 2^31 - 1 frames");
-  PlanArgs p{table, table_stride, n_rows, width, queue, n_pages, page_size, Divisor(page_size), cursors_in, cursors_out, rows_in, rows_out,
+  PlanArgs p{table, table_stride, n_rows, width, queue, n_pages, page_size, Divisor(page_size), Divisor(n_pages), cursors_in, cursors_out, rows_in, rows_out,
              first, length, keep, add, batch, slots, max_add, status};
   return launch_on(device, what, [&] { return launch_plan(p, static_cast<hipStream_t>(stream)); });
 }
