@@ -66,6 +66,13 @@ struct Shape {
   static_assert(F * kBits <= 32 && kRefresh % F == 0 && 2 * kRefresh % R == 0, "whole words and lanes");
 };
 
+// a barrier for what the waves pass on in LDS: __syncthreads would also wait for the loads and the word stores under way
+__device__ __forceinline__ void lds_barrier() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+}
+
 // lane i: lane i - 1's value (wave_shr 1); lane 0 keeps `edge`'s
 __device__ __forceinline__ int shift_in(int v, int edge) { return __builtin_amdgcn_update_dpp(edge, v, 0x138, 0xf, 0xf, false); }
 __device__ __forceinline__ float shift_in(float v, float edge) {
@@ -110,66 +117,82 @@ struct Frames {
   __device__ __forceinline__ int blank_column() const { return p.direct ? pitch() * p.blank : 0; }
 };
 
-// A loader wave: frames loader, loader + kLoaders, ... of each stage, 64 columns at a time.  What is in flight is the data of
-// the stage after the next and the rows of the one after that, so a stage waits for neither; only frames of many columns
-// have more than kBatch loads, and those behind are loaded as they are written.
+// A loader wave: frames loader, loader + kLoaders, ... of each stage, 64 columns at a time.  The data of the stage after the
+// next and the rows of the one after that are loaded a stage ahead of their use, so a stage waits for neither; only frames
+// of many columns have more than kBatch loads, and those behind are loaded as they are written.
 template <bool SUM>
 __device__ __forceinline__ void load_frames(const Frames& fr, int loader, int lane) {
   const AlignArgs& p = fr.p;
   const int n = fr.n, ahead = p.ahead, per = max(1, ahead / kLoaders), shift = 31 - __builtin_clz(per), items = (p.columns / 64 + 1) * per;
-  const bool wide = p.type == TONE_TYPE_FP32;
-  const char* x = static_cast<const char*>(p.x) + (p.rows ? 0 : (int64_t)fr.b * p.batch_stride * (wide ? 4 : 2));
+  const int type = p.type, size = type == TONE_TYPE_FP32 ? 4 : 2, pitch = fr.pitch();
+  const char* x = static_cast<const char*>(p.x) + (p.rows ? 0 : (int64_t)fr.b * p.batch_stride * size);
   const int64_t* rows = p.rows ? p.rows + (int64_t)fr.b * p.frames : nullptr;
-  int64_t row = -1, row_next = -1;               // lane f: row of frame f of a stage
-  uint32_t raw[kBatch];
-  bool have[kBatch];
+  const int64_t stride = p.stride * size, x_rows = rows ? p.x_rows : INT64_MAX;
+  int64_t row1 = -1, row2 = -1, row3 = -1;       // lane f: row of frame f, one, two and three stages on
+  uint32_t raw_a[kBatch], raw_b[kBatch];
+  bool have_a[kBatch], have_b[kBatch];
   auto frame = [&](int i) { return loader + kLoaders * (i & (per - 1)); };
-  auto load = [&](int i, uint32_t& to) -> bool {
-    const int f = frame(i), c = (i >> shift) * 64 + lane;
-    const int64_t r = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), f) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, f);
-    int label = c;
-    if (!p.direct) label = c && c < p.columns ? fr.tok[c - 1] : p.blank;
-    const bool ok = c < p.columns && label >= 0 && label < p.vocab && r >= 0 && (!rows || r < p.x_rows);
-    const int64_t off = ok ? r * p.stride + label : 0;
-    if (ok) to = wide ? *reinterpret_cast<const uint32_t*>(x + 4 * off) : *reinterpret_cast<const uint16_t*>(x + 2 * off);
-    return ok;
+  // byte offset of column c in a row; -1 where it is none
+  auto offset = [&](int c) {
+    if (c >= p.columns) return -1;
+    const int label = p.direct ? c : c ? fr.tok[c - 1] : p.blank;
+    return label >= 0 && label < p.vocab ? label * size : -1;
   };
-  auto write = [&](int stage, int i, uint32_t bits, bool ok) {
+  const int offset0 = offset(lane);
+  // the frame's row is uniform: a scalar base, and what the lane adds (columns that are none load the row's first entry)
+  auto load = [&](int64_t row, int i, int off, uint32_t& to) -> bool {
+    const int f = frame(i);
+    const int64_t r = ((int64_t)__builtin_amdgcn_readlane((int)(row >> 32), f) << 32) | (uint32_t)__builtin_amdgcn_readlane((int)row, f);
+    if (r < 0 || r >= x_rows) return false;
+    const char* base = x + r * stride;
+    const uint32_t o = max(off, 0);
+    if (size == 4) to = *reinterpret_cast<const uint32_t*>(base + o);
+    else to = *reinterpret_cast<const uint16_t*>(base + o);
+    return true;
+  };
+  auto write = [&](int stage, int i, int off, uint32_t bits, bool ok) {
     const int c = (i >> shift) * 64 + lane;
+    float v = __uint_as_float(type == TONE_TYPE_BF16 ? bits << 16 : bits);
+    if (type == TONE_TYPE_FP16) v = __half2float(__ushort_as_half((uint16_t)bits));
+    if (!(fabsf(v) < kClosed) || off < 0 || !ok) v = -INFINITY;
     if (c > p.columns) return;
-    float v = __uint_as_float(p.type == TONE_TYPE_BF16 ? bits << 16 : bits);
-    if (p.type == TONE_TYPE_FP16) v = __half2float(__ushort_as_half((uint16_t)bits));
-    if (!ok || !(fabsf(v) < kClosed)) v = -INFINITY;
-    char* to = fr.stage(stage) + c * fr.pitch() + 8 * frame(i);
+    char* to = fr.stage(stage) + c * pitch + 8 * frame(i);
     if constexpr (SUM) *reinterpret_cast<Prob*>(to) = prob_of(v);
     else *reinterpret_cast<double*>(to) = v;
   };
-  for (int t0 = -3 * ahead, stage = -3; t0 < n; t0 += ahead, ++stage) {
-    if (t0 + ahead >= 0 && t0 + ahead < n) {
-      const int m = n - (t0 + ahead);
-#pragma unroll
-      for (int j = 0; j < kBatch; ++j)
-        if (j < items && frame(j) < min(m, ahead)) write(stage + 1, j, raw[j], have[j]);
-      for (int i = kBatch; i < items; ++i)       // `row` is still that stage's
-        if (frame(i) < min(m, ahead)) {
-          uint32_t bits = 0;
-          const bool ok = load(i, bits);
-          write(stage + 1, i, bits, ok);
-        }
-    }
-    row = row_next;
+  // one stage: loads of the one after the next issued, then the next one written from the loads issued a stage ago
+  auto step = [&](int t0, int stage, uint32_t (&now)[kBatch], bool (&have)[kBatch], uint32_t (&later)[kBatch], bool (&have_later)[kBatch]) {
+    row1 = row2;
+    row2 = row3;
+    row3 = -1;
+    const int t = t0 + 3 * ahead + lane;
+    if (lane < ahead && t < n) row3 = rows ? rows[t] : t;
     if (t0 + 2 * ahead >= 0) {
-      const int m = n - (t0 + 2 * ahead);
+      const int m = min(n - (t0 + 2 * ahead), ahead);
 #pragma unroll
       for (int j = 0; j < kBatch; ++j) {
-        have[j] = false;
-        if (j < items && frame(j) < min(m, ahead)) have[j] = load(j, raw[j]);
+        have_later[j] = false;
+        if (j < items && frame(j) < m) have_later[j] = load(row2, j, j < per ? offset0 : offset((j >> shift) * 64 + lane), later[j]);
       }
     }
-    row_next = -1;
-    const int t = t0 + 3 * ahead + lane;
-    if (lane < ahead && t < n) row_next = rows ? rows[t] : t;
-    if (t0 + ahead >= 0 && t0 + ahead < n) __syncthreads();      // as the stepping waves: before stage 0, and between stages
+    if (t0 + ahead >= 0 && t0 + ahead < n) {
+      const int m = min(n - (t0 + ahead), ahead);
+#pragma unroll
+      for (int j = 0; j < kBatch; ++j)
+        if (j < items && frame(j) < m) write(stage + 1, j, j < per ? offset0 : offset((j >> shift) * 64 + lane), now[j], have[j]);
+      for (int i = kBatch; i < items; ++i)
+        if (frame(i) < m) {
+          const int off = offset((i >> shift) * 64 + lane);
+          uint32_t bits = 0;
+          const bool ok = load(row1, i, off, bits);
+          write(stage + 1, i, off, bits, ok);
+        }
+      lds_barrier();                             // as the stepping waves: before stage 0, and between stages
+    }
+  };
+  for (int t0 = -3 * ahead, stage = -3; t0 < n; t0 += 2 * ahead, stage += 2) {
+    step(t0, stage, raw_a, have_a, raw_b, have_b);
+    if (t0 + ahead < n) step(t0 + ahead, stage + 1, raw_b, have_b, raw_a, have_a);
   }
 }
 
@@ -338,7 +361,7 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, 
     return;
   }
   const int low = wave * SH::N, high = low + 64 * SH::R - 1;
-  __syncthreads();
+  lds_barrier();
   for (int t0 = 0, stage = 0; t0 < n; t0 += ahead, ++stage) {
     const bool more = t0 + ahead < n;
     const int half = ((t0 + ahead) / kRefresh) & 1;
@@ -374,7 +397,7 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, 
       }
     }
     if (now) refresh(true, half);
-    if (more) __syncthreads();
+    if (more) lds_barrier();
     if (now) refresh(false, half);
   }
 }
@@ -433,6 +456,14 @@ __device__ __forceinline__ void trace(const AlignArgs& p, int s, int t0, int t1,
   if (t == n - 1 && (path & 1)) spans[path | 1] = n;
 }
 
+// The stepping waves are 0 .. W - 1, the loaders W ...  A workgroup's waves are dealt to the CU's four SIMDs in turn, so of
+// five the first and the last share one: the single stepping wave is the second.
+template <class SH>
+__device__ __forceinline__ int role() {
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  return SH::W == 1 && wave < 2 ? 1 - wave : wave;
+}
+
 template <class SH>
 __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
   constexpr int W = SH::W, R = SH::R, HL = SH::HL, kThreads = 64 * (W + kLoaders);
@@ -440,7 +471,7 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
   __shared__ double s_end[2];
   __shared__ int s_state[kLegs];
   __shared__ double s_over[2][W][W > 1 ? HL * R : 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
+  const int lane = threadIdx.x & 63, wave = role<SH>(), base = wave * SH::N + lane * R;
   uint32_t* words = p.words + (int64_t)b * ((p.frames + SH::F - 1) / SH::F) * W * 64;
   uint16_t* came = p.came + (int64_t)b * ((p.frames + kRefresh - 1) / kRefresh) * SH::kStates;
   int32_t* labels = p.labels + (int64_t)b * p.frames;
@@ -522,7 +553,7 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
   constexpr int W = SH::W, R = SH::R, HL = SH::HL;
   __shared__ Prob s_end[2];
   __shared__ Prob s_over[2][W][W > 1 ? HL * R : 1];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), base = wave * SH::N + lane * R;
+  const int lane = threadIdx.x & 63, wave = role<SH>(), base = wave * SH::N + lane * R;
   const int32_t* tok = p.tokens + (int64_t)b * p.most;
   if (n == 0) {
     if (threadIdx.x == 0) p.total[b] = L == 0 ? 0.f : -INFINITY;
