@@ -12,7 +12,7 @@
 // of W waves, R consecutive ones per lane: a step moves one 64-bit value from lane to lane (DPP) and needs no LDS and no
 // barrier.  With W > 1 the waves' ranges overlap: a wave's first HL lanes repeat the last ones of the wave below, whose
 // values they lack go wrong by at most two states per frame from the left edge on, and are set right from that wave through
-// LDS every 32 frames.  Waves of their own stage the frames' log probabilities in LDS some frames ahead, the columns being
+// LDS every 32 frames (half of that halves the overlap, but a refresh costs half a microsecond).  Waves of their own stage the frames' log probabilities in LDS some frames ahead, the columns being
 // the vocabulary, or only the sequence's own labels where those are fewer.
 //
 // Which predecessor was taken is one bit (blank) or two (token) per state, F frames of a lane to a word of the workspace.
@@ -42,13 +42,13 @@ struct AlignArgs {
   float *score, *total;                 // total: or nullptr
   int32_t *labels, *spans;              // [batch][frames], [batch][most][2]
   uint32_t* words;                      // [batch][groups][W][64], groups of F frames
-  uint16_t* came;                       // [batch][legs][states], legs of kRefresh frames: the state at the frame before the leg
+  uint16_t* came;                       // [batch][legs][states], legs of kLeg frames: the state at the frame before the leg
   int columns, direct;                  // columns staged per frame: the labels (direct), or 0 = blank, 1 + i = token i
   int ahead;                            // frames per stage
 };
 
 constexpr float kClosed = 6e4f;         // entries of this size and more (masks of lowest values) count as -inf
-constexpr int kRefresh = 32;            // frames of a leg: between two refreshes of the waves' overlap, and two marks of the path
+constexpr int kLeg = 32;                // frames between two refreshes of the waves' overlap, and two marks of the path
 constexpr int kLoaders = 4;             // waves that stage the frames
 constexpr int kBatch = 8;               // loads a loader lane has in flight
 // exponents of probability 0: a factor of 0 takes kShut off, what passed one stays below kNone and counts as 0.  They are
@@ -58,12 +58,16 @@ constexpr int kShut = -(1 << 25), kNone = -(1 << 24), kZero = -(1 << 29);
 template <int W_, int R_>
 struct Shape {
   static constexpr int W = W_, R = R_;
-  static constexpr int HL = W > 1 ? 2 * kRefresh / R : 0;   // lanes that repeat the wave below
+  static constexpr int HL = W > 1 ? 2 * kLeg / R : 0;   // lanes that repeat the wave below
   static constexpr int N = (64 - HL) * R;                    // states a wave adds
   static constexpr int kStates = (W - 1) * N + 64 * R;
   static constexpr int kBits = R / 2 * 3;
   static constexpr int F = R == 2 ? 8 : R == 4 ? 4 : 2;      // frames per word
-  static_assert(F * kBits <= 32 && kRefresh % F == 0 && 2 * kRefresh % R == 0, "whole words and lanes");
+  static_assert(F * kBits <= 32 && kLeg % F == 0 && 2 * kLeg % R == 0, "whole words and lanes");
+  static_assert(W == 1 || N >= 2 * kLeg - 2, "a leg's path touches two waves at most");
+  // which lane holds a wave's state i < 128 R
+  __device__ static __forceinline__ int lane_of(int i) { return R == 2 ? i >> 1 : R == 4 ? i >> 2 : i >> 3; }
+  static_assert(R == 2 || R == 4 || R == 8, "lane_of");
 };
 
 // a barrier for what the waves pass on in LDS: __syncthreads would also wait for the loads and the word stores under way
@@ -187,8 +191,8 @@ __device__ __forceinline__ void load_frames(const Frames& fr, int loader, int la
           const bool ok = load(row1, i, off, bits);
           write(stage + 1, i, off, bits, ok);
         }
-      lds_barrier();                             // as the stepping waves: before stage 0, and between stages
     }
+    if (t0 + ahead >= 0 && t0 + ahead < n) lds_barrier();      // as the stepping waves: before stage 0, and between stages
   };
   for (int t0 = -3 * ahead, stage = -3; t0 < n; t0 += 2 * ahead, stage += 2) {
     step(t0, stage, raw_a, have_a, raw_b, have_b);
@@ -348,12 +352,14 @@ struct Sum {
   }
 };
 
-// Takes `st` through the frames of a sequence (n > 0).  word(g) after the last frame of every group g of F frames and after
-// the last one, refresh(write, half) every kRefresh frames.  The loader waves fill the next stage meanwhile.  A wave steps
-// only where a path can be: before frame s / 2 none has reached its first state s, and from the frame on from which its last
-// state cannot reach the end any more its values are of no use (nor are those that would be drawn from them).
-template <class SH, bool SUM, class State, class Word, class Refresh>
-__device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, int wave, int lane, Word&& word, Refresh&& refresh) {
+// Takes `st` through the frames of a sequence (n > 0): word() after the last frame of every group of F frames the wave steps
+// (skip(groups): it does not step these), leg(l) after the last frame of leg l, refresh(write, half) between two legs (W > 1).
+// The loader waves fill the next stage meanwhile.  A wave steps only where a path can be: before frame s / 2 none has reached
+// its first state s, and from the frame on from which its last state cannot reach the end any more its values are of no use
+// (nor are those that would be drawn from them).
+template <class SH, bool SUM, class State, class Word, class Skip, class Leg, class Refresh>
+__device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, int wave, int lane, Word&& word, Skip&& skip, Leg&& leg,
+                                            Refresh&& refresh) {
   constexpr int F = SH::F;
   const int n = fr.n, ahead = fr.p.ahead, blank = fr.blank_column();
   if (wave >= SH::W) {
@@ -363,21 +369,18 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, 
   const int low = wave * SH::N, high = low + 64 * SH::R - 1;
   lds_barrier();
   for (int t0 = 0, stage = 0; t0 < n; t0 += ahead, ++stage) {
-    const bool more = t0 + ahead < n;
-    const int half = ((t0 + ahead) / kRefresh) & 1;
-    const bool now = more && ((t0 + ahead) & (kRefresh - 1)) == 0;
     const int m = min(ahead, n - t0);
     if (low <= 2 * L && low <= 2 * (t0 + m) - 1 && (int64_t)high + 2 * (int64_t)(n - 1 - t0) >= 2 * L - 1) {
-      const char* frame = fr.stage(stage);
+      const char* at = fr.stage(stage);
       typename State::Rows r, next;
-      st.read(r, frame, blank);
+      st.read(r, at, blank);
       for (int f = 0; f < m; f += F) {
-        // the next two frames' entries under way (they are in the stage, also where the sequence has ended)
+        // the next two frames' entries under way (behind the sequence's or the stage's end: read and not used)
         if (t0 + f > 0 && f + F <= m) {
 #pragma unroll
           for (int i = 0; i < F; i += 2) {
-            frame += 16;
-            if (i + 2 < F || f + F < m) st.read(next, frame, blank);
+            at += 16;
+            st.read(next, at, blank);
             st.step({r, 0});
             st.step({r, 1});
             r = next;
@@ -385,20 +388,27 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, 
         } else {
 #pragma unroll 1
           for (int i = 0; i < F; i += 2) {
-            frame += 16;
-            if (f + i + 2 < m) st.read(next, frame, blank);
+            at += 16;
+            st.read(next, at, blank);
             if (t0 + f + i == 0) st.first({r, 0}, low + lane * SH::R);
             else if (f + i < m) st.step({r, 0});
             if (f + i + 1 < m) st.step({r, 1});
             r = next;
           }
         }
-        word((t0 + f) / F);
+        word();
       }
+      if (((t0 + m) & (kLeg - 1)) == 0 || t0 + m == n) leg((t0 + m - 1) / kLeg);
+    } else {
+      skip((m + F - 1) / F);
     }
-    if (now) refresh(true, half);
-    if (more) lds_barrier();
-    if (now) refresh(false, half);
+    if (t0 + m < n) {
+      const bool now = SH::W > 1 && ((t0 + m) & (kLeg - 1)) == 0;
+      const int half = ((t0 + m) / kLeg) & 1;
+      if (now) refresh(true, half);
+      lds_barrier();
+      if (now) refresh(false, half);
+    }
   }
 }
 
@@ -407,11 +417,10 @@ __device__ __forceinline__ void over_frames(const Frames& fr, State& st, int L, 
 template <class SH>
 __device__ __forceinline__ void trace(const AlignArgs& p, int s, int t0, int t1, int n, const uint32_t* words, const int32_t* tok, int32_t* labels,
                                       int32_t* spans) {
-  constexpr int W = SH::W, R = SH::R, F = SH::F, G = kRefresh / F, V = W > 1 ? 2 : 1, kLane = R == 2 ? 1 : R == 4 ? 2 : 3;
+  constexpr int W = SH::W, R = SH::R, F = SH::F, G = kLeg / F, V = W > 1 ? 2 : 1;
   constexpr int kOver = SH::HL * R;
   // steps back by the state's bits: even states (blank) bit 0; odd ones bit 2 over bit 1 (token: c1, c2): 2 if c2 else c1
   constexpr uint32_t kSteps = 0xa5a04444u;
-  static_assert(R <= 8, "kLane");
   const int lane = threadIdx.x & 63;
   int w = 0, at = s;
   while (at >= 64 * R) {
@@ -435,10 +444,11 @@ __device__ __forceinline__ void trace(const AlignArgs& p, int s, int t0, int t1,
     const int first = (g0 + i) * F;
     int drop = 0;                        // bits of the frames behind t in the word
     for (int t = min(t1, first + F - 1); t >= first; --t, drop += SH::kBits) {
-      uint32_t word = __builtin_amdgcn_readlane(words_of[i][0], (at >> kLane) & 63);
-      if (V > 1 && at >= 64 * R) word = __builtin_amdgcn_readlane(words_of[i][V - 1], (at >> kLane) & 63);
+      const int l = SH::lane_of(at), q = (at - l * R) >> 1;
+      uint32_t word = __builtin_amdgcn_readlane(words_of[i][0], l & 63);
+      if (V > 1 && at >= 64 * R) word = __builtin_amdgcn_readlane(words_of[i][V - 1], l & 63);
       path = lane == t - t0 ? s : path;
-      const uint32_t bits = (word >> (drop + 3 * ((at >> 1) & (R / 2 - 1)))) & 7;
+      const uint32_t bits = (word >> (drop + 3 * q)) & 7;
       const int how = (kSteps >> (2 * bits + 16 * (at & 1))) & 3;
       s -= how;
       at -= how;
@@ -473,7 +483,7 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
   __shared__ double s_over[2][W][W > 1 ? HL * R : 1];
   const int lane = threadIdx.x & 63, wave = role<SH>(), base = wave * SH::N + lane * R;
   uint32_t* words = p.words + (int64_t)b * ((p.frames + SH::F - 1) / SH::F) * W * 64;
-  uint16_t* came = p.came + (int64_t)b * ((p.frames + kRefresh - 1) / kRefresh) * SH::kStates;
+  uint16_t* came = p.came + (int64_t)b * ((p.frames + kLeg - 1) / kLeg) * SH::kStates;
   int32_t* labels = p.labels + (int64_t)b * p.frames;
   int32_t* spans = p.spans + (int64_t)b * p.most * 2;
   const int32_t* tok = p.tokens + (int64_t)b * p.most;
@@ -491,18 +501,19 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
     st.clear(base);
     over_frames<SH, false>(
         fr, st, L, wave, lane,
-        [&](int g) {
-          out[(int64_t)g * (W * 64)] = st.word;
+        [&] {
+          *out = st.word;
+          out += W * 64;
           st.word = 0;
-          constexpr int G = kRefresh / SH::F;
-          if ((g & (G - 1)) == G - 1 || g == (n - 1) / SH::F) {            // the end of a leg, or of the sequence
-            if (wave == 0 || lane >= HL) {
-              uint32_t* to = reinterpret_cast<uint32_t*>(came + (int64_t)(g / G) * SH::kStates + base);
+        },
+        [&](int groups) { out += groups * (W * 64); },
+        [&](int l) {
+          if (wave == 0 || lane >= HL) {
+            uint32_t* to = reinterpret_cast<uint32_t*>(came + (int64_t)l * SH::kStates + base);
 #pragma unroll
-              for (int q = 0; q < R / 2; ++q) to[q] = st.o[2 * q] | st.o[2 * q + 1] << 16;
-            }
-            st.mark(base);
+            for (int q = 0; q < R / 2; ++q) to[q] = st.o[2 * q] | st.o[2 * q + 1] << 16;
           }
+          st.mark(base);
         },
         [&](bool write, int half) {
           if constexpr (W > 1) {
@@ -533,7 +544,7 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
   if (threadIdx.x == 0) p.score[b] = (float)score;
   if (!alive || n == 0) return;
   int s = at_token > at_blank ? 2 * L - 1 : 2 * L;
-  for (int leg = (n - 1) / kRefresh; leg >= 0; leg -= kLegs) {              // s: the state at the end of `leg`
+  for (int leg = (n - 1) / kLeg; leg >= 0; leg -= kLegs) {              // s: the state at the end of `leg`
     const int low = max(0, leg - kLegs + 1);
     if (wave == 0) {
       for (int k = leg; k >= low; --k) {
@@ -543,7 +554,7 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
     }
     __syncthreads();
     for (int k = leg - wave; k >= low; k -= W + kLoaders)
-      trace<SH>(p, __builtin_amdgcn_readfirstlane(s_state[leg - k]), k * kRefresh, min(n, (k + 1) * kRefresh) - 1, n, words, tok, labels, spans);
+      trace<SH>(p, __builtin_amdgcn_readfirstlane(s_state[leg - k]), k * kLeg, min(n, (k + 1) * kLeg) - 1, n, words, tok, labels, spans);
     __syncthreads();
   }
 }
@@ -571,9 +582,7 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
   st.clear();
   over_frames<SH, true>(
       fr, st, L, wave, lane,
-      [&](int g) {
-        if ((g & (kRefresh / SH::F - 1)) == kRefresh / SH::F - 1) st.renormalize();
-      },
+      [] {}, [](int) {}, [&](int) { st.renormalize(); },
       [&](bool write, int half) {
         if constexpr (W > 1) {
           if (write) {
@@ -620,14 +629,16 @@ template <int W, int R>
 hipError_t launch_as(AlignArgs p, hipStream_t st) {
   p.direct = p.vocab <= p.most + 1;
   p.columns = p.direct ? p.vocab : p.most + 1;
-  // frames per stage: a divisor of the refresh interval, two stages beside the rest of the LDS
-  p.ahead = kRefresh;
-  while (p.ahead > 2 && 16 * (p.ahead + 2) * (p.columns + 1) > 128 * 1024) p.ahead /= 2;
-  static_assert(16 * (2 + 2) * (TONE_ALIGN_MAX_TOKENS + 2) <= 128 * 1024, "two frames of the longest sequences fit");
+  // frames per stage: a leg, or a divisor of it that leaves room for two stages beside the rest of the LDS (never fewer than a
+  // word has)
+  p.ahead = kLeg;
+  constexpr int kLds = 128 * 1024;
+  while (p.ahead > 2 && 16 * (p.ahead + 2) * (p.columns + 1) > kLds) p.ahead /= 2;
+  static_assert(16 * (2 + 2) * (TONE_ALIGN_MAX_TOKENS + 2) <= kLds, "two frames of the longest sequences fit");
   const size_t lds = (size_t)16 * (p.ahead + 2) * (p.columns + 1);
   auto* fn = align_kernel<W, R>;
-  if (lds > 32 * 1024) {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (lds > 32 * 1024) {                 // the same limit whoever calls: calls on several threads do not undo each other's
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (e != hipSuccess) return e;
   }
   hipLaunchKernelGGL(fn, dim3(p.total ? 2 * p.batch : p.batch), dim3(64 * (W + kLoaders)), lds, st, p);
@@ -657,7 +668,7 @@ struct Workspace {
 Workspace align_workspace(int batch, int frames, int most) {
   return by_tokens(most, [&](auto sh) -> Workspace {
     using SH = decltype(sh);
-    return {(int64_t)batch * ((frames + SH::F - 1) / SH::F) * SH::W * 64 * 4, (int64_t)batch * ((frames + kRefresh - 1) / kRefresh) * SH::kStates * 2};
+    return {(int64_t)batch * ((frames + SH::F - 1) / SH::F) * SH::W * 64 * 4, (int64_t)batch * ((frames + kLeg - 1) / kLeg) * SH::kStates * 2};
   });
 }
 
