@@ -275,13 +275,13 @@ struct Part {
   Best best;
   int* shared;                           // the largest floor of the row's waves, as order_of
 
-  // x[q][j]: entry base + q * span + lane * N + j; those of lanes from valid[q] on are none (-inf)
-  template <int Q, int N>
+  // x[q][j]: entry base + (64 q + lane) N + j; those of lanes from valid[q] on are none (-inf).  ALL: there are no such lanes
+  template <bool ALL, int Q, int N>
   __device__ __forceinline__ void batch(const float (&x)[Q][N], int base, const int (&valid)[Q], int lane, int k, float xt, int t) {
     float top[Q], most;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {        // steps of which no lane has an entry are left out here and below
-      if (q && valid[q] <= 0) continue;
+      if (!ALL && q && valid[q] <= 0) continue;
       top[q] = x[q][0];
 #pragma unroll
       for (int j = 1; j < N; ++j) top[q] = fmaxf(top[q], x[q][j]);
@@ -289,11 +289,11 @@ struct Part {
     }
     const float other = shared ? value_of(*static_cast<volatile int*>(shared)) : -INFINITY;
     if ((!full || __ballot(most > floor)) && (k == 0 || __ballot(most >= other)))
-      news<Q, N>(x, top, most, other, base, valid, lane, k);
+      news<ALL, Q, N>(x, top, most, other, base, valid, lane, k);
     else if (__ballot(most > m)) larger(most);
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
-      if (q && valid[q] <= 0) continue;
+      if (!ALL && q && valid[q] <= 0) continue;
 #pragma unroll
       for (int j = 0; j < N; ++j) {
         const float z = x[q][j] - m, e = exp_neg(z);
@@ -305,17 +305,17 @@ struct Part {
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int b = base + q * 64 * N;
-      if (t < 0 || (q && valid[q] <= 0)) continue;
+      if (t < 0 || (!ALL && q && valid[q] <= 0)) continue;
       if (t >= b + 64 * N) {
 #pragma unroll
-        for (int j = 0; j < N; ++j) above += __builtin_popcountll(__ballot(x[q][j] >= xt && lane < valid[q]));
+        for (int j = 0; j < N; ++j) above += __builtin_popcountll(__ballot(x[q][j] >= xt && (ALL || lane < valid[q])));
       } else if (t < b) {
 #pragma unroll
         for (int j = 0; j < N; ++j) above += __builtin_popcountll(__ballot(x[q][j] > xt));
       } else {
 #pragma unroll
         for (int j = 0; j < N; ++j)
-          above += __builtin_popcountll(__ballot(lane < valid[q] && (x[q][j] > xt || (x[q][j] == xt && b + lane * N + j < t))));
+          above += __builtin_popcountll(__ballot((ALL || lane < valid[q]) && (x[q][j] > xt || (x[q][j] == xt && b + lane * N + j < t))));
       }
     }
   }
@@ -331,7 +331,7 @@ struct Part {
     }
   }
 
-  template <int Q, int N>
+  template <bool ALL, int Q, int N>
   __device__ __forceinline__ void news(const float (&x)[Q][N], const float (&top)[Q], float most, float other, int base, const int (&valid)[Q], int lane,
                                        int k) {
     larger(most);
@@ -347,7 +347,7 @@ struct Part {
       float largest = x[0][0];
 #pragma unroll
       for (int q = Q - 1; q >= 0; --q) {
-        if (q && valid[q] <= 0) continue;
+        if (!ALL && q && valid[q] <= 0) continue;
 #pragma unroll
         for (int j = N - 1; j >= 0; --j)
           if (x[q][j] == most) {
@@ -355,17 +355,17 @@ struct Part {
             largest = most;
           }
       }
-      best.sort(lane < valid[0] ? key_of(largest, base + (best_at / N * 64 + lane) * N + best_at % N) : 0, lane, k);
+      best.sort(ALL || lane < valid[0] ? key_of(largest, base + (best_at / N * 64 + lane) * N + best_at % N) : 0, lane, k);
     }
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       // nothing below another wave's floor can be among the row's k best; what equals it can, by its index
       const float low = fmaxf(best.floor ? key_value(best.floor) : -INFINITY, other);
-      if ((q && valid[q] <= 0) || (best.floor && __ballot(top[q] >= low) == 0)) continue;      // (a NaN is above no floor, but fills a list)
+      if ((!ALL && q && valid[q] <= 0) || (best.floor && __ballot(top[q] >= low) == 0)) continue;      // (a NaN is above no floor, but fills a list)
 #pragma unroll
       for (int j = 0; j < N; ++j)
         if (!best.floor || __ballot(x[q][j] >= low))
-          best.take(lane < valid[q] && q * N + j != best_at ? key_of(x[q][j], base + (q * 64 + lane) * N + j) : 0, lane, k);
+          best.take((ALL || lane < valid[q]) && q * N + j != best_at ? key_of(x[q][j], base + (q * 64 + lane) * N + j) : 0, lane, k);
     }
     full = best.floor != 0;
     if (full) {
@@ -421,26 +421,34 @@ __global__ void __launch_bounds__(64 * W * ROWS) scores_long_kernel(ScoreArgs p)
   for (int c = v0; c < v1; c += 64 * Q) {
     float f[Q][N];
     int valid[Q];
+    if (c + 64 * Q <= v1) {
 #pragma unroll
-    for (int q = 0; q < Q; ++q) {
-      valid[q] = v1 - (c + 64 * q);
+      for (int q = 0; q < Q; ++q)
 #pragma unroll
-      for (int j = 0; j < N; ++j) f[q][j] = lane < valid[q] ? load_elem(&v[q].e[j]) : -INFINITY;
+        for (int j = 0; j < N; ++j) f[q][j] = load_elem(&v[q].e[j]);
+      load(c + 64 * Q);
+      a.batch<true, Q, N>(f, head + c * N, valid, lane, p.k, xt, t);
+    } else {
+#pragma unroll
+      for (int q = 0; q < Q; ++q) {
+        valid[q] = v1 - (c + 64 * q);
+#pragma unroll
+        for (int j = 0; j < N; ++j) f[q][j] = lane < valid[q] ? load_elem(&v[q].e[j]) : -INFINITY;
+      }
+      a.batch<false, Q, N>(f, head + c * N, valid, lane, p.k, xt, t);
     }
-    load(c + 64 * Q);
-    a.batch<Q, N>(f, head + c * N, valid, lane, p.k, xt, t);
   }
   const int tail = head + vecs * N;
   if (wr == W - 1 && tail < p.vocab) {
     const int valid[1] = {p.vocab - tail};
     const float one[1][1] = {{lane < valid[0] ? load_elem(x + tail + lane) : -INFINITY}};
-    a.batch<1, 1>(one, tail, valid, lane, p.k, xt, t);
+    a.batch<false, 1, 1>(one, tail, valid, lane, p.k, xt, t);
   }
   if (wr == 0 && head) {
     const int valid[1] = {head};
     const float one[1][1] = {{lane < head ? load_elem(x + lane) : -INFINITY}};
     a.full = false;                      // lower indices than what is held: equal values have to be looked at
-    a.batch<1, 1>(one, 0, valid, lane, p.k, xt, t);
+    a.batch<false, 1, 1>(one, 0, valid, lane, p.k, xt, t);
   }
   a.s = over_wave(a.s, [](float p_, float q_) { return p_ + q_; });
   a.u = over_wave(a.u, [](float p_, float q_) { return p_ + q_; });
