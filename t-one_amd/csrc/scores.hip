@@ -521,13 +521,14 @@ hipError_t launch_as(const ScoreArgs& p, hipStream_t st) {
     }
     return hipGetLastError();
   }
-  // Waves per row, by the 64-lane loads it takes (measured, us, k = 10, with 1 / 4 / 16 waves): few rows are a matter of one
-  // row's time (bf16 65,537: 1 row 79 / 31 / 19, 256 rows 93 / 35 / 22, 400 rows 92 / 40 / 40; 5000: 256 rows 17 / 10 / 11), and
-  // from some 2000 rows on the card is full with one wave each (bf16 5000: 1024 rows 17 / 13 / 34, 2048 19 / 20 / 63, 16,384
-  // 73 / 116 / 462; 32,000: 2048 rows 63 / 58 / 92, 4096 87 / 98 / 177; 1000: 1024 rows 8 / 10 / 41).
+  // Waves per row, by the 64-lane loads it takes (us, k = 10, with 1 / 4 / 16 waves).  Few rows are a matter of one row's time
+  // (bf16 65,537: 1 row 79 / 31 / 19, 256 rows 93 / 35 / 22, 400 rows 92 / 40 / 40; 5000: 256 rows 17 / 10 / 11), and from some
+  // 1500 rows on the card is full with one wave each, which sorts once per row instead of four times (bf16 65,537: 1024 rows
+  // 77 / 51, 2048 88 / 90; 32,000: 1500 rows 54 / 47, 2600 64 / 73, 4096 77 / 102; 5000: 1024 rows 16 / 13, 2048 17 / 21,
+  // 16,384 73 / 116; 2500: 600 rows 11 / 11, 2048 13 / 19).
   const int64_t steps = (p.vocab / Vec<T>::N + 63) / 64;
   if (steps >= 20 && p.n <= 256) hipLaunchKernelGGL((scores_long_kernel<T, 16, 1>), dim3((unsigned)p.n), dim3(1024), 0, st, p);
-  else if (steps >= 4 && p.n <= (steps >= 32 ? 2048 : 1536))
+  else if (steps >= 4 && p.n <= (steps >= 16 ? 1536 : 1024))
     hipLaunchKernelGGL((scores_long_kernel<T, 4, 1>), dim3((unsigned)p.n), dim3(256), 0, st, p);
   else hipLaunchKernelGGL((scores_long_kernel<T, 1, 4>), dim3((unsigned)((p.n + 3) / 4)), dim3(256), 0, st, p);
   return hipGetLastError();
