@@ -257,7 +257,9 @@ struct Best {
       int o_token, o_blank;
       uint64_t c0, c1, c2;
       // one by hand: (a) v_max_f64 without the quieting of operands that fmax brings, (b) each compare's mask pushed into
-      // the word by one add with carry, two instructions at least behind the compare as gfx950 demands of masks
+      // the word by one add with carry, two instructions at least behind the compare as gfx950 demands of masks.  What a
+      // DPP move reads next (o_token) is written three instructions before the end: two are demanded, and the compiler
+      // does not look inside
       asm("v_cmp_gt_f64_e64 %[c1], %[one], %[stay]\n\t"
           "v_cmp_gt_f64_e64 %[c0], %[from], %[one]\n\t"
           "v_max_f64 %[m], %[stay], %[one]\n\t"
@@ -266,10 +268,10 @@ struct Best {
           "v_max_f64 %[token], %[m], %[two]\n\t"
           "v_cndmask_b32_e64 %[o_token], %[o_stay], %[o_one], %[c1]\n\t"
           "v_cndmask_b32_e64 %[o_blank], %[o_one], %[o_from], %[c0]\n\t"
+          "v_cndmask_b32_e64 %[o_token], %[o_token], %[o_from], %[c2]\n\t"
           "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c1]\n\t"
           "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c2]\n\t"
-          "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c0]\n\t"
-          "v_cndmask_b32_e64 %[o_token], %[o_token], %[o_from], %[c2]"
+          "v_addc_co_u32_e64 %[word], vcc, %[word], %[word], %[c0]"
           : [o_token] "=&v"(o_token), [o_blank] "=&v"(o_blank), [word] "+v"(word), [m] "=&v"(m), [blank] "=&v"(blank), [token] "=&v"(token), [c0] "=&s"(c0), [c1] "=&s"(c1), [c2] "=&s"(c2)
           : [o_stay] "v"(o[2 * q + 1]), [o_one] "v"(o[2 * q]), [o_from] "v"(o_from), [stay] "v"(stay), [one] "v"(one), [two] "v"(two), [from] "v"(from)
           : "vcc");
