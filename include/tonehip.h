@@ -187,7 +187,7 @@ int tone_session_debug_read(tone_session *s, const char *buffer, void *host_dst,
  *                                              (`width` entries, -1 behind the last page): ping-pong rows as
  *                                              tone_session_run_rows, all named rows distinct
  *   queue        int32 [n_pages]               free pages at [head, tail) modulo n_pages
- *   cursors_in / _out  int64 [2]               head, tail before / after (distinct buffers)
+ *   cursors_in / _out  int64 [2]               head, tail before / after (they must not overlap)
  *   first, length, keep, add  int32 [batch]
  *   slots        int64 [batch][max_add]        page * page_size + offset of new frame length + j; -1 for j >= add and for
  *                                              frames before keep

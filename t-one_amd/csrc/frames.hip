@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(64 * WAVES) plan_kernel(PlanArgs p, int per) {
     for (int w = 0; w < WAVES; ++w) v[i] += part[w][i];
   }
   // free + released <= n_pages holds for every state these calls produce; anything else is not a queue of this pool
-  if (head < 0 || tail < head || tail - head + v[2] > p.n_pages) flags |= TONE_FRAMES_BAD_QUEUE;
+  // (tail - head by itself first: cursors near 2^63 would pass the sum's end)
+  if (head < 0 || tail < head || tail - head > p.n_pages || tail - head + v[2] > p.n_pages) flags |= TONE_FRAMES_BAD_QUEUE;
   else if (v[0] > tail - head) flags |= TONE_FRAMES_NO_PAGES;
   if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) {
     p.cursors_out[0] = head + (flags ? 0 : v[0]);
@@ -333,7 +334,7 @@ int tone_frames_plan(int device, int32_t* table, int64_t table_stride, int n_row
   if (!table || !queue || !cursors_in || !cursors_out || !status) return refuse(what, "null table, queue, cursors or status");
   if (batch && (!rows_in || !rows_out || !first || !length || !keep || !add || (max_add && !slots)))
     return refuse(what, "null request array or slots");
-  if (cursors_in == cursors_out) return refuse(what, "cursors_out must differ from cursors_in");
+  if (cursors_in < cursors_out + 2 && cursors_out < cursors_in + 2) return refuse(what, "cursors_out overlaps cursors_in");
   if (n_rows <= 0 || width <= 0 || n_pages <= 0 || page_size <= 0 || table_stride < width)
     return refuse(what, "rows, width, pages and page size must be positive, table_stride >= width");
   if ((int64_t)width * page_size > INT32_MAX) return refuse(what, "width x page_size exceeds 2^31 - 1 frames");

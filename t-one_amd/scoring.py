@@ -135,7 +135,7 @@ def frames_plan(table, queue, cursors_in, cursors_out, rows_in, rows_out, first,
         raise ValueError(f"slots must be a contiguous ({b}, {max_add}) int64 tensor")
     if status is not None:
         _vector(status, "status", torch.int32, 1)
-    if cursors_in.data_ptr() == cursors_out.data_ptr():
+    if abs(cursors_in.data_ptr() - cursors_out.data_ptr()) < 16:
         raise ValueError("cursors_out must not alias cursors_in")
     ins = (table, queue, cursors_in, cursors_out, rows_in, rows_out, first, length, keep, add, slots, status)
     dev = _device(*ins)

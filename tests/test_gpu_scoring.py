@@ -132,6 +132,21 @@ def test_plan_refused_on_the_device_changes_nothing(what, bit):
             assert torch.equal(t[int(rows_out[b])], before[0][int(rows_in[b])])
 
 
+@pytest.mark.parametrize("cursors", [(0, 2 ** 63 - 1), (2 ** 62, 2 ** 63 - 1), (3, 2 ** 63 - 2), (-1, 5), (-2 ** 63, 2 ** 63 - 1), (0, 41)])
+def test_plan_of_cursors_of_any_size(cursors):
+    """Cursors that describe no queue, their difference plus the released pages beyond 63 bits among them."""
+    p = Pool(np.random.default_rng(2), 4, 4, 5, 40)
+    p.step([0, 1, 2, 3], [0, 0, 0, 0], [6, 9, 1, 4], 12)
+    t, q, _, cout = p.dev
+    cin = _dev(np.array(cursors))
+    queue = q.clone()
+    rows = (2 * np.arange(4) + p.par, 2 * np.arange(4) + 1 - p.par)
+    slots, status = S().frames_plan(t, q, cin, cout, *(_dev(v, np.int32) for v in (*rows, p.first, p.length, p.length, np.zeros(4))),
+                                    page_size=4, max_add=12)
+    assert int(status) == 8 and bool((slots == -1).all())
+    assert torch.equal(cout, cin) and torch.equal(q, queue)
+
+
 def test_plan_near_the_largest_frame_numbers():
     """Frame numbers up to 2^31 - 1 (a stream that never closes) do not wrap."""
     p = Pool(np.random.default_rng(2), 2, 64, 6, 30)

@@ -181,6 +181,12 @@ def test_c_frames_plan_refuses():
     _refused(call(page=1 << 30), "2^31")
 
 
+def test_c_frames_plan_refuses_overlapping_cursors():
+    at = [ctypes.c_void_p(4096 + 8 * i) for i in range(5)]
+    for i, j in ((2, 1), (2, 2), (2, 3)):
+        _refused(_lib.load().tone_frames_plan(0, P, 3, 4, 3, P, 8, 4, at[i], at[j], P, P, P, P, P, P, 2, P, 2, P, None), "cursors_out")
+
+
 def test_c_frames_slots_and_put_refuse():
     lib = _lib.load()
     _refused(lib.tone_frames_slots(0, P, 3, 4, 3, 8, 4, None, P, P, P, 1, P, 2, None), "null")
