@@ -682,7 +682,7 @@ using namespace tone;
 extern "C" {
 
 int64_t tone_ctc_align_workspace(int batch, int frames, int tokens) {
-  if (batch < 0 || frames < 0 || tokens < 0 || tokens > TONE_ALIGN_MAX_TOKENS) return -1;
+  if (batch < 0 || frames < 0 || frames > kMaxFrames || tokens < 0 || tokens > TONE_ALIGN_MAX_TOKENS) return -1;
   const Workspace w = align_workspace(batch, frames, tokens);
   return w.words + w.came;
 }
@@ -694,6 +694,7 @@ int tone_ctc_align(int device, const void* x, int type, int64_t stride, int64_t 
   const char* what = "tone_ctc_align";
   if (batch < 0 || frames < 0 || x_rows < 0 || vocab <= 0 || vocab > (1 << 24))
     return refuse(what, "batch, frames, x_rows or vocab out of range");
+  if (frames > kMaxFrames || batch > kMaxThreads / (2 * 64 * (8 + kLoaders))) return refuse(what, "batch or frames too large for one launch");
   if (max_tokens < 0 || max_tokens > TONE_ALIGN_MAX_TOKENS) return refuse(what, "max_tokens must be in 0 .. TONE_ALIGN_MAX_TOKENS");
   if (!known_type(type)) return refuse(what, "unknown element type");
   if (blank < 0 || blank >= vocab) return refuse(what, "blank outside the vocabulary");

@@ -331,6 +331,7 @@ int tone_frames_plan(int device, int32_t* table, int64_t table_stride, int n_row
                      const int32_t* add, int batch, int64_t* slots, int max_add, int32_t* status, void* stream) {
   const char* what = "tone_frames_plan";
   if (batch < 0 || max_add < 0) return refuse(what, "negative batch or max_add");
+  if (max_add > kMaxFrames || batch > kMaxThreads / 128) return refuse(what, "batch or max_add too large for one launch");
   if (!table || !queue || !cursors_in || !cursors_out || !status) return refuse(what, "null table, queue, cursors or status");
   if (batch && (!rows_in || !rows_out || !first || !length || !keep || !add || (max_add && !slots)))
     return refuse(what, "null request array or slots");
@@ -352,7 +353,7 @@ int tone_frames_slots(int device, const int32_t* table, int64_t table_stride, in
   if (!table || !rows || !first || !begin || !count || !slots) return refuse(what, "null pointer");
   if (n_rows <= 0 || width <= 0 || n_pages <= 0 || page_size <= 0 || table_stride < width)
     return refuse(what, "rows, width, pages and page size must be positive, table_stride >= width");
-  if (((int64_t)max_count + 255) / 256 * batch > INT32_MAX) return refuse(what, "batch x max_count too large for one launch");
+  if (max_count > kMaxFrames || ((int64_t)max_count + 255) / 256 * batch > kMaxThreads / 256) return refuse(what, "batch x max_count too large for one launch");
   SlotArgs p{table, table_stride, n_rows, width, n_pages, page_size, Divisor(page_size), rows, first, begin, count, batch, slots, max_count};
   return launch_on(device, what, [&] { return launch_slots(p, static_cast<hipStream_t>(stream)); });
 }
@@ -366,7 +367,7 @@ int tone_frames_put(int device, const void* src, int src_type, int64_t src_strid
   if (!src || !slots || (!pool && pool_rows)) return refuse(what, "null pointer");
   if (src_stride < vocab || pool_stride < vocab) return refuse(what, "row stride < vocab");
   if (!aligned(src, src_type) || !aligned(pool, pool_type)) return refuse(what, "src or pool not aligned to its element type");
-  if (n > ((int64_t)INT32_MAX << 8) / vocab) return refuse(what, "too many rows for one launch");
+  if (n > (kMaxThreads / 256 - 1) * kPutChunk / vocab) return refuse(what, "too many rows for one launch");
   PutArgs p{src, src_type, src_stride, slots, n, vocab, pool, pool_type, pool_stride, pool_rows};
   return launch_on(device, what, [&] { return launch_put(p, static_cast<hipStream_t>(stream)); });
 }

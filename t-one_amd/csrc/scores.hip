@@ -562,7 +562,7 @@ int tone_token_scores(int device, const void* x, int type, int64_t stride, int64
   if (!rows && x_rows < n) return refuse(what, "fewer rows in x than outputs");
   if (stride < vocab && x_rows > 1) return refuse(what, "row stride < vocab");
   if (!aligned(x, type)) return refuse(what, "x not aligned to its element type");
-  if (n > INT32_MAX) return refuse(what, "too many rows for one launch");
+  if (n > kMaxThreads / (vocab <= 64 ? 8 : 64) - 32) return refuse(what, "too many rows for one launch");
   ScoreArgs p{x, stride, x_rows, rows, n, vocab, k, tokens, tokens ? logprob : nullptr, entropy, tokens ? rank : nullptr,
               top_logprob, top_ids};
   return launch_on(device, what, [&] { return launch_scores(p, type, static_cast<hipStream_t>(stream)); });

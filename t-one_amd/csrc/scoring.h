@@ -28,6 +28,10 @@ __device__ __forceinline__ void store_elem(Bf16* p, float v) { *p = static_cast<
 
 inline bool known_type(int t) { return t == TONE_TYPE_FP32 || t == TONE_TYPE_FP16 || t == TONE_TYPE_BF16; }
 
+// A launch's threads are counted in 32 bits, and loops over a row's frames run in 32-bit integers with room for a stride.
+constexpr int64_t kMaxThreads = UINT32_MAX;
+constexpr int kMaxFrames = 1 << 29;
+
 // whether a pointer lies on a whole element of its type
 inline bool aligned(const void* p, int type) { return (reinterpret_cast<uintptr_t>(p) & (type == TONE_TYPE_FP32 ? 3 : 1)) == 0; }
 

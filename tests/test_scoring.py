@@ -241,6 +241,22 @@ def test_c_ctc_align_refuses():
     assert lib.tone_ctc_align_workspace(2, 6, S.MAX_TOKENS + 1) == -1
 
 
+def test_c_sizes_past_one_launch_are_refused():
+    """Sizes whose counts of threads pass 32 bits, or whose frame loops pass 31."""
+    lib = _lib.load()
+    big = 1 << 30
+    _refused(lib.tone_frames_plan(0, P, 3, 4, 3, P, 8, 4, P, Q, P, P, P, P, P, P, 2, P, big, P, None), "one launch")
+    _refused(lib.tone_frames_plan(0, P, 3, 4, 3, P, 8, 4, P, Q, P, P, P, P, P, P, 1 << 26, P, 2, P, None), "one launch")
+    _refused(lib.tone_frames_slots(0, P, 3, 4, 3, 8, 4, P, P, P, P, 1, P, big, None), "one launch")
+    _refused(lib.tone_frames_slots(0, P, 3, 4, 3, 8, 4, P, P, P, P, 1 << 24, P, 1, None), "one launch")
+    _refused(lib.tone_frames_put(0, P, 0, 64, P, 1 << 29, 64, P, 0, 64, 9, None), "one launch")
+    for vocab, n in ((35, 1 << 29), (64, 1 << 29), (65, 1 << 26)):
+        _refused(lib.tone_token_scores(0, P, 0, vocab, n, None, n, vocab, None, 0, None, P, None, None, None, None), "one launch")
+    for batch, frames in ((1, big), (1 << 22, 4)):
+        _refused(lib.tone_ctc_align(0, P, 0, 5, 30, 0, None, batch, frames, 5, 4, P, 3, P, P, P, None, P, P, P, 1 << 60, None), "one launch")
+    assert lib.tone_ctc_align_workspace(1, big, 3) == -1 < lib.tone_ctc_align_workspace(1, 1 << 29, 3)
+
+
 def test_c_empty_calls_do_nothing():
     lib = _lib.load()
     assert lib.tone_frames_slots(0, None, 3, 4, 3, 8, 4, None, None, None, None, 0, None, 2, None) == 0
