@@ -29,10 +29,11 @@ constexpr float kLog2e = 1.4426950408889634f;
 // e^z for z <= 0 (v_exp_f32; z log2 e is rounded once, so e^z is off by about |z| 2^-24 of its value)
 __device__ __forceinline__ float exp_neg(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 
-// total order of the values as integers: larger value = larger integer, -0 and +0 are one value, never INT_MIN
+// total order of the values as integers: larger value = larger integer, -0 and +0 are one value, never INT_MIN or INT_MAX
+// (1 can be added; the ends are NaN)
 __device__ __forceinline__ int order_of(float v) {
   const int b = __float_as_int(v + 0.0f);
-  return max(b < 0 ? b ^ 0x7fffffff : b, -0x7fffffff);
+  return min(max(b < 0 ? b ^ 0x7fffffff : b, -0x7fffffff), 0x7ffffffe);
 }
 // larger value = larger key; equal values: the lower index has the larger key.  Never 0.
 __device__ __forceinline__ uint64_t key_of(float v, int i) {

@@ -343,6 +343,21 @@ def test_scores_through_a_slot_map(v):
     assert torch.equal(flat.entropy, r.entropy.view(-1))
 
 
+@pytest.mark.parametrize("v", [7, 35, 64, 65, 700])
+def test_scores_of_nan_of_any_bits(v):
+    """NaN with every bit set, of both signs, more than once in a row: ids stay distinct and in range, ranks in range."""
+    bits = np.random.default_rng(v).standard_normal((40, v)).astype(np.float32).view(np.uint32)
+    for i in range(40):
+        at = np.random.default_rng(i).permutation(v)[: 1 + i % min(v, 9)]
+        bits[i, at] = [0x7FFFFFFF, 0xFFFFFFFF, 0x7F800001, 0x7FC00000][i % 4]
+    x = _dev(bits.view(np.int32), np.int32).view(torch.float32)
+    tokens = _dev(np.arange(40) % v, np.int32)
+    r = S().token_scores(x, tokens, k=min(v, 64))
+    ids, rank = r.top_ids.cpu().numpy(), r.rank.cpu().numpy()
+    assert ((ids >= 0) & (ids < v)).all() and all(len(set(row)) == len(row) for row in ids.tolist())
+    assert ((rank >= 0) & (rank < v)).all()
+
+
 def test_scores_of_no_rows():
     r = S().token_scores(torch.empty((0, 35), device="cuda"), torch.empty(0, dtype=torch.int32, device="cuda"), k=3)
     assert tuple(r.top_ids.shape) == (0, 3) and r.entropy.numel() == 0
