@@ -11,11 +11,12 @@ those rows where they are, on the device, until the phrase they belong to has en
 The functions are stateless (``include/tonehip.h`` has the exact definitions): they check types, shapes, strides and devices
 here, write new tensors (or the caller's buffers, where they are arguments), do not synchronize, and run on ``stream`` or the
 current stream of the tensors' device.  Contents are checked on the device: an index outside its range is left out or counts as
-"none", as documented per argument.  Every call can be captured into a graph.
+"none", as documented per argument.  Every one can be captured into a graph.  No gradient flows through them.
 """
 
 from __future__ import annotations
 
+import contextlib
 from typing import NamedTuple, Optional
 
 import numpy as np
@@ -335,10 +336,11 @@ class FrameStore:
     """The latest rows of many streams, in pages of one pool on the device.
 
     Stream i holds its frames [first, length), counted from its start.  :meth:`append` adds a step's rows for any subset of
-    the streams (:meth:`reserve`: only their slots) and lets go of the frames before ``keep``; :meth:`slots` gives the pool rows of a range of frames, for
-    ``token_scores`` / ``ctc_align`` with ``rows=``.  Page tables, slot maps and the free list live on the device; the host
-    keeps the counts, so a call that would run out of pages raises before anything has changed.  The calls on one store
-    belong on one stream (or ordered by events); the pool and the tables are the store's own."""
+    the streams (:meth:`reserve`: only their slots) and lets go of the frames before ``keep``; :meth:`slots` gives the pool rows
+    of a range of frames, for ``token_scores`` / ``ctc_align`` with ``rows=``.  Page tables, slot maps and the free list live on
+    the device; the host keeps the counts, so a call that would run out of pages raises before anything has changed.  The
+    calls on one store belong on one stream (or ordered by events) and, as the counts are the host's, not into a graph; the
+    pool and the tables are the store's own."""
 
     def __init__(self, n_streams: int, max_frames: int, *, page_size: int = 64, n_pages: Optional[int] = None, vocab: int = C.VOCAB,
                  dtype=None, device: int = 0):
@@ -362,11 +364,29 @@ class FrameStore:
         self._table = torch.full((2 * self.n_streams, self.width), -1, dtype=torch.int32, device=self.dev)
         self._queue = torch.arange(self.n_pages, dtype=torch.int32, device=self.dev)
         self._cursors = torch.tensor([[0, self.n_pages], [0, 0]], dtype=torch.int64, device=self.dev)
+        self._home = torch.cuda.current_stream(self.dev)                 # what the allocator knows the buffers by
         self._side = 0                                                   # which cursors are current
         self.first = np.zeros(self.n_streams, np.int64)
         self.length = np.zeros(self.n_streams, np.int64)
         self._parity = np.zeros(self.n_streams, np.int64)
         self.free_pages = self.n_pages
+        torch.cuda.current_stream(self.dev).synchronize()                # the buffers are as they should be, for any stream
+
+    @contextlib.contextmanager
+    def _use(self, stream):
+        """The call's stream as the current one; the buffers are marked as in use on it, so that the store may be dropped while
+        its calls are under way."""
+        torch = _torch()
+        if stream is not None and stream.device != self.dev:
+            raise ValueError(f"stream on {stream.device}, the store on {self.dev}")
+        with (torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.dev)):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("the calls of a FrameStore cannot be captured into a graph: their counts are the host's")
+            now = torch.cuda.current_stream(self.dev)
+            if now != self._home:
+                for t in (self.pool, self._table, self._queue, self._cursors):
+                    t.record_stream(now)
+            yield
 
     def _ids(self, ids) -> np.ndarray:
         ids = np.asarray(ids, np.int64).reshape(-1)
@@ -419,7 +439,7 @@ class FrameStore:
         keep = self.first[ids] if keep is None else np.asarray(keep, np.int64).reshape(-1)
         if add.shape != ids.shape or keep.shape != ids.shape or (add < 0).any() or (add > frames).any():
             raise ValueError(f"counts must be {ids.size} numbers in 0 .. {frames}, keep {ids.size} frame numbers")
-        with (torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.dev)):
+        with self._use(stream):
             return self._plan(ids, keep, add, frames)
 
     def append(self, rows, ids, keep=None, counts=None, stream=None):
@@ -442,7 +462,7 @@ class FrameStore:
         ids = self._ids(ids)
         if ids.size == 0:
             return
-        with (torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.dev)):
+        with self._use(stream):
             self._plan(ids, self.length[ids], np.zeros(ids.size, np.int64), 0)
         self.first[ids] = self.length[ids] = 0
 
@@ -457,6 +477,6 @@ class FrameStore:
         if (count < 0).any() or (begin < self.first[ids]).any() or (begin + count > self.length[ids]).any():
             raise ValueError("ranges must lie inside the frames their streams hold")
         most = int(count.max()) if ids.size else 0
-        with (torch.cuda.stream(stream) if stream is not None else torch.cuda.device(self.dev)):
+        with self._use(stream):
             req = self._upload(2 * ids + self._parity[ids], self.first[ids], begin, count)
             return frames_slots(self._table, *req.unbind(0), page_size=self.page_size, n_pages=self.n_pages, max_count=most)

@@ -767,6 +767,42 @@ def test_store_refuses_and_stays_as_it_was():
             S().FrameStore(**bad)
 
 
+def test_store_refuses_capture_and_stays_as_it_was():
+    store = S().FrameStore(2, 20, page_size=4, vocab=5)
+    rows = _rows(2, 15, "fp32", 3).view(2, 3, 5)
+    store.append(rows, [0, 1])
+    out = torch.zeros(4, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out += 1
+        for call in (lambda: store.append(rows, [0, 1]), lambda: store.release([0]), lambda: store.slots([0], [0], [3])):
+            with pytest.raises(RuntimeError, match="captured"):
+                call()
+    g.replay()
+    assert list(store.length) == [3, 3] and store.free_pages == store.n_pages - 2
+    slots = store.slots([0, 1], [0, 0], [3, 3])
+    assert torch.equal(store.pool[slots], rows)
+
+
+def test_store_dropped_while_its_calls_are_under_way():
+    """Its buffers go back to the allocator only when the stream of its calls has passed them."""
+    s = torch.cuda.Stream()
+    rows = _rows(8, 35 * 400, "fp32", 1).view(8, 400, 35)
+    torch.cuda.synchronize()
+    store = S().FrameStore(8, 400, vocab=35)
+    size = store.pool.shape
+    big = torch.zeros(64 << 20, device="cuda")
+    torch.cuda.synchronize()
+    with torch.cuda.stream(s):
+        for _ in range(20):
+            big += 1                          # holds the store's work back
+    store.append(rows, list(range(8)), stream=s)
+    del store
+    taken = [torch.zeros(size, device="cuda") for _ in range(3)]
+    torch.cuda.synchronize()
+    assert all(not bool(t.any()) for t in taken)
+
+
 def test_store_on_a_stream_of_its_own():
     store, want = S().FrameStore(2, 64, page_size=8, vocab=5), S().FrameStore(2, 64, page_size=8, vocab=5)
     side = torch.cuda.Stream()
