@@ -12,8 +12,9 @@
 // of W waves, R consecutive ones per lane: a step moves one 64-bit value from lane to lane (DPP) and needs no LDS and no
 // barrier.  With W > 1 the waves' ranges overlap: a wave's first HL lanes repeat the last ones of the wave below, whose
 // values they lack go wrong by at most two states per frame from the left edge on, and are set right from that wave through
-// LDS every 32 frames (half of that halves the overlap, but a refresh costs half a microsecond).  Waves of their own stage the frames' log probabilities in LDS some frames ahead, the columns being
-// the vocabulary, or only the sequence's own labels where those are fewer.
+// LDS every 32 frames (half of that halves the overlap, but a refresh costs half a microsecond).  Waves of their own stage
+// the frames' log probabilities in LDS some frames ahead, the columns being the vocabulary, or only the sequence's own labels
+// where those are fewer.
 //
 // Which predecessor was taken is one bit (blank) or two (token) per state, F frames of a lane to a word of the workspace.
 // Each state also carries where its path was 32 frames ago, so the path is first found at every 32nd frame, one look-up
@@ -52,7 +53,8 @@ constexpr int kLeg = 32;                // frames between two refreshes of the w
 constexpr int kLoaders = 4;             // waves that stage the frames
 constexpr int kBatch = 8;               // loads a loader lane has in flight
 // exponents of probability 0: a factor of 0 takes kShut off, what passed one stays below kNone and counts as 0.  They are
-// held above kZero every 32 frames, and 32 factors of 0 from there do not leave 31 bits.
+// held above kZero (and, for entries that are no log probabilities, below -kZero) every 32 frames, and 32 factors from there
+// do not leave 31 bits.
 constexpr int kShut = -(1 << 25), kNone = -(1 << 24), kZero = -(1 << 29);
 
 template <int W_, int R_>
@@ -348,7 +350,7 @@ struct Sum {
   __device__ __forceinline__ void renormalize() {
 #pragma unroll
     for (int r = 0; r < SH::R; ++r) {
-      e[r] = max(e[r] + __builtin_amdgcn_frexp_expf(m[r]), kZero);
+      e[r] = min(max(e[r] + __builtin_amdgcn_frexp_expf(m[r]), kZero), -kZero);
       m[r] = __builtin_amdgcn_frexp_mantf(m[r]);
     }
   }

@@ -533,6 +533,19 @@ def test_align_with_nan_and_infinity():
     _check_align(_dev(x, np.float32), tokens, tlen, flen, 7, True)
 
 
+@pytest.mark.parametrize("most", [2, 60, 300])
+def test_align_of_entries_that_are_no_log_probabilities(most):
+    """Large positive entries: the score is their sum, the total ends at 2^29 ln 2 instead of wrapping around."""
+    frames = 40000
+    x = torch.full((1, 1, 9), 5.9e4, device="cuda").expand(1, frames, 9)
+    tokens = _dev((np.arange(most) % 8)[None], np.int32)
+    r = S().ctc_align(x, tokens, _dev([most], np.int32), _dev([frames], np.int32), blank=8, total=True)
+    assert float(r.score) == np.float32(5.9e4 * frames)
+    assert 3.7e8 < float(r.total) < 3.8e8
+    r = S().ctc_align(x[:, :1000], tokens, _dev([most], np.int32), _dev([1000], np.int32), blank=8, total=True)
+    assert 5.9e7 <= float(r.total) <= 5.9e7 + 1000 * np.log(3) + 5.9e7 * 2 * EPS
+
+
 def test_align_reads_any_strides_and_slot_maps():
     rng = np.random.default_rng(5)
     x, tokens, tlen, flen = _ctc(rng, 5, 50, 12, 35, 34)
