@@ -394,6 +394,18 @@ def test_scores_of_one_wide_row(dtype, v):
         _check_scores(x[i : i + 1], [v // 3], 32)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("v,k", [(2500, 1), (9001, 10), (9001, 64), (40000, 20)])
+def test_scores_of_ordered_rows(v, k, dtype):
+    """Rows that ascend, descend, ascend from the middle on, ascend lane by lane, and ascend with NaN-free masks in between."""
+    x = _rows(5, v, dtype, v + k).float().sort(-1)[0]
+    x[1] = x[1].flip(0)
+    x[2] = x[2].roll(v // 2)
+    x[3] = x[3][torch.arange(v, device="cuda").mul(97).remainder(v).argsort()]
+    x[4, ::3] = float("-inf")
+    _check_scores(x.to(TYPES[dtype]), [v - 1, 0, v // 2, v // 3, v - 2], k)
+
+
 def test_scores_are_the_same_every_time():
     x = _rows(3, 131072, "bf16", 1)
     tokens = torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda")
