@@ -24,6 +24,10 @@
 // The sum over paths runs in a workgroup of its own, beside the one that finds the best path.  Each state is a 32-bit mantissa
 // and a 32-bit exponent of 2 (never a logarithm: no exp and log per state and frame, and no underflow, however unlikely a
 // prefix is): three terms aligned to the largest exponent, added, times the label's probability, itself mantissa and exponent.
+//
+// What bounds it is the issue of one wave's instructions, one after the other at some 2.4 ns each: 98 ns per frame with two
+// states per lane and one wave (187 frames and 43 tokens with the trace: 25 us), 102 with four waves, 138 with four states per
+// lane, 172 with eight waves of those (48 phrases of 2000 frames and 700 tokens with their sums: 350 us, 13 MB read).
 #include "scoring.h"
 
 #include <algorithm>
@@ -649,7 +653,9 @@ hipError_t launch_as(AlignArgs p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// the fewest states per lane and waves that hold the sequences
+// The fewest states per lane and waves that hold the sequences.  One sequence of 2000 frames: 43 tokens 196 us, 150 (four
+// waves) 203, 400 (four states per lane) 277, 700 (eight waves) 344, 900 (eight states per lane) 587; 700 tokens on four waves
+// of eight states take 532.
 template <class Fn>
 auto by_tokens(int most, Fn&& fn) {
   const int states = 2 * most + 1;

@@ -85,6 +85,17 @@ def test_plan_over_steps(n, page, max_add, steps):
         p.step(ids, keep, add, max_add)
 
 
+@pytest.mark.parametrize("n", [512, 513, 2048, 2049])
+def test_plan_of_whole_batches(n):
+    """Either side of the sizes at which the launch changes its shape; every stream in a call, then every other one."""
+    rng = np.random.default_rng(n)
+    p = Pool(rng, n, 6, 8, n * 9)
+    p.step(rng.permutation(n), np.zeros(n, int), rng.integers(0, 12, n), 11)
+    ids = np.arange(0, n, 2)
+    p.step(ids, p.length[ids] // 2, rng.integers(0, 12, len(ids)), 11)
+    p.step(np.arange(n), p.length - np.minimum(p.length - p.first, 3), np.full(n, 2), 2)
+
+
 def test_plan_of_no_requests_and_no_frames():
     p = Pool(np.random.default_rng(0), 3, 4, 5, 20)
     slots = p.step(np.array([], int), np.array([], int), np.array([], int), 6)
