@@ -347,7 +347,7 @@ struct Part {
   template <bool ALL, int Q, int N>
   __device__ __forceinline__ void news(const float (&x)[Q][N], const float (&top)[Q], float most, float other, int base, const int (&valid)[Q], int lane,
                                        int k) {
-    larger(most);
+    if (__ballot(most > m)) larger(most);
     if (k == 0) {
       floor = m;
       full = true;
