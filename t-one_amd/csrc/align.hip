@@ -654,8 +654,8 @@ hipError_t launch_as(AlignArgs p, hipStream_t st) {
 }
 
 // The fewest states per lane and waves that hold the sequences.  One sequence of 2000 frames: 43 tokens 196 us, 150 (four
-// waves) 203, 400 (four states per lane) 277, 700 (eight waves) 344, 900 (eight states per lane) 587; 700 tokens on four waves
-// of eight states take 532.
+// waves) 203, 400 (four states per lane) 277, 700 (eight waves) 344, 900 (twelve waves) 385, 1300 (eight waves of eight states)
+// 541; 700 tokens on four waves of eight states take 532, 900 on eight of eight 587.
 template <class Fn>
 auto by_tokens(int most, Fn&& fn) {
   const int states = 2 * most + 1;
@@ -663,6 +663,7 @@ auto by_tokens(int most, Fn&& fn) {
   if (states <= Shape<4, 2>::kStates) return fn(Shape<4, 2>{});
   if (states <= Shape<4, 4>::kStates) return fn(Shape<4, 4>{});
   if (states <= Shape<8, 4>::kStates) return fn(Shape<8, 4>{});
+  if (states <= Shape<12, 4>::kStates) return fn(Shape<12, 4>{});
   return fn(Shape<8, 8>{});
 }
 static_assert(Shape<8, 8>::kStates >= 2 * TONE_ALIGN_MAX_TOKENS + 1, "the longest sequences fit");
@@ -702,7 +703,7 @@ int tone_ctc_align(int device, const void* x, int type, int64_t stride, int64_t 
   const char* what = "tone_ctc_align";
   if (batch < 0 || frames < 0 || x_rows < 0 || vocab <= 0 || vocab > (1 << 24))
     return refuse(what, "batch, frames, x_rows or vocab out of range");
-  if (frames > kMaxFrames || batch > kMaxThreads / (2 * 64 * (8 + kLoaders))) return refuse(what, "batch or frames too large for one launch");
+  if (frames > kMaxFrames || batch > kMaxThreads / (2 * 64 * (12 + kLoaders))) return refuse(what, "batch or frames too large for one launch");
   if (max_tokens < 0 || max_tokens > TONE_ALIGN_MAX_TOKENS) return refuse(what, "max_tokens must be in 0 .. TONE_ALIGN_MAX_TOKENS");
   if (!known_type(type)) return refuse(what, "unknown element type");
   if (blank < 0 || blank >= vocab) return refuse(what, "blank outside the vocabulary");

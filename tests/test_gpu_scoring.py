@@ -484,6 +484,15 @@ def test_align_long(f, most):
     _align_by_rows(rng, x, tokens, lens)
 
 
+@pytest.mark.parametrize("most", [63, 64, 159, 160, 415, 416, 799, 800, 1183, 1184])
+def test_align_either_side_of_a_shape(most):
+    """Token counts around those at which the launch takes more waves or more states per lane."""
+    rng = np.random.default_rng(most)
+    f = most + most // 4 + 40
+    x, tokens, _, _ = _ctc(rng, 2, f, most, 35, 34)
+    _align_by_rows(rng, x, tokens, np.array([[most, f], [most - 1, f - 1]], np.int32))
+
+
 def _align_by_rows(rng, x, tokens, lens):
     """Against the definition evaluated a frame at a time over all states (the oracle's loops are too slow here)."""
     b, f, vocab = x.shape
