@@ -301,7 +301,8 @@ struct Part {
       most = q ? fmaxf(most, top[q]) : top[q];
     }
     const float other = shared ? value_of(*static_cast<volatile int*>(shared)) : -INFINITY;
-    if ((!full || __ballot(most > floor)) && (k == 0 || __ballot(most >= other)))
+    // (a NaN is not below `other`: lanes of nothing else fill a list that is not full)
+    if ((!full || __ballot(most > floor)) && (k == 0 || __ballot(!(most < other))))
       news<ALL, Q, N>(x, top, most, other, base, valid, lane, k);
     else if (__ballot(most > m)) larger(most);
 #pragma unroll

@@ -966,3 +966,27 @@ def test_pipeline_out_of_pages_leaves_its_streams_as_they_were(session):
     assert torch.equal(pipe.state_of(b), state) and pipe._open[b].offset == 0
     with pytest.raises(ValueError):
         P.StreamingGreedyPipeline(session, 2, scores=36)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("n,v", [(5, 65), (5, 128), (5, 256), (5, 512), (5, 1024), (5, 4096), (5, 65536), (5, 65537), (5, 131072), (300, 5000),
+                                 (1600, 16384)])
+def test_scores_of_rows_of_nan(n, v, dtype):
+    """Rows of nothing but NaN, of either sign, and of NaN but for a few entries: ids distinct and in range, ranks in range, floating
+    outputs NaN; the other rows as they are without them."""
+    x = _rows(n, v, dtype, v)
+    clean = x.clone()
+    nan = torch.tensor([0x7FC00000, -0x400000], dtype=torch.int32, device="cuda").view(torch.float32).to(TYPES[dtype])
+    x[0] = nan[0]
+    x[1] = nan[1]
+    x[2, : v - 1] = nan[0]
+    x[3, : v // 2] = nan[1]
+    x[3, v // 2 + 3 :] = nan[0]
+    tokens = torch.arange(n, dtype=torch.int32, device="cuda") * 31 % v
+    for k in (1, 10, 64):
+        r, want = S().token_scores(x, tokens, k=k), S().token_scores(clean, tokens, k=k)
+        ids, rank = r.top_ids.cpu().numpy(), r.rank.cpu().numpy()
+        assert ids.min() >= 0 and ids.max() < v and rank.min() >= 0 and rank.max() < v, k
+        assert all(len(set(row)) == k for row in ids.tolist())
+        assert all(bool(t[:4].isnan().all()) for t in (r.logprob, r.entropy, r.top_logprob))
+        assert all(torch.equal(a[4:], b[4:]) for a, b in zip(r, want))
