@@ -269,18 +269,19 @@ class StreamingGreedyPipeline:
 
     # --- one step ----------------------------------------------------------------------------
     def step_frames(self, chunks: np.ndarray, slots: Sequence[int]) -> np.ndarray:
-        """Advance ``slots`` by one chunk each on the device; returns their frame info (n, 10) int32."""
+        """Advance ``slots`` by one chunk each on the device; returns their frame info (n, 10) int32.  The splitter does not see
+        these frames, so with ``scores`` their rows are not held: they are of no phrase."""
+        return self._step(chunks, slots)
+
+    def _step(self, chunks: np.ndarray, slots: Sequence[int], kept=None) -> np.ndarray:
+        """:meth:`step_frames`; with ``kept`` (n, 10), the step's rows go to those slots of the store."""
         import torch
         n = len(slots)
         mb = self.session.max_batch
         info = np.empty((n, self.frames), np.int32)
         logp = np.empty((n, self.frames, C.VOCAB), np.float32) if self.decoder is not None else None
-        kept = None
-        if self._store is not None:
-            # before the step, so that a store out of pages raises with the streams as they were; frames before the
-            # splitter's buffer are of no phrase to come
+        if kept is not None:
             from .scoring import frames_put
-            kept = self._store.reserve(slots, self.frames, keep=[self._open[s].offset for s in slots])
         self.session.set_frame_info(self._info)    # frame_info is session state: claim it every step
         for b0 in range(0, n, mb):
             b1 = min(n, b0 + mb)
@@ -328,7 +329,15 @@ class StreamingGreedyPipeline:
         if len(set(slots)) != n or any(s not in self._open for s in slots):
             raise ValueError("slots must be distinct open stream slots")
         is_last = [False] * n if is_last is None else list(is_last)
-        info = self.step_frames(chunks, slots) if n else np.zeros((0, self.frames), np.int32)
+        if n == 0:
+            info = np.zeros((0, self.frames), np.int32)
+        elif self._store is None:
+            info = self.step_frames(chunks, slots)
+        else:
+            # before the step, so that a store out of pages raises with the streams as they were; frames before the
+            # splitter's buffer are of no phrase to come
+            kept = self._store.reserve(slots, self.frames, keep=[self._open[s].offset for s in slots])
+            info = self._step(chunks, slots, kept)
         out: list[list[TextPhrase]] = []
         held = {slot: self._open[slot].offset for slot in slots}
         for i, slot in enumerate(slots):

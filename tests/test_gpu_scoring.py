@@ -990,3 +990,21 @@ def test_scores_of_rows_of_nan(n, v, dtype):
         assert all(len(set(row)) == k for row in ids.tolist())
         assert all(bool(t[:4].isnan().all()) for t in (r.logprob, r.entropy, r.top_logprob))
         assert all(torch.equal(a[4:], b[4:]) for a, b in zip(r, want))
+
+
+def test_pipeline_steps_without_the_splitter(session):
+    """step_frames by itself answers with the frame info for as long as a caller likes, scores or not, and holds no rows back:
+    what the splitter does not see is of no phrase."""
+    from tone_amd import pipeline as P
+    pipe, plain = P.StreamingGreedyPipeline(session, 1, scores=2, score_pages=40), P.StreamingGreedyPipeline(session, 1)
+    a, b = pipe.open_stream(), plain.open_stream()
+    audio = _speech(3, 12)
+    for step in range(230):
+        np.testing.assert_array_equal(pipe.step_frames(audio[step % 12][None], [a]), plain.step_frames(audio[step % 12][None], [b]))
+    assert pipe._store.free_pages == pipe._store.n_pages and pipe._store.length[a] == 0
+    with pytest.raises(ValueError):
+        pipe.step_frames(audio[:1, :100], [a])
+    got = [p for i in range(12) for p in pipe.forward(audio[i][None], [a], [i == 11])[0]]
+    want = [p for i in range(12) for p in plain.forward(audio[i][None], [b], [i == 11])[0]]
+    assert len(got) > 0 and [(p.text, p.start_time, p.end_time) for p in got] == [(p.text, p.start_time, p.end_time) for p in want]
+    assert all(len(p.tokens) == len(p.text) and p.score is not None for p in got)
