@@ -338,24 +338,19 @@ class StreamingGreedyPipeline:
             # splitter's buffer are of no phrase to come
             kept = self._store.reserve(slots, self.frames, keep=[self._open[s].offset for s in slots])
             info = self._step(chunks, slots, kept)
-        out: list[list[TextPhrase]] = []
-        held = {slot: self._open[slot].offset for slot in slots}
+        # every stream's splitter first: a decoder that raises loses this step's phrases, and no stream its frames
+        held = [self._open[slot].offset for slot in slots]
+        found = []
         for i, slot in enumerate(slots):
             toks, speech = decode_frame_info(info[i])
-            if self._store is not None:
-                payload = toks if self.decoder is None else self._last_logp[i]
-                found, self._open[slot] = split_frames(payload, speech, self._open[slot], is_last=is_last[i])
-                decode = greedy_text if self.decoder is None else self.decoder.forward
-                out.append([(ScoredPhrase(decode(t), *phrase_times(s, e)), max(held[slot], s - SPEECH_EXPAND), len(t))
-                            for t, s, e in found])
-                continue
-            if self.decoder is None:
-                phrases, self._open[slot] = frames_to_phrases(toks, speech, self._open[slot], is_last=is_last[i])
-            else:
-                phrases, self._open[slot] = frames_to_phrases(self._last_logp[i], speech, self._open[slot],
-                                                              is_last=is_last[i], decode=self.decoder.forward)
-            out.append(phrases)
-        return out if self._store is None else self._scored(out, slots)
+            phrases, self._open[slot] = split_frames(toks if self.decoder is None else self._last_logp[i], speech, self._open[slot],
+                                                     is_last=is_last[i])
+            found.append(phrases)
+        decode = greedy_text if self.decoder is None else self.decoder.forward
+        if self._store is None:
+            return [[TextPhrase(decode(t), *phrase_times(s, e)) for t, s, e in phrases] for phrases in found]
+        return self._scored([[(ScoredPhrase(decode(t), *phrase_times(s, e)), max(h, s - SPEECH_EXPAND), len(t)) for t, s, e in phrases]
+                             for h, phrases in zip(held, found)], slots)
 
     def _scored(self, found, slots) -> list[list[TextPhrase]]:
         """Fill in the phrases' scores: found[i] = [(phrase, first frame, frames)] of stream slots[i]."""

@@ -1008,3 +1008,61 @@ def test_pipeline_steps_without_the_splitter(session):
     want = [p for i in range(12) for p in plain.forward(audio[i][None], [b], [i == 11])[0]]
     assert len(got) > 0 and [(p.text, p.start_time, p.end_time) for p in got] == [(p.text, p.start_time, p.end_time) for p in want]
     assert all(len(p.tokens) == len(p.text) and p.score is not None for p in got)
+
+
+
+
+class _Flags:
+    """Speech flags and tokens in the place of the model's (synthetic weights hear speech everywhere): pauses of 25 frames."""
+
+    def __init__(self, monkeypatch, pauses, steps):
+        from tone_amd import pipeline as P
+        self.tokens = np.random.default_rng(len(pauses)).integers(0, 34, (len(pauses), 10 * steps)).astype(np.int32)
+        self.tokens[:, ::3] = 34
+        self.speech = np.ones((len(pauses), 10 * steps), bool)
+        for i, begins in enumerate(pauses):
+            for b in begins:
+                self.speech[i, b : b + 25] = False
+        monkeypatch.setattr(P, "decode_frame_info", lambda info: next(self.left))
+
+    def at(self, step):
+        now = slice(10 * step, 10 * step + 10)
+        self.left = iter([(t[now], s[now]) for t, s in zip(self.tokens, self.speech)])
+
+
+@pytest.mark.parametrize("scores", [None, 3])
+def test_pipeline_after_a_decoder_that_raised(session, monkeypatch, scores):
+    """A decoder that raises loses the phrases of its step alone: every stream's later phrases and scores are as undisturbed."""
+    from tone_amd import pipeline as P
+
+    class Once(P.GreedyLogprobDecoder):
+        broken = False
+
+        def forward(self, logprobs):
+            if self.broken:
+                self.broken = False
+                raise RuntimeError("on purpose")
+            return super().forward(logprobs)
+    chunks = np.stack([_speech(4, 14), _speech(5, 14)])
+    flags = _Flags(monkeypatch, [[30, 100], [60]], 14)            # stream 0 pauses in step 3, stream 1 in step 6
+    runs = []
+    for broken in (False, True):
+        dec = Once()
+        pipe = P.StreamingGreedyPipeline(session, 2, dec, scores=scores)
+        slots = [pipe.open_stream(), pipe.open_stream()]
+        steps, raised = [], None
+        for step in range(14):
+            dec.broken = broken and raised is None and step >= 3
+            flags.at(step)
+            try:
+                steps.append(pipe.forward(chunks[:, step], slots, [step == 13] * 2))
+            except RuntimeError:
+                raised = step
+                steps.append(None)
+        runs.append(steps)
+        assert (raised is not None) == broken
+        if scores is not None:
+            assert all(pipe._store.length[s] == pipe._open[s].offset + pipe._open[s].speech.size for s in slots)
+    assert [len(p) for p in runs[0][raised]] == [1, 0] and sum(len(p) for s in runs[0][raised + 1 :] for p in s) == 4
+    for want, got in zip(*runs):
+        assert got is None or got == want
