@@ -329,28 +329,34 @@ class StreamingGreedyPipeline:
         if len(set(slots)) != n or any(s not in self._open for s in slots):
             raise ValueError("slots must be distinct open stream slots")
         is_last = [False] * n if is_last is None else list(is_last)
-        if n == 0:
-            info = np.zeros((0, self.frames), np.int32)
-        elif self._store is None:
-            info = self.step_frames(chunks, slots)
-        else:
-            # before the step, so that a store out of pages raises with the streams as they were; frames before the
-            # splitter's buffer are of no phrase to come
-            kept = self._store.reserve(slots, self.frames, keep=[self._open[s].offset for s in slots])
-            info = self._step(chunks, slots, kept)
-        # every stream's splitter first: a decoder that raises loses this step's phrases, and no stream its frames
         held = [self._open[slot].offset for slot in slots]
-        found = []
-        for i, slot in enumerate(slots):
-            toks, speech = decode_frame_info(info[i])
-            phrases, self._open[slot] = split_frames(toks if self.decoder is None else self._last_logp[i], speech, self._open[slot],
-                                                     is_last=is_last[i])
-            found.append(phrases)
+        if n == 0:
+            split = []
+        elif self._store is None:
+            split = self._split(self.step_frames(chunks, slots), slots, is_last)
+        else:
+            # the store counts a stream's frames as its splitter does, so an error in between takes the reservation back
+            with self._store._undone():
+                # before the step, so that a store out of pages raises with the streams as they were; frames before the
+                # splitter's buffer are of no phrase to come
+                kept = self._store.reserve(slots, self.frames, keep=held)
+                split = self._split(self._step(chunks, slots, kept), slots, is_last)
+        # every stream's splitter first: a decoder that raises loses this step's phrases, and no stream its frames
+        self._open.update((slot, state) for slot, (_, state) in zip(slots, split))
+        found = [phrases for phrases, _ in split]
         decode = greedy_text if self.decoder is None else self.decoder.forward
         if self._store is None:
             return [[TextPhrase(decode(t), *phrase_times(s, e)) for t, s, e in phrases] for phrases in found]
         return self._scored([[(ScoredPhrase(decode(t), *phrase_times(s, e)), max(h, s - SPEECH_EXPAND), len(t)) for t, s, e in phrases]
                              for h, phrases in zip(held, found)], slots)
+
+    def _split(self, info: np.ndarray, slots: Sequence[int], is_last: Sequence[bool]):
+        """A step's frames through the streams' splitters: ([(payload, start, end)], next state) per stream."""
+        out = []
+        for i, slot in enumerate(slots):
+            toks, speech = decode_frame_info(info[i])
+            out.append(split_frames(toks if self.decoder is None else self._last_logp[i], speech, self._open[slot], is_last=is_last[i]))
+        return out
 
     def _scored(self, found, slots) -> list[list[TextPhrase]]:
         """Fill in the phrases' scores: found[i] = [(phrase, first frame, frames)] of stream slots[i]."""

@@ -430,6 +430,18 @@ class FrameStore:
         self.free_pages += drop - take
         return slots
 
+    @contextlib.contextmanager
+    def _undone(self):
+        """Takes back what is reserved under it where the block raises.  The host's counts are all there is to take back: a
+        plan writes spare table rows, the other cursors and queue entries behind the free ones, and the next one is made from
+        the rows and cursors it was made from itself."""
+        was = self.first.copy(), self.length.copy(), self._parity.copy(), self._side, self.free_pages
+        try:
+            yield
+        except BaseException:
+            self.first, self.length, self._parity, self._side, self.free_pages = was
+            raise
+
     def reserve(self, ids, frames: int, keep=None, counts=None, stream=None):
         """Slots int64 (n, frames) for the next counts[i] (default: ``frames``) frames of the streams ``ids`` (distinct), to be
         written with :func:`frames_put`.  Frames before keep[i] (default: none) are let go; new ones among them get no slot."""

@@ -1066,3 +1066,80 @@ def test_pipeline_after_a_decoder_that_raised(session, monkeypatch, scores):
     assert [len(p) for p in runs[0][raised]] == [1, 0] and sum(len(p) for s in runs[0][raised + 1 :] for p in s) == 4
     for want, got in zip(*runs):
         assert got is None or got == want
+
+
+def _run(pipe, chunks, flags, at=None, fail=None):
+    """All phrases per step and stream; in step ``at`` the call raises once under ``fail`` and is made again."""
+    slots = [pipe.open_stream() for _ in chunks]
+    got = []
+    for step in range(chunks.shape[1]):
+        last = [step == chunks.shape[1] - 1] * len(slots)
+        if step == at:
+            flags.at(step)
+            with fail(), pytest.raises(RuntimeError, match="on purpose"):
+                pipe.forward(chunks[:, step], slots, last)
+        flags.at(step)
+        got.append(pipe.forward(chunks[:, step], slots, last))
+    return slots, got
+
+
+@pytest.mark.parametrize("resident", [True, False])
+@pytest.mark.parametrize("where", ["run", "put", "split"])
+@pytest.mark.parametrize("at", [0, 7])
+def test_pipeline_scores_after_a_step_that_raised(session, monkeypatch, resident, where, at):
+    """A step that raises leaves the store with the splitter: made again, the phrases and scores are those of an undisturbed run."""
+    from tone_amd import pipeline as P
+    chunks = np.stack([_speech(4, 14), _speech(5, 14)])
+
+    def raising(*a, **k):
+        raise RuntimeError("on purpose")
+
+    def fail():
+        m = pytest.MonkeyPatch()
+        if where == "run":
+            m.setattr(session, "run_ring" if resident else "run_rows", raising)
+        elif where == "put":
+            m.setattr(S(), "frames_put", raising)
+        else:
+            m.setattr(P, "split_frames", raising)
+        return _undone(m)
+    flags = _Flags(monkeypatch, [[30, 100], [60]], 14)
+    want, pipe = (P.StreamingGreedyPipeline(session, 2, scores=3, resident=resident) for _ in range(2))
+    _, a = _run(want, chunks, flags)
+    if where != "run":
+        # the model has stepped: its state is put back as a caller would, so that the same step can be made again
+        kept = {}
+        monkeypatch.setattr(pipe, "forward", _run_of(pipe, kept))
+    slots, b = _run(pipe, chunks, flags, at, fail)
+    assert sum(len(p) for step in a for p in step) == 5 and a == b
+    assert all(pipe._store.length[s] == pipe._open[s].offset + pipe._open[s].speech.size for s in slots)
+
+
+def _undone(m):
+    import contextlib
+
+    @contextlib.contextmanager
+    def block():
+        try:
+            yield
+        finally:
+            m.undo()
+    return block()
+
+
+def _run_of(pipe, kept):
+    """pipe.forward that puts the model's state back where the call raises."""
+    forward = pipe.forward
+
+    def call(*args):
+        kept.update(slab=pipe._slab.clone(), parity=pipe._parity.copy(), rings=None if pipe._rings is None else pipe._rings.clone())
+        try:
+            return forward(*args)
+        except RuntimeError:
+            torch.cuda.synchronize()
+            pipe._slab.copy_(kept["slab"])
+            pipe._parity[:] = kept["parity"]
+            if pipe._rings is not None:
+                pipe._rings.copy_(kept["rings"])
+            raise
+    return call
