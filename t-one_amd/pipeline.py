@@ -329,6 +329,8 @@ class StreamingGreedyPipeline:
         if len(set(slots)) != n or any(s not in self._open for s in slots):
             raise ValueError("slots must be distinct open stream slots")
         is_last = [False] * n if is_last is None else list(is_last)
+        if len(is_last) < n:
+            raise ValueError(f"'is_last' must have one entry per stream, got {len(is_last)} for {n}")
         held = [self._open[slot].offset for slot in slots]
         if n == 0:
             split = []

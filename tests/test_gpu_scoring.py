@@ -1143,3 +1143,14 @@ def _run_of(pipe, kept):
                 pipe._rings.copy_(kept["rings"])
             raise
     return call
+
+
+def test_pipeline_refuses_too_few_is_last(session):
+    """Before the step: the streams are as they were."""
+    from tone_amd import pipeline as P
+    pipe = P.StreamingGreedyPipeline(session, 2, scores=0)
+    a, b = pipe.open_stream(), pipe.open_stream()
+    state = pipe.state_of(a).clone()
+    with pytest.raises(ValueError, match="is_last"):
+        pipe.forward(np.stack([_speech(1, 1)[0], _speech(2, 1)[0]]), [a, b], [False])
+    assert torch.equal(pipe.state_of(a), state) and list(pipe._store.length) == [0, 0]
