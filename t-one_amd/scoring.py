@@ -199,20 +199,26 @@ def _rows_of(t, name: str) -> int:
     return t.shape[-1] if step is None else step
 
 
-def frames_put(src, slots, pool, stream=None) -> None:
-    """pool[slots[i]] = row i of ``src`` (..., vocab), rounded once to the pool's type; slots int64 with one entry per row,
-    distinct, those outside the pool left out.  pool (n_rows, vocab) float32 / float16 / bfloat16."""
-    torch = _torch()
+def _check_put(src, pool) -> tuple[int, int, int, int]:
+    """What :func:`frames_put` asks of its rows and its pool: (type of src, type of the pool, distance of src's rows, rows)."""
     stype, ptype = _type(src, "src"), _type(pool, "pool")
     sstride = _rows_of(src, "src")
     if pool.dim() != 2 or pool.shape[1] != src.shape[-1] or (pool.shape[1] > 1 and pool.stride(1) != 1) \
             or (pool.shape[0] > 1 and pool.stride(0) < pool.shape[1]):
         raise ValueError(f"pool must be (rows, {src.shape[-1]}) with unit column stride, got {tuple(pool.shape)}")
     n = src.numel() // src.shape[-1]
-    if slots.dtype != torch.int64 or slots.numel() != n or not slots.is_contiguous():
-        raise ValueError(f"slots must be {n} contiguous int64 entries, got {tuple(slots.shape)} {slots.dtype}")
     if n > 1 and sstride < src.shape[-1]:
         raise ValueError("src rows must not overlap")
+    return stype, ptype, sstride, n
+
+
+def frames_put(src, slots, pool, stream=None) -> None:
+    """pool[slots[i]] = row i of ``src`` (..., vocab), rounded once to the pool's type; slots int64 with one entry per row,
+    distinct, those outside the pool left out.  pool (n_rows, vocab) float32 / float16 / bfloat16."""
+    torch = _torch()
+    stype, ptype, sstride, n = _check_put(src, pool)
+    if slots.dtype != torch.int64 or slots.numel() != n or not slots.is_contiguous():
+        raise ValueError(f"slots must be {n} contiguous int64 entries, got {tuple(slots.shape)} {slots.dtype}")
     dev = _device(src, slots, pool)
     lib = _lib.load()
     with _On(dev, stream, src, slots, pool) as st:
@@ -462,10 +468,10 @@ class FrameStore:
             raise ValueError(f"rows must be ({ids.size}, T, {self.pool.shape[1]}), got {tuple(rows.shape)}")
         if rows.device != self.dev:
             raise ValueError(f"rows on {rows.device}, the store on {self.dev}")
-        _type(rows, "rows")
-        _rows_of(rows, "rows")
-        slots = self.reserve(ids, int(rows.shape[1]), keep, counts, stream)
-        frames_put(rows, slots, self.pool, stream=stream)
+        _check_put(rows, self.pool)
+        with self._undone():
+            slots = self.reserve(ids, int(rows.shape[1]), keep, counts, stream)
+            frames_put(rows, slots, self.pool, stream=stream)
         return slots
 
     def release(self, ids, stream=None) -> None:

@@ -1154,3 +1154,33 @@ def test_pipeline_refuses_too_few_is_last(session):
     with pytest.raises(ValueError, match="is_last"):
         pipe.forward(np.stack([_speech(1, 1)[0], _speech(2, 1)[0]]), [a, b], [False])
     assert torch.equal(pipe.state_of(a), state) and list(pipe._store.length) == [0, 0]
+
+
+def test_store_refuses_rows_that_cannot_be_put_and_stays_as_it_was():
+    """Rows that are one row repeated: refused before any frame is reserved."""
+    store = S().FrameStore(2, 32, page_size=8, vocab=5)
+    store.append(_rows(20, 5, "fp32", 1).view(2, 10, 5), [0, 1])
+    now = lambda: (store.pool, store._table, store._queue, store._cursors)  # noqa: E731
+    before, first, length, free = [t.clone() for t in now()], store.first.copy(), store.length.copy(), store.free_pages
+    for rows in (_rows(1, 5, "fp32", 2).view(1, 1, 5).expand(2, 10, 5), _rows(2, 5, "fp32", 2).view(2, 1, 5).expand(2, 10, 5)):
+        with pytest.raises(ValueError):
+            store.append(rows, [0, 1])
+    assert all(torch.equal(a, b) for a, b in zip(before, now()))
+    assert (store.first == first).all() and (store.length == length).all() and store.free_pages == free
+
+
+def test_store_takes_a_reservation_back_where_the_copy_raises(monkeypatch):
+    store = S().FrameStore(2, 32, page_size=8, n_pages=6, vocab=5)
+    rows = _rows(60, 5, "fp32", 1).view(2, 30, 5)
+    store.append(rows[:, :10].contiguous(), [0, 1])
+
+    def raising(*a, **k):
+        raise RuntimeError("on purpose")
+    with monkeypatch.context() as m:
+        m.setattr(S(), "frames_put", raising)
+        for _ in range(3):
+            with pytest.raises(RuntimeError, match="on purpose"):
+                store.append(rows[:, 10:16].contiguous(), [1, 0], keep=[9, 9])
+    assert list(store.first) == [0, 0] and list(store.length) == [10, 10] and store.free_pages == 2
+    store.append(rows[:, 10:16].contiguous(), [0, 1])
+    assert torch.equal(store.pool[store.slots([0, 1], [0, 0], [16, 16])], rows[:, :16])
