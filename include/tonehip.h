@@ -205,7 +205,8 @@ int tone_frames_slots(int device, const int32_t *table, int64_t table_stride, in
                       int64_t *slots, int max_count, void *stream);
 
 /* pool row slots[i] = src row i (strides in elements; one rounding to the pool's type) for i < n; slots outside
- * [0, pool_rows) are left out, pool rows that no slot names are left as they were.  Slots must be distinct. */
+ * [0, pool_rows) are left out, pool rows that no slot names are left as they were.  Slots must be distinct; src must not
+ * overlap the pool (columns side by side in rows of the same length may lie in one buffer). */
 int tone_frames_put(int device, const void *src, int src_type, int64_t src_stride, const int64_t *slots, int64_t n, int vocab,
                     void *pool, int pool_type, int64_t pool_stride, int64_t pool_rows, void *stream);
 

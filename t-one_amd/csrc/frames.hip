@@ -314,6 +314,24 @@ hipError_t launch_slots(const SlotArgs& p, hipStream_t st) {
   return hipGetLastError();
 }
 
+// Whether the rows of src and the pool share memory.  Rows are copied in no order, so a row that is read and written would be
+// torn; columns side by side in rows of one length are apart.
+bool meet(const void* src, int src_type, int64_t src_stride, int64_t n, const void* pool, int pool_type, int64_t pool_stride,
+          int64_t pool_rows, int vocab) {
+  if (pool_rows == 0) return false;
+  using Wide = __int128;                 // strides are the caller's: no product below can overflow
+  const auto size = [](int type) { return type == TONE_TYPE_FP32 ? 4 : 2; };
+  const Wide row = (Wide)vocab * size(src_type), pool_row = (Wide)vocab * size(pool_type);
+  Wide pitch = (Wide)src_stride * size(src_type);
+  const Wide pool_pitch = (Wide)pool_stride * size(pool_type);
+  const Wide at = (Wide) reinterpret_cast<uintptr_t>(src) - (Wide) reinterpret_cast<uintptr_t>(pool);
+  if (at >= (pool_rows - 1) * pool_pitch + pool_row || at + (n - 1) * pitch + row <= 0) return false;
+  if (n == 1) pitch = pool_pitch;
+  else if (pool_rows > 1 && pitch != pool_pitch) return true;
+  const Wide in = (at % pitch + pitch) % pitch;
+  return !(in >= pool_row && in + row <= pitch);
+}
+
 hipError_t launch_put(const PutArgs& a, hipStream_t st) {
   switch (a.src_type) {
     case TONE_TYPE_FP32: return put_from<float>(a, st);
@@ -372,6 +390,7 @@ int tone_frames_put(int device, const void* src, int src_type, int64_t src_strid
   if (src_stride < vocab || pool_stride < vocab) return refuse(what, "row stride < vocab");
   if (!aligned(src, src_type) || !aligned(pool, pool_type)) return refuse(what, "src or pool not aligned to its element type");
   if (n > (kMaxThreads / 256 - 1) * kPutChunk / vocab) return refuse(what, "too many rows for one launch");
+  if (meet(src, src_type, src_stride, n, pool, pool_type, pool_stride, pool_rows, vocab)) return refuse(what, "src overlaps the pool");
   PutArgs p{src, src_type, src_stride, slots, n, vocab, pool, pool_type, pool_stride, pool_rows};
   return launch_on(device, what, [&] { return launch_put(p, static_cast<hipStream_t>(stream)); });
 }

@@ -209,12 +209,30 @@ def _check_put(src, pool) -> tuple[int, int, int, int]:
     n = src.numel() // src.shape[-1]
     if n > 1 and sstride < src.shape[-1]:
         raise ValueError("src rows must not overlap")
+    if n and pool.shape[0] and src.device == pool.device and _meet(src, sstride, n, pool):
+        raise ValueError("src must not overlap the pool")
     return stype, ptype, sstride, n
+
+
+def _meet(src, sstride: int, n: int, pool) -> bool:
+    """Whether rows of ``src`` (n, sstride entries apart) and the pool share memory; columns side by side in rows of the same
+    length do not."""
+    vocab, rows = src.shape[-1], pool.shape[0]
+    each, to = src.element_size(), pool.element_size()
+    pitch, pool_pitch = sstride * each, pool.stride(0) * to
+    at = src.data_ptr() - pool.data_ptr()
+    if at >= (rows - 1) * pool_pitch + vocab * to or at + (n - 1) * pitch + vocab * each <= 0:
+        return False
+    if n == 1:
+        pitch = pool_pitch
+    elif rows > 1 and pitch != pool_pitch:
+        return True
+    return not (at % pitch >= vocab * to and at % pitch + vocab * each <= pitch)
 
 
 def frames_put(src, slots, pool, stream=None) -> None:
     """pool[slots[i]] = row i of ``src`` (..., vocab), rounded once to the pool's type; slots int64 with one entry per row,
-    distinct, those outside the pool left out.  pool (n_rows, vocab) float32 / float16 / bfloat16."""
+    distinct, those outside the pool left out.  pool (n_rows, vocab) float32 / float16 / bfloat16; ``src`` must not lie in it."""
     torch = _torch()
     stype, ptype, sstride, n = _check_put(src, pool)
     if slots.dtype != torch.int64 or slots.numel() != n or not slots.is_contiguous():

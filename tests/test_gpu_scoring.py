@@ -1184,3 +1184,18 @@ def test_store_takes_a_reservation_back_where_the_copy_raises(monkeypatch):
     assert list(store.first) == [0, 0] and list(store.length) == [10, 10] and store.free_pages == 2
     store.append(rows[:, 10:16].contiguous(), [0, 1])
     assert torch.equal(store.pool[store.slots([0, 1], [0, 0], [16, 16])], rows[:, :16])
+
+
+@pytest.mark.parametrize("src,pool", [((slice(None), slice(35)), (slice(None), slice(35, 70))), ((slice(None), slice(35, 70)), (slice(None), slice(35))),
+                                      ((slice(0, 20), slice(35)), (slice(20, None), slice(35))), ((slice(7, 8), slice(36, 71)), (slice(None), slice(1, 36)))])
+def test_put_beside_the_rows_it_reads(src, pool):
+    """Rows and a pool in one buffer that share no entry."""
+    b = _rows(60, 71, "fp32", 4)
+    want = b.clone()
+    n = b[src].shape[0]
+    slots = torch.randperm(b[pool].shape[0], device="cuda", generator=torch.Generator(device="cuda").manual_seed(n))[:n].contiguous()
+    want[pool][slots] = b[src]
+    S().frames_put(b[src], slots, b[pool])
+    assert torch.equal(b, want)
+    with pytest.raises(ValueError, match="overlap"):
+        S().frames_put(b[src], slots, b[:, src[1]])

@@ -263,3 +263,35 @@ def test_c_empty_calls_do_nothing():
     assert lib.tone_frames_put(0, None, 0, 5, None, 0, 5, None, 0, 5, 9, None) == 0
     assert lib.tone_token_scores(0, None, 0, 5, 0, None, 0, 5, None, 0, None, None, None, None, None, None) == 0
     assert lib.tone_ctc_align(0, None, 0, 5, 0, 0, None, 0, 6, 5, 4, None, 3, None, None, None, None, None, None, None, 0, None) == 0
+
+
+def _overlaps():
+    """Rows and a pool in one buffer of (12, 16) entries: (src, pool, whether they share memory)."""
+    b = torch.zeros((12, 16))
+    h = torch.zeros((12, 32), dtype=torch.float16)
+    flat = b.view(-1)
+    return [
+        (b[2:5, :5], b[:, :5], True), (b[:4, :5], b[4:, :5], False), (b[4:, :5], b[:4, :5], False), (b[:5, :5], b[4:, :5], True),
+        (b[:, :5], b[:, 5:10], False), (b[:, 5:10], b[:, :5], False), (b[:, 4:9], b[:, :5], True), (b[:, 11:], b[:, :5], False),
+        (b[3:4, 5:10], b[:, :5], False), (b[3:4, 4:9], b[:, :5], True), (b[3:4, 12:], b[:, :4], False), (b[::2, :5], b[:, 8:13], True),
+        (flat[30:35].view(1, 5), b[:, :5], True), (b[:, :5], flat[21:26].view(1, 5), False), (b[:, :5], flat[18:23].view(1, 5), True),
+        (b[:, :5], b[:0, :5], False), (b[:0, :5], b[:, :5], False), (b, b, True), (b[:3], b[3:], False), (h[:, :8], h[:, 8:16], False),
+        (h[:, :8], h[:, 7:15], True), (h.view(torch.float32)[:, :8], h[:, 16:24], False), (h.view(torch.float32)[:, :8], h[:, 15:23], True),
+        (h[:, :8], h.view(torch.float32)[:, 4:12], False), (h[:, 16:24], h.view(torch.float32)[:, :8], False), (h[:, 15:23], h.view(torch.float32)[:, :8], True),
+    ]
+
+
+@pytest.mark.parametrize("i", range(26))
+def test_frames_put_refuses_rows_of_the_pool(i):
+    """Rows in the memory of the pool would be read and written in no order; what lies beside them may be copied."""
+    src, pool, meets = _overlaps()[i]
+    mine = {a + j for r in range(src.shape[0]) for a in [src[r].data_ptr()] for j in range(src.shape[1] * src.element_size())}
+    theirs = {a + j for r in range(pool.shape[0]) for a in [pool[r].data_ptr()] for j in range(pool.shape[1] * pool.element_size())}
+    assert meets >= bool(mine & theirs)
+    n = src.shape[0]
+    with pytest.raises(ValueError, match="overlap" if meets else "on a GPU"):
+        S.frames_put(src, torch.arange(n), pool)
+    if not meets:
+        return
+    _refused(_lib.load().tone_frames_put(0, src.data_ptr(), S._type(src, ""), src.stride(0), P, n, src.shape[1], pool.data_ptr(),
+                                         S._type(pool, ""), pool.stride(0), pool.shape[0], None), "overlaps")
