@@ -103,6 +103,12 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
+def _fits(*sizes: int) -> None:
+    """Sizes that the library takes as int: ctypes would pass on their low 32 bits."""
+    if max(sizes) > 2 ** 31 - 1:
+        raise ValueError(f"sizes past 2^31 - 1 among {sizes}")
+
+
 # --- pages ------------------------------------------------------------------------------------------------------------
 
 def _check_table(table, page_size: int, n_pages: int) -> None:
@@ -110,6 +116,7 @@ def _check_table(table, page_size: int, n_pages: int) -> None:
     if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 \
             or (table.shape[1] > 1 and table.stride(1) != 1) or table.stride(0) < table.shape[1]:
         raise ValueError("table must be a (rows, width) int32 tensor with unit column stride")
+    _fits(*table.shape, page_size, n_pages)
     if page_size < 1 or n_pages < 1 or table.shape[1] * page_size > 2 ** 31 - 1:
         raise ValueError("page_size and n_pages must be positive and width * page_size below 2^31")
 
@@ -132,6 +139,7 @@ def frames_plan(table, queue, cursors_in, cursors_out, rows_in, rows_out, first,
     _check_table(table, page_size, queue.numel())
     if max_add < 0:
         raise ValueError(f"max_add must not be negative, got {max_add}")
+    _fits(b, max_add)
     if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (b, max_add) or not slots.is_contiguous()):
         raise ValueError(f"slots must be a contiguous ({b}, {max_add}) int64 tensor")
     if status is not None:
@@ -164,6 +172,7 @@ def frames_slots(table, rows, first, begin, count, *, page_size: int, n_pages: i
     _check_table(table, page_size, n_pages)
     if max_count < 0:
         raise ValueError(f"max_count must not be negative, got {max_count}")
+    _fits(b, max_count)
     if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (b, max_count) or not slots.is_contiguous()):
         raise ValueError(f"slots must be a contiguous ({b}, {max_count}) int64 tensor")
     ins = (table, rows, first, begin, count, slots)
@@ -207,6 +216,7 @@ def _check_put(src, pool) -> tuple[int, int, int, int]:
             or (pool.shape[0] > 1 and pool.stride(0) < pool.shape[1]):
         raise ValueError(f"pool must be (rows, {src.shape[-1]}) with unit column stride, got {tuple(pool.shape)}")
     n = src.numel() // src.shape[-1]
+    _fits(src.shape[-1])
     if n > 1 and sstride < src.shape[-1]:
         raise ValueError("src rows must not overlap")
     if n and pool.shape[0] and src.device == pool.device and _meet(src, sstride, n, pool):
@@ -277,6 +287,7 @@ def token_scores(x, tokens=None, k: int = 0, rows=None, stream=None) -> TokenSco
     n = rows.numel() if rows is not None else x_rows
     if tokens is not None and (tokens.dtype != torch.int32 or tokens.shape != shape or not tokens.is_contiguous()):
         raise ValueError(f"tokens must be a contiguous {tuple(shape)} int32 tensor, got {tuple(tokens.shape)} {tokens.dtype}")
+    _fits(vocab)
     k = int(k)
     if not 0 <= k <= min(vocab, MAX_K):
         raise ValueError(f"k must be in 0 .. min(vocab, {MAX_K}), got {k}")
@@ -338,15 +349,18 @@ def ctc_align(x, tokens, token_lens, frame_lens, rows=None, blank: int = C.BLANK
     vocab = int(x.shape[-1])
     if vocab < 1 or (vocab > 1 and x.stride(-1) != 1):
         raise ValueError("x must have unit stride along a vocabulary of at least one entry")
+    _fits(b, frames, vocab)
     if not 0 <= blank < vocab:
         raise ValueError(f"blank {blank} outside the vocabulary of {vocab}")
     dev = _device(x, tokens, token_lens, frame_lens, rows)
     lib = _lib.load()
+    need = lib.tone_ctc_align_workspace(b, frames, most)
+    if need < 0:
+        raise ValueError(f"{frames} frames are too many for one launch")
     with _On(dev, stream, x, tokens, token_lens, frame_lens, rows) as st:
         score = token_lens.new_empty(b, dtype=torch.float32)
         tot = torch.empty_like(score) if total else None
         labels, spans = tokens.new_empty((b, frames)), tokens.new_empty((b, most, 2))
-        need = lib.tone_ctc_align_workspace(b, frames, most)
         ws = tokens.new_empty(need, dtype=torch.uint8) if need else None
         _lib.check(lib.tone_ctc_align(dev.index, x.data_ptr(), typ, stride, bstride, x_rows, _ptr(rows), b, frames, vocab, blank,
                                       tokens.data_ptr(), most, token_lens.data_ptr(), frame_lens.data_ptr(), score.data_ptr(),

@@ -1199,3 +1199,10 @@ def test_put_beside_the_rows_it_reads(src, pool):
     assert torch.equal(b, want)
     with pytest.raises(ValueError, match="overlap"):
         S().frames_put(b[src], slots, b[:, src[1]])
+
+
+def test_align_of_too_many_frames_is_refused():
+    """Before anything is allocated: one frame repeated 2^29 + 1 times."""
+    one = torch.ones(1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="frames"):
+        S().ctc_align(torch.zeros((1, 1, 5), device="cuda").expand(1, 2 ** 29 + 1, 5), one.view(1, 1), one, one, blank=4)

@@ -295,3 +295,29 @@ def test_frames_put_refuses_rows_of_the_pool(i):
         return
     _refused(_lib.load().tone_frames_put(0, src.data_ptr(), S._type(src, ""), src.stride(0), P, n, src.shape[1], pool.data_ptr(),
                                          S._type(pool, ""), pool.stride(0), pool.shape[0], None), "overlaps")
+
+
+def test_sizes_past_31_bits_are_refused():
+    """The library takes them as int, and ctypes would pass on their low 32 bits: 2^32 + 35 entries as 35."""
+    big = 2 ** 32 + 5
+    meta = lambda *shape, dtype=torch.float32: torch.empty(shape, dtype=dtype, device="meta")  # noqa: E731
+    i32, i64 = (lambda *s: meta(*s, dtype=torch.int32)), (lambda *s: meta(*s, dtype=torch.int64))  # noqa: E731
+    calls = [
+        lambda: S.token_scores(meta(1, big)),
+        lambda: S.frames_put(meta(1, big), i64(1), meta(1, big)),
+        lambda: S.ctc_align(meta(1, big, 5), i32(1, 2), i32(1), i32(1), blank=4),
+        lambda: S.ctc_align(meta(1, 6, big), i32(1, 2), i32(1), i32(1), blank=4),
+        lambda: S.ctc_align(meta(9, 5), i32(1, 2), i32(1), i32(1), rows=i64(1, big), blank=4),
+        lambda: S.ctc_align(meta(big, 6, 5), i32(big, 2), i32(big), i32(big), blank=4),
+        lambda: S.frames_plan(**_plan_args(max_add=big)),
+        lambda: S.frames_plan(**_plan_args(queue=i32(big))),
+        lambda: S.frames_plan(**_plan_args(table=i32(big, 3))),
+        lambda: S.frames_plan(**_plan_args(**{n: i32(big) for n in ("rows_in", "rows_out", "first", "length", "keep", "add")})),
+        lambda: S.frames_slots(i32(4, 3), i32(2), i32(2), i32(2), i32(2), page_size=4, n_pages=big, max_count=2),
+        lambda: S.frames_slots(i32(4, 3), i32(2), i32(2), i32(2), i32(2), page_size=big, n_pages=4, max_count=2),
+        lambda: S.frames_slots(i32(4, 3), i32(2), i32(2), i32(2), i32(2), page_size=4, n_pages=4, max_count=big),
+    ]
+    for i, call in enumerate(calls):
+        with pytest.raises(ValueError, match=r"2\^31 - 1"):
+            call()
+            pytest.fail(f"call {i}")
