@@ -234,7 +234,7 @@ int tone_token_scores(int device, const void *x, int type, int64_t stride, int64
  * A sequence no path fits (more tokens and repeats than frames, a token outside the vocabulary or equal to `blank`, -inf
  * on every path) has score and total -inf, labels and spans -1; no frames and no tokens score 0.  NaN and entries of 6e4 and
  * more in size (infinities, the types' lowest values as masks) count as -inf, frames whose row is outside [0, x_rows) as
- * -inf throughout, a total below -1.1e7 as -inf; entries need not be normalized, but a total ends at 3.7e8.  Lengths are
+ * -inf throughout, a total below -1.8e8 as -inf; entries need not be normalized, but a total ends at 3.7e8.  Lengths are
  * clamped to [0, frames] and [0, max_tokens]. */
 #define TONE_ALIGN_MAX_TOKENS 1800
 int64_t tone_ctc_align_workspace(int batch, int frames, int tokens);

@@ -56,10 +56,11 @@ constexpr float kClosed = 6e4f;         // entries of this size and more (masks 
 constexpr int kLeg = 32;                // frames between two refreshes of the waves' overlap, and two marks of the path
 constexpr int kLoaders = 4;             // waves that stage the frames
 constexpr int kBatch = 8;               // loads a loader lane has in flight
-// exponents of probability 0: a factor of 0 takes kShut off, what passed one stays below kNone and counts as 0.  They are
-// held above kZero (and, for entries that are no log probabilities, below -kZero) every 32 frames, and 32 factors from there
-// do not leave 31 bits.
-constexpr int kShut = -(1 << 25), kNone = -(1 << 24), kZero = -(1 << 29);
+// Probability 0 is a mantissa of 0, which no later factor changes.  Its exponent has to stay below every other one, as the
+// largest of a sum's exponents is what its terms are aligned to: a factor of 0 takes kShut off (adding saturates), and every
+// 32 frames it is put to kZero.  Other exponents are held in [kLow, kHigh] there, what is below kLow becoming 0, and move by
+// some 3 million (entries of 6e4) until the next time; kHigh + kShut lies far enough below kLow for that.
+constexpr int kShut = -(1 << 30), kZero = -(1 << 30), kLow = -(1 << 28), kHigh = 1 << 29;
 
 template <int W_, int R_>
 struct Shape {
@@ -99,7 +100,7 @@ struct Prob {
   int e;
 };
 __device__ __forceinline__ Prob prob_of(float v) {
-  if (v == -INFINITY) return {1.f, kShut};
+  if (v == -INFINITY) return {0.f, kShut};
   const float n = rintf(v * 1.44269502f);
   const float f = fmaf(v, 1.92596299e-8f, fmaf(v, 1.44269502f, -n));
   return {__builtin_amdgcn_exp2f(f), (int)n};
@@ -295,7 +296,7 @@ struct Sum {
   float m[SH::R], below_m;
   int e[SH::R], below_e;
   int col[Q];
-  int shut[Q];                          // 0, or kShut where token q must not follow the token before it directly
+  bool apart[Q];                        // token q may follow the token before it directly
 
   struct alignas(16) Two {
     Prob x, y;
@@ -318,10 +319,10 @@ struct Sum {
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < SH::R; ++i) {
-      m[i] = 1.f;
+      m[i] = 0.f;
       e[i] = kZero;
     }
-    below_m = 1.f;
+    below_m = 0.f;
     below_e = kZero;
   }
   __device__ __forceinline__ void first(const Row& r, int base) {      // the first frame
@@ -340,22 +341,26 @@ struct Sum {
       const float fm = q ? m[q ? 2 * q - 1 : 0] : below_m;
       const int fe = q ? e[q ? 2 * q - 1 : 0] : below_e;
       {
-        const int e2 = fe + shut[q], hi = max(max(e[2 * q + 1], e[2 * q]), e2);
-        const float sum = (ldexpf(m[2 * q + 1], e[2 * q + 1] - hi) + ldexpf(m[2 * q], e[2 * q] - hi)) + ldexpf(fm, e2 - hi);
+        const float two = apart[q] ? fm : 0.f;
+        const int e2 = apart[q] ? fe : kZero, hi = max(max(e[2 * q + 1], e[2 * q]), e2);
+        const float sum = (scaled(m[2 * q + 1], e[2 * q + 1], hi) + scaled(m[2 * q], e[2 * q], hi)) + scaled(two, e2, hi);
         m[2 * q + 1] = sum * r.tok[q].m;
-        e[2 * q + 1] = hi + r.tok[q].e;
+        e[2 * q + 1] = __builtin_elementwise_add_sat(hi, r.tok[q].e);
       }
       const int hi = max(e[2 * q], fe);
-      m[2 * q] = (ldexpf(m[2 * q], e[2 * q] - hi) + ldexpf(fm, fe - hi)) * r.blank.m;
-      e[2 * q] = hi + r.blank.e;
+      m[2 * q] = (scaled(m[2 * q], e[2 * q], hi) + scaled(fm, fe, hi)) * r.blank.m;
+      e[2 * q] = __builtin_elementwise_add_sat(hi, r.blank.e);
     }
   }
+  __device__ static __forceinline__ float scaled(float m_, int e_, int hi) { return ldexpf(m_, __builtin_elementwise_sub_sat(e_, hi)); }
   // a frame multiplies a mantissa by 0.7 to 4.3: 32 frames stay far inside fp32
   __device__ __forceinline__ void renormalize() {
 #pragma unroll
     for (int r = 0; r < SH::R; ++r) {
-      e[r] = min(max(e[r] + __builtin_amdgcn_frexp_expf(m[r]), kZero), -kZero);
-      m[r] = __builtin_amdgcn_frexp_mantf(m[r]);
+      const int at = __builtin_elementwise_add_sat(e[r], __builtin_amdgcn_frexp_expf(m[r]));
+      const bool none = m[r] == 0.f || at < kLow;
+      e[r] = none ? kZero : min(at, kHigh);
+      m[r] = none ? 0.f : __builtin_amdgcn_frexp_mantf(m[r]);
     }
   }
 };
@@ -585,7 +590,7 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
   for (int q = 0; q < R / 2; ++q) {
     const int i = (base >> 1) + q;
     st.col[q] = wave < W ? fr.column(i, L) : 0;
-    st.shut[q] = wave < W && i > 0 && i < L && tok[i] == tok[i - 1] ? kShut : 0;
+    st.apart[q] = !(wave < W && i > 0 && i < L && tok[i] == tok[i - 1]);
   }
   st.clear();
   over_frames<SH, true>(
@@ -617,7 +622,7 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
   if (threadIdx.x == 0) {
     const int hi = max(s_end[0].e, s_end[1].e);
     const float sum = ldexpf(s_end[0].m, s_end[0].e - hi) + ldexpf(s_end[1].m, s_end[1].e - hi);
-    p.total[b] = hi < kNone ? -INFINITY : (float)((double)hi * 0.693147180559945309 + (double)logf(sum));
+    p.total[b] = sum == 0.f ? -INFINITY : (float)((double)hi * 0.693147180559945309 + (double)logf(sum));
   }
 }
 

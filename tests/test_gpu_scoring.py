@@ -1206,3 +1206,30 @@ def test_align_of_too_many_frames_is_refused():
     one = torch.ones(1, dtype=torch.int32, device="cuda")
     with pytest.raises(ValueError, match="frames"):
         S().ctc_align(torch.zeros((1, 1, 5), device="cuda").expand(1, 2 ** 29 + 1, 5), one.view(1, 1), one, one, blank=4)
+
+
+@pytest.mark.parametrize("most", [2, 60, 300, 700, 900, 1300])
+def test_align_of_large_entries_and_a_closed_frame(most):
+    """Large entries of either sign make no path out of none: a closed frame or label and too few frames leave both outputs
+    -inf, and an unlikely path that is open is not lost among likely ones that are closed."""
+    frames = 2700
+    tokens = _dev(np.stack([np.arange(most) % 8, np.zeros(most)]), np.int32)
+    lens = _dev([most, most], np.int32)
+    for size in (5.9e4, 40.0, -5.9e4):
+        x = torch.full((2, frames, 9), size, device="cuda")
+        x[0, frames // 3] = float("-inf")              # no way through this frame
+        short = torch.tensor([frames, min(frames, 2 * most - 2)], dtype=torch.int32, device="cuda")      # repeats need a blank between
+        r = S().ctc_align(x, tokens, lens, short, blank=8, total=True)
+        assert r.score.tolist() == [-np.inf] * 2 and r.total.tolist() == [-np.inf] * 2 and bool((r.labels == -1).all())
+    # the blank unlikely and open in every frame, the tokens likely and each closed in its turn: blanks alone are left
+    x = torch.full((1, 1000, 9), 5.9e4, device="cuda")
+    x[:, :, 8] = -5.9e4
+    x[:, 500, :8] = float("-inf")
+    r = S().ctc_align(x, tokens[:1], _dev([0], np.int32), _dev([1000], np.int32), blank=8, total=True)
+    assert float(r.score) == -5.9e7 and abs(float(r.total) + 5.9e7) <= 5.9e7 * 8 * EPS
+    # one token: it lies on either side of the closed frame, the rest are unlikely blanks
+    x[:, :, :8] = -5.9e4
+    x[:, 500, :8] = float("-inf")
+    r = S().ctc_align(x, _dev([[3]], np.int32), _dev([1], np.int32), _dev([1000], np.int32), blank=8, total=True)
+    paths = np.log(500 * 501 / 2 + 499 * 500 / 2)
+    assert float(r.score) == -5.9e7 and abs(float(r.total) + 5.9e7 - paths) <= 5.9e7 * 8 * EPS
