@@ -228,7 +228,9 @@ int tone_token_scores(int device, const void *x, int type, int64_t stride, int64
  *   score  fp32 [batch]                 log probability of the best path; of equal ones the path that, looked at from
  *                                       its end, stays before it moves by one and moves by one before it skips a blank,
  *                                       and that ends in a blank
- *   total  fp32 [batch] or NULL         log of the summed probability of all paths
+ *   total  fp32 [batch] or NULL         log of the summed probability of all paths, off by at most 2^-21 of the
+ *                                       size of their entries (summed over a path, a mean over the paths) before its
+ *                                       last rounding: where a single path counts it can come out as much below score
  *   labels int32 [batch][frames]        the best path's label per frame, `blank` or a token; -1 behind the last frame
  *   spans  int32 [batch][max_tokens][2] each token's frames [begin, end); -1 behind the last token
  * A sequence no path fits (more tokens and repeats than frames, a token outside the vocabulary or equal to `blank`, -inf

@@ -21,13 +21,16 @@
 // each, and then between them by all waves at once: a wave loads the words of its 32 frames and walks them with the state in
 // scalar registers (v_readlane), so no load waits for the state it belongs to.
 //
-// The sum over paths runs in a workgroup of its own, beside the one that finds the best path.  Each state is a 32-bit mantissa
+// The sum over paths runs in a workgroup of its own, beside the one that finds the best path.  Each state is a 64-bit mantissa
 // and a 32-bit exponent of 2 (never a logarithm: no exp and log per state and frame, and no underflow, however unlikely a
-// prefix is): three terms aligned to the largest exponent, added, times the label's probability, itself mantissa and exponent.
+// prefix is): three terms aligned to the largest exponent, added, times the label's probability.  That one is 1 + d times a
+// power of 2 with d in 32 bits, which is off in proportion to the label's log probability and not to 1: rows that are almost
+// sure of their label add up to a total close to 0, and it is right in proportion as well (in 32 bits throughout the same took
+// 5 to 8 % less time, and a total of -1e-2 was off by 0.3 %, one of -1e-6 by all of it).
 //
 // What bounds it is the issue of one wave's instructions, one after the other at some 2.4 ns each: 98 ns per frame with two
 // states per lane and one wave (187 frames and 43 tokens with the trace: 25 us), 102 with four waves, 138 with four states per
-// lane, 172 with eight waves of those (48 phrases of 2000 frames and 700 tokens with their sums: 350 us, 13 MB read).
+// lane, 172 with eight waves of those (48 phrases of 2000 frames and 700 tokens with their sums: 370 us, 13 MB read).
 #include "scoring.h"
 
 #include <algorithm>
@@ -93,17 +96,24 @@ __device__ __forceinline__ double shift_in(double v, double edge) {
   return __hiloint2double(shift_in(__double2hiint(v), __double2hiint(edge)), shift_in(__double2loint(v), __double2loint(edge)));
 }
 
-// a probability e^v as mantissa in [0.7, 1.42) and exponent: v log2 e in two terms, so the mantissa is off by a few 2^-24
-// however large |v| is
+// a probability e^v as (1 + d) 2^e, 1 + d in [0.7, 1.42): v less n ln 2 in two terms (the reduction of Cody and Waite; the first
+// is v itself where n is 0), d by the series of e^r - 1, whose first term left out is below 2^-25 of it.  d is off by two roundings
+// at most, so the factor's logarithm by less than 2^-21 |v|, whatever v is.
 struct Prob {
-  float m;
+  float d;
   int e;
 };
 __device__ __forceinline__ Prob prob_of(float v) {
-  if (v == -INFINITY) return {0.f, kShut};
-  const float n = rintf(v * 1.44269502f);
-  const float f = fmaf(v, 1.92596299e-8f, fmaf(v, 1.44269502f, -n));
-  return {__builtin_amdgcn_exp2f(f), (int)n};
+  if (v == -INFINITY) return {-1.f, kShut};
+  const float n = rintf(v * 1.44269504f);
+  const float r = fmaf(n, 1.90465430e-9f, fmaf(n, -0.693147182f, v));      // ln 2 = 0.693147182 - 1.90465430e-9
+  float c = 1.f / 5040;
+  c = fmaf(c, r, 1.f / 720);
+  c = fmaf(c, r, 1.f / 120);
+  c = fmaf(c, r, 1.f / 24);
+  c = fmaf(c, r, 1.f / 6);
+  c = fmaf(c, r, 0.5f);
+  return {fmaf(r * r, c, r), (int)n};
 }
 
 // What is staged: [2][columns + 1][ahead + 2] entries of 8 bytes, a double (best path) or a Prob (sum); the last column is
@@ -293,7 +303,7 @@ struct Best {
 template <class SH>
 struct Sum {
   static constexpr int Q = SH::R / 2;
-  float m[SH::R], below_m;
+  double m[SH::R], below_m;
   int e[SH::R], below_e;
   int col[Q];
   bool apart[Q];                        // token q may follow the token before it directly
@@ -319,17 +329,17 @@ struct Sum {
   __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int i = 0; i < SH::R; ++i) {
-      m[i] = 0.f;
+      m[i] = 0.0;
       e[i] = kZero;
     }
-    below_m = 0.f;
+    below_m = 0.0;
     below_e = kZero;
   }
   __device__ __forceinline__ void first(const Row& r, int base) {      // the first frame
     if (base == 0) {
-      m[0] = r.blank.m;
+      m[0] = 1.0 + r.blank.d;
       e[0] = r.blank.e;
-      m[1] = r.tok[0].m;
+      m[1] = 1.0 + r.tok[0].d;
       e[1] = r.tok[0].e;
     }
   }
@@ -338,29 +348,29 @@ struct Sum {
     below_e = shift_in(e[SH::R - 1], below_e);
 #pragma unroll
     for (int q = Q - 1; q >= 0; --q) {
-      const float fm = q ? m[q ? 2 * q - 1 : 0] : below_m;
+      const double fm = q ? m[q ? 2 * q - 1 : 0] : below_m;
       const int fe = q ? e[q ? 2 * q - 1 : 0] : below_e;
-      {
-        const float two = apart[q] ? fm : 0.f;
-        const int e2 = apart[q] ? fe : kZero, hi = max(max(e[2 * q + 1], e[2 * q]), e2);
-        const float sum = (scaled(m[2 * q + 1], e[2 * q + 1], hi) + scaled(m[2 * q], e[2 * q], hi)) + scaled(two, e2, hi);
-        m[2 * q + 1] = sum * r.tok[q].m;
-        e[2 * q + 1] = __builtin_elementwise_add_sat(hi, r.tok[q].e);
-      }
+      // from the two states below: what the blank takes, and the token where it may
       const int hi = max(e[2 * q], fe);
-      m[2 * q] = (scaled(m[2 * q], e[2 * q], hi) + scaled(fm, fe, hi)) * r.blank.m;
+      const double sum = scaled(m[2 * q], e[2 * q], hi) + scaled(fm, fe, hi);
+      const double up = apart[q] ? sum : m[2 * q];
+      const int up_e = apart[q] ? hi : e[2 * q], top = max(e[2 * q + 1], up_e);
+      const double all = scaled(m[2 * q + 1], e[2 * q + 1], top) + scaled(up, up_e, top);
+      m[2 * q + 1] = fma(all, (double)r.tok[q].d, all);
+      e[2 * q + 1] = __builtin_elementwise_add_sat(top, r.tok[q].e);
+      m[2 * q] = fma(sum, (double)r.blank.d, sum);
       e[2 * q] = __builtin_elementwise_add_sat(hi, r.blank.e);
     }
   }
-  __device__ static __forceinline__ float scaled(float m_, int e_, int hi) { return ldexpf(m_, __builtin_elementwise_sub_sat(e_, hi)); }
-  // a frame multiplies a mantissa by 0.7 to 4.3: 32 frames stay far inside fp32
+  __device__ static __forceinline__ double scaled(double m_, int e_, int hi) { return ldexp(m_, __builtin_elementwise_sub_sat(e_, hi)); }
+  // a frame multiplies a mantissa by 0.7 to 4.3: 32 frames stay far inside fp64
   __device__ __forceinline__ void renormalize() {
 #pragma unroll
     for (int r = 0; r < SH::R; ++r) {
-      const int at = __builtin_elementwise_add_sat(e[r], __builtin_amdgcn_frexp_expf(m[r]));
-      const bool none = m[r] == 0.f || at < kLow;
+      const int at = __builtin_elementwise_add_sat(e[r], __builtin_amdgcn_frexp_exp(m[r]));
+      const bool none = m[r] == 0.0 || at < kLow;
       e[r] = none ? kZero : min(at, kHigh);
-      m[r] = none ? 0.f : __builtin_amdgcn_frexp_mantf(m[r]);
+      m[r] = none ? 0.0 : __builtin_amdgcn_frexp_mant(m[r]);
     }
   }
 };
@@ -487,13 +497,24 @@ __device__ __forceinline__ int role() {
   return SH::W == 1 && wave < 2 ? 1 - wave : wave;
 }
 
+// what the waves pass on to the next one, by half, wave and state: a double, and behind all of them an int
 template <class SH>
-__device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
+struct Over {
+  static constexpr int kStates = SH::HL * SH::R, kAll = 2 * SH::W * kStates;
+  static constexpr int kBytes = kAll ? kAll * 12 : 16;
+  char* buf;
+  __device__ __forceinline__ double& value(int half, int wave, int i) const { return reinterpret_cast<double*>(buf)[(half * SH::W + wave) * kStates + i]; }
+  __device__ __forceinline__ int& exponent(int half, int wave, int i) const {
+    return reinterpret_cast<int*>(buf + kAll * 8)[(half * SH::W + wave) * kStates + i];
+  }
+};
+
+template <class SH>
+__device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds, Over<SH> over) {
   constexpr int W = SH::W, R = SH::R, HL = SH::HL, kThreads = 64 * (W + kLoaders);
   constexpr int kLegs = 256;             // legs traced between two barriers
   __shared__ double s_end[2];
   __shared__ int s_state[kLegs];
-  __shared__ double s_over[2][W][W > 1 ? HL * R : 1];
   const int lane = threadIdx.x & 63, wave = role<SH>(), base = wave * SH::N + lane * R;
   uint32_t* words = p.words + (int64_t)b * ((p.frames + SH::F - 1) / SH::F) * W * 64;
   uint16_t* came = p.came + (int64_t)b * ((p.frames + kLeg - 1) / kLeg) * SH::kStates;
@@ -533,10 +554,10 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
             if (write) {
               if (lane >= 64 - HL)
 #pragma unroll
-                for (int r = 0; r < R; ++r) s_over[half][wave][(lane - (64 - HL)) * R + r] = st.a[r];
+                for (int r = 0; r < R; ++r) over.value(half, wave, (lane - (64 - HL)) * R + r) = st.a[r];
             } else if (wave > 0 && lane < HL) {
 #pragma unroll
-              for (int r = 0; r < R; ++r) st.a[r] = s_over[half][wave - 1][lane * R + r];
+              for (int r = 0; r < R; ++r) st.a[r] = over.value(half, wave - 1, lane * R + r);
             }
           }
         });
@@ -573,17 +594,20 @@ __device__ void best_path(const AlignArgs& p, int b, int L, int n, char* lds) {
 }
 
 template <class SH>
-__device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
+__device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds, Over<SH> over) {
   constexpr int W = SH::W, R = SH::R, HL = SH::HL;
-  __shared__ Prob s_end[2];
-  __shared__ Prob s_over[2][W][W > 1 ? HL * R : 1];
+  __shared__ double s_end_m[2];
+  __shared__ int s_end_e[2];
   const int lane = threadIdx.x & 63, wave = role<SH>(), base = wave * SH::N + lane * R;
   const int32_t* tok = p.tokens + (int64_t)b * p.most;
   if (n == 0) {
     if (threadIdx.x == 0) p.total[b] = L == 0 ? 0.f : -INFINITY;
     return;
   }
-  if (threadIdx.x < 2) s_end[threadIdx.x] = {0.f, kZero};
+  if (threadIdx.x < 2) {
+    s_end_m[threadIdx.x] = 0.0;
+    s_end_e[threadIdx.x] = kZero;
+  }
   const Frames fr(p, b, n, lds);
   Sum<SH> st;
 #pragma unroll
@@ -601,13 +625,15 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
           if (write) {
             if (lane >= 64 - HL)
 #pragma unroll
-              for (int r = 0; r < R; ++r) s_over[half][wave][(lane - (64 - HL)) * R + r] = {st.m[r], st.e[r]};
+              for (int r = 0; r < R; ++r) {
+                over.value(half, wave, (lane - (64 - HL)) * R + r) = st.m[r];
+                over.exponent(half, wave, (lane - (64 - HL)) * R + r) = st.e[r];
+              }
           } else if (wave > 0 && lane < HL) {
 #pragma unroll
             for (int r = 0; r < R; ++r) {
-              const Prob v = s_over[half][wave - 1][lane * R + r];
-              st.m[r] = v.m;
-              st.e[r] = v.e;
+              st.m[r] = over.value(half, wave - 1, lane * R + r);
+              st.e[r] = over.exponent(half, wave - 1, lane * R + r);
             }
           }
         }
@@ -616,13 +642,21 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds) {
 #pragma unroll
     for (int r = 0; r < R; ++r)
       for (int i = 0; i < 2; ++i)
-        if (base + r == 2 * L - i) s_end[i] = {st.m[r], st.e[r]};
+        if (base + r == 2 * L - i) {
+          s_end_m[i] = st.m[r];
+          s_end_e[i] = st.e[r];
+        }
   }
   __syncthreads();
   if (threadIdx.x == 0) {
-    const int hi = max(s_end[0].e, s_end[1].e);
-    const float sum = ldexpf(s_end[0].m, s_end[0].e - hi) + ldexpf(s_end[1].m, s_end[1].e - hi);
-    p.total[b] = sum == 0.f ? -INFINITY : (float)((double)hi * 0.693147180559945309 + (double)logf(sum));
+    // mantissas are in [0.5, 1): a total close to 0 is the logarithm of a number close to 1, with no exponent to take off it
+    int hi = max(s_end_e[0], s_end_e[1]);
+    double sum = ldexp(s_end_m[0], s_end_e[0] - hi) + ldexp(s_end_m[1], s_end_e[1] - hi);
+    if (sum < 0.70710678) {
+      sum *= 2;
+      --hi;
+    }
+    p.total[b] = sum == 0.0 ? -INFINITY : (float)(hi * 0.693147180559945309 + log(sum));
   }
 }
 
@@ -631,11 +665,12 @@ template <int W, int R>
 __global__ void __launch_bounds__(64 * (W + kLoaders)) align_kernel(AlignArgs p) {
   extern __shared__ __attribute__((aligned(16))) char lds[];
   using SH = Shape<W, R>;
+  __shared__ __attribute__((aligned(16))) char s_over[Over<SH>::kBytes];
   const bool sum = (int)blockIdx.x >= p.batch;
   const int b = sum ? blockIdx.x - p.batch : blockIdx.x;
   const int L = min(max(p.token_lens[b], 0), p.most), n = min(max(p.frame_lens[b], 0), p.frames);
-  if (sum) all_paths<SH>(p, b, L, n, lds);
-  else best_path<SH>(p, b, L, n, lds);
+  if (sum) all_paths<SH>(p, b, L, n, lds, {s_over});
+  else best_path<SH>(p, b, L, n, lds, {s_over});
 }
 
 template <int W, int R>

@@ -1233,3 +1233,52 @@ def test_align_of_large_entries_and_a_closed_frame(most):
     r = S().ctc_align(x, _dev([[3]], np.int32), _dev([1], np.int32), _dev([1000], np.int32), blank=8, total=True)
     paths = np.log(500 * 501 / 2 + 499 * 500 / 2)
     assert float(r.score) == -5.9e7 and abs(float(r.total) + 5.9e7 - paths) <= 5.9e7 * 8 * EPS
+
+
+def _sums(x, tokens, blank):
+    """(score, total) of one sequence: x float64 (F, V), all states of a frame at once, in 64 bits."""
+    lab = np.full(2 * len(tokens) + 1, blank)
+    lab[1::2] = tokens
+    jump = np.zeros(len(lab), bool)
+    jump[3::2] = lab[3::2] != lab[1:-2:2]
+    v = w = np.where(np.arange(len(lab)) < 2, x[0, lab], -np.inf)
+    for row in x[1:]:
+        c = np.full((2, 3, len(lab)), -np.inf)
+        for at, src in ((0, v), (1, w)):
+            c[at, 0], c[at, 1, 1:], c[at, 2, 2:] = src, src[:-1], np.where(jump[2:], src[:-2], -np.inf)
+        h = np.maximum(c[1].max(0), -1e300)
+        with np.errstate(divide="ignore"):
+            w = h + np.log(np.exp(c[1] - h).sum(0)) + row[lab]
+        v = c[0].max(0) + row[lab]
+    return max(v[-1], v[-2]), np.logaddexp(w[-1], w[-2])
+
+
+@pytest.mark.parametrize("f,most,vocab", [(1, 1, 35), (40, 9, 35), (187, 43, 35), (500, 120, 35), (500, 120, 300), (2000, 300, 35), (2000, 700, 35),
+                                          (2300, 1000, 35)])
+@pytest.mark.parametrize("sure", [0.5, 1e-2, 1e-5, 1e-7, 1e-9])
+def test_align_of_confident_rows(f, most, vocab, sure):
+    """Rows that leave about ``sure`` to all but the label said: the total lies close to 0 and has to be right in proportion.
+
+    Each entry's factor e^v is held as 1 + d and a power of 2, d in 32 bits.  With |v| <= ln 2 / 2 the power is 1 and d is off by
+    2 EPS of itself (its last rounding, and four roundings of the rest of its series, which is at most a fifth of it), so the
+    factor's logarithm by 2 EPS |d| / (1 + d) <= 2.4 EPS |v|.  Beyond, two roundings of the reduced argument (EPS / 4 each) and
+    2 EPS of |d| <= 0.42, divided by 1 + d >= 0.7, are below 2 EPS, which is below 6 EPS |v|.  The total is a mean over the paths,
+    weighted by their probability, so it is off by at most 6 EPS of that mean of sum |v|: minus the derivative of the total by a
+    common factor of all entries.  The states are 64 bits wide: at most 8 roundings a frame of the kernel, and as many of the
+    definition evaluated here.  Then one rounding to 32 bits."""
+    rng = np.random.default_rng(f)
+    tokens = rng.integers(0, vocab - 1, most)
+    tokens[tokens >= 34] += 1 if vocab > 35 else 0
+    said = np.full(f, 34)
+    said[((np.arange(most) + 0.5) * f / most).astype(int)] = tokens
+    left = sure * rng.random(f) + 1e-30
+    x = np.log(left)[:, None] + np.log(rng.dirichlet(np.ones(vocab), f) + 1e-30)
+    x[np.arange(f), said] = np.log1p(-left)
+    x = x.astype(np.float32)
+    r = S().ctc_align(_dev(x[None]), _dev(tokens[None], np.int32), _dev([most], np.int32), _dev([f], np.int32), blank=34, total=True)
+    x = x.astype(np.float64)
+    score, total = _sums(x, tokens, 34)
+    assert r.score.item() == np.float32(score)
+    size = (_sums(x * (1 - 1e-4), tokens, 34)[1] - total) / 1e-4
+    tol = 6 * EPS * size * 1.01 + 16 * f * 2.0 ** -53 + EPS * abs(total)
+    assert abs(r.total.item() - total) <= tol, (r.total.item(), total, tol)
