@@ -1282,3 +1282,42 @@ def test_align_of_confident_rows(f, most, vocab, sure):
     size = (_sums(x * (1 - 1e-4), tokens, 34)[1] - total) / 1e-4
     tol = 6 * EPS * size * 1.01 + 16 * f * 2.0 ** -53 + EPS * abs(total)
     assert abs(r.total.item() - total) <= tol, (r.total.item(), total, tol)
+
+
+@pytest.mark.parametrize("most,f", [(170, 230), (700, 760)])
+def test_long_alignment_captured_and_replayed(most, f):
+    """Shapes whose stages need more LDS than a launch has by default, in two graphs with eager calls between."""
+    rng = np.random.default_rng(most)
+    x, tokens, _, _ = _ctc(rng, 2, f, most, 900, 34)
+    xd, td = _dev(x, np.float32), _dev(tokens)
+    lens = _dev([most, most - 7], np.int32), _dev([f, f - 3], np.int32)
+    fn = lambda: S().ctc_align(xd, td, *lens, total=True)  # noqa: E731
+    fn()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=side):
+            out = fn()
+        graphs.append((g, out))
+    torch.cuda.synchronize()
+    for step in range(3):
+        xd.add_(torch.randn_like(xd).mul_(0.1))
+        want = [t.clone() for t in fn()]
+        torch.cuda.synchronize()
+        for g, out in graphs:
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(a, b) for a, b in zip(want, out)), f"replay {step}"
+
+
+def test_store_calls_of_no_streams():
+    store = S().FrameStore(2, 32, page_size=8, vocab=5)
+    assert tuple(store.reserve([], 4).shape) == (0, 4) and tuple(store.append(torch.empty((0, 3, 5), device="cuda"), []).shape) == (0, 3)
+    assert tuple(store.append(torch.empty((2, 0, 5), device="cuda"), [0, 1]).shape) == (2, 0)
+    store.release([])
+    assert tuple(store.slots([], [], []).shape) == (0, 0) and tuple(store.slots([1], [0], [0]).shape) == (1, 0)
+    rows = _rows(6, 5, "fp32", 1).view(2, 3, 5)
+    assert torch.equal(store.pool[store.append(rows, [0, 1])], rows) and store.free_pages == store.n_pages - 2
