@@ -103,10 +103,12 @@ def _ptr(t) -> int:
     return 0 if t is None else t.data_ptr()
 
 
-def _fits(*sizes: int) -> None:
-    """Sizes that the library takes as int: ctypes would pass on their low 32 bits."""
-    if max(sizes) > 2 ** 31 - 1:
-        raise ValueError(f"sizes past 2^31 - 1 among {sizes}")
+_INT_MAX = 2 ** 31 - 1
+
+
+def _too_large(*sizes: int) -> ValueError:
+    """For sizes that the library takes as int: ctypes would pass on their low 32 bits."""
+    return ValueError(f"sizes past 2^31 - 1 among {sizes}")
 
 
 # --- pages ------------------------------------------------------------------------------------------------------------
@@ -116,8 +118,10 @@ def _check_table(table, page_size: int, n_pages: int) -> None:
     if table.dtype != torch.int32 or table.dim() != 2 or table.shape[0] < 1 or table.shape[1] < 1 \
             or (table.shape[1] > 1 and table.stride(1) != 1) or table.stride(0) < table.shape[1]:
         raise ValueError("table must be a (rows, width) int32 tensor with unit column stride")
-    _fits(*table.shape, page_size, n_pages)
-    if page_size < 1 or n_pages < 1 or table.shape[1] * page_size > 2 ** 31 - 1:
+    rows, width = table.shape
+    if rows > _INT_MAX or width > _INT_MAX or page_size > _INT_MAX or n_pages > _INT_MAX:
+        raise _too_large(rows, width, page_size, n_pages)
+    if page_size < 1 or n_pages < 1 or width * page_size > _INT_MAX:
         raise ValueError("page_size and n_pages must be positive and width * page_size below 2^31")
 
 
@@ -139,7 +143,8 @@ def frames_plan(table, queue, cursors_in, cursors_out, rows_in, rows_out, first,
     _check_table(table, page_size, queue.numel())
     if max_add < 0:
         raise ValueError(f"max_add must not be negative, got {max_add}")
-    _fits(b, max_add)
+    if b > _INT_MAX or max_add > _INT_MAX:
+        raise _too_large(b, max_add)
     if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (b, max_add) or not slots.is_contiguous()):
         raise ValueError(f"slots must be a contiguous ({b}, {max_add}) int64 tensor")
     if status is not None:
@@ -172,7 +177,8 @@ def frames_slots(table, rows, first, begin, count, *, page_size: int, n_pages: i
     _check_table(table, page_size, n_pages)
     if max_count < 0:
         raise ValueError(f"max_count must not be negative, got {max_count}")
-    _fits(b, max_count)
+    if b > _INT_MAX or max_count > _INT_MAX:
+        raise _too_large(b, max_count)
     if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (b, max_count) or not slots.is_contiguous()):
         raise ValueError(f"slots must be a contiguous ({b}, {max_count}) int64 tensor")
     ins = (table, rows, first, begin, count, slots)
@@ -212,25 +218,29 @@ def _check_put(src, pool) -> tuple[int, int, int, int]:
     """What :func:`frames_put` asks of its rows and its pool: (type of src, type of the pool, distance of src's rows, rows)."""
     stype, ptype = _type(src, "src"), _type(pool, "pool")
     sstride = _rows_of(src, "src")
-    if pool.dim() != 2 or pool.shape[1] != src.shape[-1] or (pool.shape[1] > 1 and pool.stride(1) != 1) \
-            or (pool.shape[0] > 1 and pool.stride(0) < pool.shape[1]):
-        raise ValueError(f"pool must be (rows, {src.shape[-1]}) with unit column stride, got {tuple(pool.shape)}")
-    n = src.numel() // src.shape[-1]
-    _fits(src.shape[-1])
-    if n > 1 and sstride < src.shape[-1]:
+    vocab = src.shape[-1]
+    if pool.dim() != 2 or pool.shape[1] != vocab or (vocab > 1 and pool.stride(1) != 1) or (pool.shape[0] > 1 and pool.stride(0) < vocab):
+        raise ValueError(f"pool must be (rows, {vocab}) with unit column stride, got {tuple(pool.shape)}")
+    n = src.numel() // vocab
+    if vocab > _INT_MAX:
+        raise _too_large(vocab)
+    if n > 1 and sstride < vocab:
         raise ValueError("src rows must not overlap")
-    if n and pool.shape[0] and src.device == pool.device and _meet(src, sstride, n, pool):
+    # (no entry has more than 4 bytes: most calls need no closer look)
+    at = src.data_ptr() - pool.data_ptr()
+    if -4 * (n * sstride) < at < 4 * (pool.shape[0] * max(pool.stride(0), vocab)) and _meet(src, sstride, n, pool, at):
         raise ValueError("src must not overlap the pool")
     return stype, ptype, sstride, n
 
 
-def _meet(src, sstride: int, n: int, pool) -> bool:
-    """Whether rows of ``src`` (n, sstride entries apart) and the pool share memory; columns side by side in rows of the same
-    length do not."""
+def _meet(src, sstride: int, n: int, pool, at: int) -> bool:
+    """Whether rows of ``src`` (n, sstride entries apart, the first ``at`` bytes behind the pool's) and the pool share memory;
+    columns side by side in rows of the same length do not."""
     vocab, rows = src.shape[-1], pool.shape[0]
+    if n == 0 or rows == 0 or src.device != pool.device:
+        return False
     each, to = src.element_size(), pool.element_size()
     pitch, pool_pitch = sstride * each, pool.stride(0) * to
-    at = src.data_ptr() - pool.data_ptr()
     if at >= (rows - 1) * pool_pitch + vocab * to or at + (n - 1) * pitch + vocab * each <= 0:
         return False
     if n == 1:
@@ -287,7 +297,8 @@ def token_scores(x, tokens=None, k: int = 0, rows=None, stream=None) -> TokenSco
     n = rows.numel() if rows is not None else x_rows
     if tokens is not None and (tokens.dtype != torch.int32 or tokens.shape != shape or not tokens.is_contiguous()):
         raise ValueError(f"tokens must be a contiguous {tuple(shape)} int32 tensor, got {tuple(tokens.shape)} {tokens.dtype}")
-    _fits(vocab)
+    if vocab > _INT_MAX:
+        raise _too_large(vocab)
     k = int(k)
     if not 0 <= k <= min(vocab, MAX_K):
         raise ValueError(f"k must be in 0 .. min(vocab, {MAX_K}), got {k}")
@@ -349,7 +360,8 @@ def ctc_align(x, tokens, token_lens, frame_lens, rows=None, blank: int = C.BLANK
     vocab = int(x.shape[-1])
     if vocab < 1 or (vocab > 1 and x.stride(-1) != 1):
         raise ValueError("x must have unit stride along a vocabulary of at least one entry")
-    _fits(b, frames, vocab)
+    if b > _INT_MAX or frames > _INT_MAX or vocab > _INT_MAX:
+        raise _too_large(b, frames, vocab)
     if not 0 <= blank < vocab:
         raise ValueError(f"blank {blank} outside the vocabulary of {vocab}")
     dev = _device(x, tokens, token_lens, frame_lens, rows)
