@@ -173,7 +173,8 @@ int tone_session_debug_read(tone_session *s, const char *buffer, void *host_dst,
 #define TONE_TYPE_FP16 1
 #define TONE_TYPE_BF16 2
 
-/* status bits of tone_frames_plan (device memory): 0, or the whole call changed nothing */
+/* status bits of tone_frames_plan (device memory): 0, or the whole call took, released and slotted nothing (the new rows of
+ * its requests hold the old ones' pages) */
 #define TONE_FRAMES_NO_PAGES 1     /* more pages to take than were free before the call           */
 #define TONE_FRAMES_ROW_FULL 2     /* a stream would hold more than `width` pages                 */
 #define TONE_FRAMES_BAD_REQUEST 4  /* negative or decreasing counts, a frame past 2^31 - 2, add > max_add, row ids */

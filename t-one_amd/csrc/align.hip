@@ -28,9 +28,11 @@
 // sure of their label add up to a total close to 0, and it is right in proportion as well (in 32 bits throughout the same took
 // 5 to 8 % less time, and a total of -1e-2 was off by 0.3 %, one of -1e-6 by all of it).
 //
-// What bounds it is the issue of one wave's instructions, one after the other at some 2.4 ns each: 98 ns per frame with two
-// states per lane and one wave (187 frames and 43 tokens with the trace: 25 us), 102 with four waves, 138 with four states per
-// lane, 172 with eight waves of those (48 phrases of 2000 frames and 700 tokens with their sums: 370 us, 13 MB read).
+// What bounds it is the issue of one wave's instructions, one after the other at some 2.4 ns each: 91 ns per frame with two
+// states per lane and one wave (187 frames and 43 tokens with the trace: 24.5 us), 97 with four waves (with the sum 102), 131
+// with four states per lane, 171 with eight waves of those (48 phrases of 2000 frames and 700 tokens: 350 us, with their sums
+// 370, 13 MB read).  From 256 workgroups on two of them share a CU: 128 hypotheses of 400 frames and 110 tokens with their sums
+// take 48 us as one does, 192 take 61.
 #include "scoring.h"
 
 #include <algorithm>
@@ -693,9 +695,10 @@ hipError_t launch_as(AlignArgs p, hipStream_t st) {
   return hipGetLastError();
 }
 
-// The fewest states per lane and waves that hold the sequences.  One sequence of 2000 frames: 43 tokens 196 us, 150 (four
-// waves) 203, 400 (four states per lane) 277, 700 (eight waves) 344, 900 (twelve waves) 385, 1300 (eight waves of eight states)
-// 541; 700 tokens on four waves of eight states take 532, 900 on eight of eight 587.
+// The fewest states per lane and waves that hold the sequences.  One sequence of 2000 frames, without and with its sum: 43
+// tokens 189 / 189 us, 150 (four waves) 201 / 209, 400 (four states per lane) 269 / 269, 700 (eight waves) 342 / 367, 900 (twelve
+// waves) 376 / 416, 1300 (eight waves of eight states) 543 / 581; without, 700 tokens on four waves of eight states take 532, 900
+// on eight of eight 587.
 template <class Fn>
 auto by_tokens(int most, Fn&& fn) {
   const int states = 2 * most + 1;

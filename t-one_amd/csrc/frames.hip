@@ -16,7 +16,8 @@
 namespace tone {
 namespace {
 
-// n / d for 0 <= n < 2^31 by one multiplication: m = ceil(2^(31 + l) / d), 2^l >= d (m < 2^32; exact over that range)
+// n / d for 0 <= n < 2^31 by one multiplication (Granlund and Montgomery, division by invariant integers): m = ceil(2^(31 + l)
+// / d), 2^l >= d (m < 2^32; exact over that range)
 struct Divisor {
   uint32_t d, m;
   int s;
@@ -109,7 +110,7 @@ __device__ __forceinline__ Request read_request(const PlanArgs& p, int b) {
 // scan kernel in front of a writing kernel.  blockIdx.x: WAVES / per requests of `per` waves each, so that a request's chain
 // of dependent loads (its row, its pages, its slots) is walked by all of them at once; blockIdx.y: a share of the slots.
 // What bounds it is that chain: everything that does not depend on the sums is loaded in front of them.  4096 streams that
-// append 10 frames each (1.2 MB) take 12.6 us, 96 recordings of up to 18,000 frames (14 MB of slots) 10.6, one stream 5.0.
+// append 10 frames each (1.2 MB) take 12.0 us, 96 recordings of up to 18,000 frames (14 MB of slots) 10.6, one stream 4.6.
 template <int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) plan_kernel(PlanArgs p, int per) {
   __shared__ int64_t part[WAVES][4];
@@ -238,7 +239,7 @@ constexpr int kPutChunk = 256 * kPutEach;
 
 // Entries kPutChunk * blockIdx.x ... of the rows laid end to end: consecutive lanes copy consecutive entries of a row, all of
 // a thread's loads are issued before its first store, and the rows' slots come from LDS.  Memory bounds it: 1.73 M rows of 35
-// fp32 entries into an fp16 pool (377 MB) take 95 us, 4.0 TB/s where a copy reaches 4.5; 40,960 rows fp32 to fp32 5.0 us.
+// fp32 entries into an fp16 pool (377 MB) take 95 us, 4.0 TB/s where a copy reaches 4.5; 40,960 rows fp32 to fp32 4.5 us.
 template <typename S, typename D>
 __global__ void __launch_bounds__(256) put_kernel(const S* __restrict__ src, int64_t src_stride, const int64_t* __restrict__ slots,
                                                   int64_t n, Divisor by_vocab, D* __restrict__ pool, int64_t pool_stride, int64_t pool_rows) {

@@ -26,7 +26,8 @@ struct ScoreArgs {
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
-// e^z for z <= 0 (v_exp_f32; z log2 e is rounded once, so e^z is off by about |z| 2^-24 of its value)
+// e^z for z <= 0 (v_exp_f32; z log2 e is rounded once, so e^z is off by about |z| 2^-24 of its value: ln s, where each
+// term counts as often as it is likely, by 2^-24 of the mean |z|, which is at most the entropy)
 __device__ __forceinline__ float exp_neg(float z) { return __builtin_amdgcn_exp2f(z * kLog2e); }
 
 // total order of the values as integers: larger value = larger integer, -0 and +0 are one value, never INT_MIN or INT_MAX
@@ -99,7 +100,7 @@ __device__ __forceinline__ void write_none(const ScoreArgs& p, int64_t n, int fi
 // entry's rank is counted against all others (the other lanes' registers come by DPP, lane ^ 1 .. 7), so one pass gives the
 // given token's rank and the place of each of the top k, whatever k is, with no selection rounds and no LDS: 8 E^2
 // compares per 8 rows.  They bound it: 40,960 rows of 35 (9.2 MB in and out, 2 us) take 8.2 us at some 700 vector
-// instructions per wave, 187 rows 4.2, of which two are the launch.
+// instructions per wave, 187 rows 4.1, of which two are the launch.
 template <typename T, int E>
 __global__ void __launch_bounds__(256) scores_short_kernel(ScoreArgs p) {
   const int sub = threadIdx.x & 7;
@@ -316,7 +317,7 @@ struct Part {
       }
     }
     // entries above x_t; equal ones count below index t.  A step without any is passed over: a token worth asking for is
-    // among the best (2048 rows over 65,537 entries, bf16: 47 us without tokens, 48 with likely ones, 58 with random ones)
+    // among the best (2048 rows over 65,537 entries, bf16: 47 us without tokens, 48 with likely ones, 56 with random ones)
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
       const int b = base + q * 64 * N;
@@ -397,8 +398,8 @@ struct Part {
 // Longer rows: W waves per row, each a contiguous part of it in 16-byte loads from the first aligned entry on (the entries in
 // front of it and behind the last whole vector are single loads of the first and the last wave), joined in LDS.  2048 rows over
 // 65,537 bf16 entries (268 MB) take 47 us for the entropy alone, 5.7 TB/s, where memory bounds it; the rank of random tokens
-// costs 11 us more and ten alternatives 28, of which each of some 35 insertions per row stalls its wave for half a
-// microsecond.  One row over 65,536 takes 19 us: the first sort, the join and a sixteenth of the row per wave.
+// costs 9 us more and ten alternatives 28, of which each of some 35 insertions per row stalls its wave for half a
+// microsecond.  One row over 65,536 takes 19.5 us: the first sort, the join and a sixteenth of the row per wave.
 template <typename T, int W, int ROWS>
 __global__ void __launch_bounds__(64 * W * ROWS) scores_long_kernel(ScoreArgs p) {
   constexpr int N = Vec<T>::N, Q = 4;
