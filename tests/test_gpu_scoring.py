@@ -1321,3 +1321,20 @@ def test_store_calls_of_no_streams():
     assert tuple(store.slots([], [], []).shape) == (0, 0) and tuple(store.slots([1], [0], [0]).shape) == (1, 0)
     rows = _rows(6, 5, "fp32", 1).view(2, 3, 5)
     assert torch.equal(store.pool[store.append(rows, [0, 1])], rows) and store.free_pages == store.n_pages - 2
+
+
+@pytest.mark.parametrize("f,most", [(8192, 20), (8193, 30), (20000, 40), (9000, 200)])
+def test_align_of_many_frames(f, most):
+    """Paths of more legs than are traced between two barriers (256 of 32 frames)."""
+    rng = np.random.default_rng(f)
+    x, tokens, _, _ = _ctc(rng, 1, f, most, 35, 34)
+    _align_by_rows(rng, x, tokens, np.array([[most, f]], np.int32))
+
+
+def test_plan_of_very_many_streams():
+    rng = np.random.default_rng(5)
+    n = 70001
+    p = Pool(rng, n, 4, 4, 3 * n, head=12345)
+    p.step(rng.permutation(n), np.zeros(n, int), rng.integers(0, 6, n), 5)
+    ids = rng.permutation(n)[: n // 2]
+    p.step(ids, p.length[ids] // 2, rng.integers(0, 6, len(ids)), 5)
