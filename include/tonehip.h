@@ -180,6 +180,9 @@ int tone_session_debug_read(tone_session *s, const char *buffer, void *host_dst,
 #define TONE_FRAMES_BAD_REQUEST 4  /* negative or decreasing counts, a frame past 2^31 - 2, add > max_add, row ids */
 #define TONE_FRAMES_BAD_QUEUE 8    /* the cursors describe no queue of n_pages pages              */
 
+/* the most requests of one tone_frames_plan, whose time grows with their square where they are many */
+#define TONE_FRAMES_MAX_BATCH (1 << 20)
+
 /* Move `batch` streams from the frames [first, length) they hold to [max(first, keep), length + add), 0 <= keep <=
  * length + add: pages of page_size frames that fall out go back to the free queue, missing ones come from it, in batch
  * order.  Pages released by a call can be taken from the next call on.

@@ -109,7 +109,8 @@ __device__ __forceinline__ Request read_request(const PlanArgs& p, int b) {
 // One launch: every workgroup adds up the pages of all requests (24 bytes each, out of L2) to place its own ones, instead of a
 // scan kernel in front of a writing kernel.  blockIdx.x: WAVES / per requests of `per` waves each, so that a request's chain
 // of dependent loads (its row, its pages, its slots) is walked by all of them at once; blockIdx.y: a share of the slots.
-// What bounds it is that chain: everything that does not depend on the sums is loaded in front of them.  4096 streams that
+// All requests are read by every workgroup: 65,536 take 0.86 ms and 262,144 20 ms, so TONE_FRAMES_MAX_BATCH is the end.
+// What bounds fewer is that chain: everything that does not depend on the sums is loaded in front of them.  4096 streams that
 // append 10 frames each (1.2 MB) take 12.0 us, 96 recordings of up to 18,000 frames (14 MB of slots) 10.6, one stream 4.6.
 template <int WAVES>
 __global__ void __launch_bounds__(64 * WAVES) plan_kernel(PlanArgs p, int per) {
@@ -354,7 +355,7 @@ int tone_frames_plan(int device, int32_t* table, int64_t table_stride, int n_row
                      const int32_t* add, int batch, int64_t* slots, int max_add, int32_t* status, void* stream) {
   const char* what = "tone_frames_plan";
   if (batch < 0 || max_add < 0) return refuse(what, "negative batch or max_add");
-  if (max_add > kMaxFrames || batch > kMaxThreads / 128) return refuse(what, "batch or max_add too large for one launch");
+  if (max_add > kMaxFrames || batch > TONE_FRAMES_MAX_BATCH) return refuse(what, "batch or max_add too large for one launch");
   if (!table || !queue || !cursors_in || !cursors_out || !status) return refuse(what, "null table, queue, cursors or status");
   if (batch && (!rows_in || !rows_out || !first || !length || !keep || !add || (max_add && !slots)))
     return refuse(what, "null request array or slots");

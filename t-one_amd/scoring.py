@@ -26,6 +26,7 @@ from . import config as C
 
 MAX_K = 64              # TONE_SCORES_MAX_K
 MAX_TOKENS = 1800       # TONE_ALIGN_MAX_TOKENS
+MAX_BATCH = 1 << 20     # TONE_FRAMES_MAX_BATCH
 STATUS = {1: "out of pages", 2: "a stream's table row is full", 4: "bad request", 8: "bad queue cursors"}   # TONE_FRAMES_*
 
 
@@ -145,6 +146,8 @@ def frames_plan(table, queue, cursors_in, cursors_out, rows_in, rows_out, first,
         raise ValueError(f"max_add must not be negative, got {max_add}")
     if b > _INT_MAX or max_add > _INT_MAX:
         raise _too_large(b, max_add)
+    if b > MAX_BATCH:
+        raise ValueError(f"at most {MAX_BATCH} requests in one plan, got {b}")
     if slots is not None and (slots.dtype != torch.int64 or tuple(slots.shape) != (b, max_add) or not slots.is_contiguous()):
         raise ValueError(f"slots must be a contiguous ({b}, {max_add}) int64 tensor")
     if status is not None:

@@ -321,3 +321,13 @@ def test_sizes_past_31_bits_are_refused():
         with pytest.raises(ValueError, match=r"2\^31 - 1"):
             call()
             pytest.fail(f"call {i}")
+
+
+def test_plans_of_too_many_requests_are_refused():
+    """Every workgroup reads all requests, so the time grows with their square: the last sizes below 2^25 would take minutes."""
+    n = S.MAX_BATCH + 1
+    ids = torch.zeros(n, dtype=torch.int32)
+    with pytest.raises(ValueError, match="requests"):
+        S.frames_plan(**_plan_args(**{k: ids for k in ("rows_in", "rows_out", "first", "length", "keep", "add")}))
+    lib = _lib.load()
+    _refused(lib.tone_frames_plan(0, P, 3, 4, 3, P, 8, 4, P, Q, P, P, P, P, P, P, n, P, 2, P, None), "one launch")
