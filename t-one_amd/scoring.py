@@ -243,7 +243,7 @@ def _meet(src, sstride: int, n: int, pool, at: int) -> bool:
     if n == 0 or rows == 0 or src.device != pool.device:
         return False
     each, to = src.element_size(), pool.element_size()
-    pitch, pool_pitch = sstride * each, pool.stride(0) * to
+    pitch, pool_pitch = sstride * each, max(pool.stride(0), vocab) * to      # (the stride of a single row says nothing)
     if at >= (rows - 1) * pool_pitch + vocab * to or at + (n - 1) * pitch + vocab * each <= 0:
         return False
     if n == 1:

@@ -331,3 +331,14 @@ def test_plans_of_too_many_requests_are_refused():
         S.frames_plan(**_plan_args(**{k: ids for k in ("rows_in", "rows_out", "first", "length", "keep", "add")}))
     lib = _lib.load()
     _refused(lib.tone_frames_plan(0, P, 3, 4, 3, P, 8, 4, P, Q, P, P, P, P, P, P, n, P, 2, P, None), "one launch")
+
+
+def test_frames_put_of_a_pool_of_one_row():
+    """Whose stride says nothing."""
+    b = torch.zeros(20)
+    one, zero = torch.zeros(1, dtype=torch.int64), b.as_strided((1, 5), (0, 1))
+    for src, meets in ((b[5:10].view(1, 5), False), (b[4:9].view(1, 5), True), (b[2:7].as_strided((1, 5), (0, 1)), True), (b[5:10].as_strided((1, 5), (0, 1)), False), (b[6:16].view(2, 5), False)):
+        with pytest.raises(ValueError, match="overlap" if meets else "on a GPU"):
+            S.frames_put(src, one.repeat(src.shape[0]), zero)
+    with pytest.raises(ValueError, match="overlap"):
+        S.frames_put(b[:10].view(2, 5), one.repeat(2), zero)
