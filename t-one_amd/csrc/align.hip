@@ -657,6 +657,9 @@ __device__ void all_paths(const AlignArgs& p, int b, int L, int n, char* lds, Ov
     if (sum < 0.70710678) {
       sum *= 2;
       --hi;
+    } else if (sum > 1.41421356) {
+      sum *= 0.5;
+      ++hi;
     }
     p.total[b] = sum == 0.0 ? -INFINITY : (float)(hi * 0.693147180559945309 + log(sum));
   }
