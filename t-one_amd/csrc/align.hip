@@ -91,9 +91,6 @@ __device__ __forceinline__ void lds_barrier() {
 
 // lane i: lane i - 1's value (wave_shr 1); lane 0 keeps `edge`'s
 __device__ __forceinline__ int shift_in(int v, int edge) { return __builtin_amdgcn_update_dpp(edge, v, 0x138, 0xf, 0xf, false); }
-__device__ __forceinline__ float shift_in(float v, float edge) {
-  return __int_as_float(shift_in(__float_as_int(v), __float_as_int(edge)));
-}
 __device__ __forceinline__ double shift_in(double v, double edge) {
   return __hiloint2double(shift_in(__double2hiint(v), __double2hiint(edge)), shift_in(__double2loint(v), __double2loint(edge)));
 }
